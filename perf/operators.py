@@ -1,0 +1,433 @@
+"""Cases and plain forms of the three operators behind the gated recurrent core and its training step.
+
+  linear  y = act(x w^T + b) + r, and the gradients of x, w and b     (ops.linear_act_fwd / linear_act_bwd)
+  scan    h_t = s(g_t) m_t h_{t-1} + (1 - s(g_t)) v_t over [T, N, H], its backward pass, and its one-token form
+                                                                      (ops.gated_scan_fwd / gated_scan_bwd / gated_scan_step)
+  adamw   AdamW over many tensors, moments in 32 or in 8 bits         (algo.AdamW)
+"""
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+DT = {'bf16': torch.bfloat16, 'f16': torch.float16, 'f32': torch.float32}
+SIZE = {'bf16': 2, 'f16': 2, 'f32': 4}
+ACTS = ('none', 'relu', 'tanh', 'silu', 'gelu')
+BLOCK = 256                    # elements that share a scale where AdamW's moments are held in 8 bits; tensors start at a multiple of it
+LR, BETAS, EPS, DECAY = 3e-4, (0.9, 0.999), 1e-5, 0.01
+
+
+def listed():
+    return [
+        # one step of 32 processes through the gate and value projection of a 512-wide core: what Policy.act pays
+        dict(name='linear act 32x1024x512', op='linear', dtype='bf16', m=32, n=1024, k=512, act='none', bias=True, residual=False,
+             train=False, pad=0),
+        # the NatureCNN feature layer (1568 -> 512) over a rollout of 128 steps x 32 processes, trained in 16 bits
+        dict(name='linear train 4096x512x1568', op='linear', dtype='bf16', m=4096, n=512, k=1568, act='relu', bias=True,
+             residual=False, train=True, pad=0),
+        # the output projection of a wide core over a long batch of trajectories: the largest product
+        dict(name='linear train 16384x2048x2048', op='linear', dtype='bf16', m=16384, n=2048, k=2048, act='silu', bias=True,
+             residual=True, train=True, pad=0),
+        # the same layer evaluated in full precision
+        dict(name='linear f32 4096x1024x512', op='linear', dtype='f32', m=4096, n=1024, k=512, act='gelu', bias=True,
+             residual=True, train=False, pad=0),
+        # a ragged minibatch with odd widths, rows that are slices of wider ones
+        dict(name='linear ragged 1011x390x777', op='linear', dtype='f16', m=1011, n=390, k=777, act='tanh', bias=True,
+             residual=True, train=True, pad=5),
+        # one environment step of 32 processes: the smallest call of all
+        dict(name='scan step 32x512', op='scan', dtype='bf16', t=1, n=32, h=512, step=True),
+        # the recurrent PPO minibatch in full precision: a rollout of 128 steps x 32 processes
+        dict(name='scan f32 128x32x512', op='scan', dtype='f32', t=128, n=32, h=512, step=False),
+        # long trajectories of many processes, wide core
+        dict(name='scan 2048x32x1024', op='scan', dtype='bf16', t=2048, n=32, h=1024, step=False),
+        # one process, very long sequence: few channels, all parallelism is in time
+        dict(name='scan 65536x1x512', op='scan', dtype='bf16', t=65536, n=1, h=512, step=False),
+        # the NatureCNN policy's own tensors, gradients clipped: launch latency counts
+        dict(name='adamw nature', op='adamw', net='nature', layers=1, width=512, bits=32, grad='f32', copy=False, clip=0.5),
+        # a deep wide core with 16-bit weights and gradients, f32 masters and moments
+        dict(name='adamw 32 16x2048', op='adamw', net='core', layers=16, width=2048, bits=32, grad='bf16', copy=True, clip=0.0),
+        # the same in 8 bits, clipped, moments read back
+        dict(name='adamw 8 16x2048', op='adamw', net='core', layers=16, width=2048, bits=8, grad='f32', copy=False, clip=0.5),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(('linear', 'scan', 'adamw'))
+    if op == 'linear':
+        n, k = _log(rng, 8, 4096), _log(rng, 8, 4096)
+        if rng.random() < 0.5:                              # widths as layers have them, the others as they fall
+            n, k = -(-n // 64) * 64, -(-k // 64) * 64
+        m = min(_log(rng, 1, 32768), 16384 * 2048 * 2048 // (n * k))
+        return dict(op=op, dtype=rng.choice(('bf16', 'bf16', 'f16', 'f32')), m=m, n=n, k=k, act=rng.choice(ACTS),
+                    bias=rng.random() < 0.8, residual=rng.random() < 0.5, train=rng.random() < 0.6,
+                    pad=rng.choice((0, 0, 8, rng.randint(1, 40))))
+    if op == 'scan':
+        h, n = _log(rng, 8, 2048), _log(rng, 1, 256)
+        if rng.random() < 0.5:
+            h = -(-h // 64) * 64
+        step = rng.random() < 0.2
+        t = 1 if step else min(_log(rng, 1, 65536), 2048 * 32 * 1024 // (n * h))
+        return dict(op=op, dtype=rng.choice(('bf16', 'bf16', 'f16', 'f32')), t=t, n=n, h=h, step=step)
+    net = rng.choice(('nature', 'core', 'core'))
+    width = _log(rng, 32, 2048)
+    layers = rng.randint(1, 16)
+    return dict(op=op, net=net, layers=layers, width=width, bits=rng.choice((32, 8)), grad=rng.choice(('f32', 'bf16', 'f16')),
+                copy=rng.random() < 0.5, clip=rng.choice((0.0, 0.5)))
+
+
+# ------------------------------------------------------------------------------------------------- inputs
+def _shapes(case):
+    w = case['width']
+    if case['net'] == 'nature':                             # convolutions, feature layer, critic and actor of the Atari policy
+        s = [(32, 4, 8, 8), (32,), (64, 32, 4, 4), (64,), (32, 64, 3, 3), (32,), (w, 1568), (w,), (1, w), (1,), (6, w), (6,)]
+        return s * case['layers']
+    s = []
+    for _ in range(case['layers']):                         # gate and value projection, output projection of a gated core
+        s += [(2 * w, w), (2 * w,), (w, w), (w,)]
+    return s
+
+
+def _offsets(shapes):
+    offs, off = [], 0
+    for s in shapes:
+        offs.append(off)
+        off += -(-math.prod(s) // BLOCK) * BLOCK
+    return offs, off
+
+
+def _gen(seed):
+    g = torch.Generator(device='cuda')
+    g.manual_seed(seed)
+    return lambda *s: torch.randn(*s, device='cuda', generator=g)
+
+
+def prepare(case, seed):
+    rn = _gen(seed)
+    st = dict(case=case)
+    if case['op'] == 'linear':
+        dt, m, n, k, pad = DT[case['dtype']], case['m'], case['n'], case['k'], case['pad']
+        st['x'] = rn(m, k + pad).to(dt)[:, :k]              # pad > 0: the rows are slices of wider ones
+        st['w'] = (rn(n, k) / math.sqrt(k)).to(dt)
+        st['b'] = (0.1 * rn(n)).to(dt) if case['bias'] else None
+        st['r'] = rn(m, n).to(dt) if case['residual'] else None
+        st['dy'] = (0.01 * rn(m, n)).to(dt) if case['train'] else None
+    elif case['op'] == 'scan':
+        dt, t, n, h = DT[case['dtype']], case['t'], case['n'], case['h']
+        proj = rn(t, n, 2 * h)                              # the projection that feeds the scan: gates (slow ones), values
+        proj[..., :h] *= 2.0
+        proj[..., :h] += 2.0
+        st['proj'] = proj.to(dt)
+        st['masks'] = 1.0 - (rn(t, n) > 2.5).float()        # an episode ends every 160 steps or so
+        st['h0'] = 0.5 * rn(n, h)
+        if not case['step']:
+            st['dout'] = (0.01 * rn(t, n, h)).to(dt)
+            st['dlast'] = 0.01 * rn(n, h)
+    else:
+        shapes = _shapes(case)
+        offs, total = _offsets(shapes)
+        gdt = DT[case['grad']]
+        st['p'], st['g'] = torch.zeros(total, device='cuda'), torch.zeros(total, device='cuda', dtype=gdt)
+        for s, o in zip(shapes, offs):
+            c = math.prod(s)
+            st['p'][o:o + c] = 0.02 * rn(c)
+            st['g'][o:o + c] = (1e-3 * rn(c) * torch.exp(rn(c))).to(gdt)      # spread over orders of magnitude
+        st['copy'] = st['p'].to(torch.bfloat16) if case['copy'] else None
+        st['seed'] = seed & 0x7fffffff
+        if own:                                             # the optimiser object that a training program keeps
+            algo, _ = _framework()
+            cut = lambda f: None if f is None else [f[o:o + math.prod(s)].view(s) for s, o in zip(shapes, offs)]
+            st['opt'] = algo.AdamW(cut(st['p']), lr=LR, betas=BETAS, eps=EPS, weight_decay=DECAY, grads=cut(st['g']),
+                                   copies=cut(st['copy']), max_grad_norm=case['clip'] or None, state_bits=case['bits'],
+                                   seed=st['seed'])
+        else:
+            st['t'] = 0
+            if case['bits'] == 32:
+                st['m'], st['v'] = torch.zeros_like(st['p']), torch.zeros_like(st['p'])
+            else:
+                for q in 'mv':
+                    st[q] = torch.zeros(total, device='cuda', dtype=torch.uint8)
+                    st[q + 's'] = torch.zeros(total // BLOCK, 1, device='cuda')
+                st['mtab'], st['vtab'] = _table(True), _table(False)
+    return st
+
+
+def _framework():
+    at = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 'pytorch-a2c-ppo-acktr-gail_amd')
+    if at not in sys.path:
+        sys.path.insert(0, at)
+    from a2c_ppo_acktr import algo, ops
+    return algo, ops
+
+
+# ------------------------------------------------------------------------------------------------- plain forms
+def _act(z, act):
+    if act == 'relu':
+        return z * (z > 0)
+    if act == 'tanh':
+        return torch.tanh(z)
+    if act == 'silu':
+        return z * torch.sigmoid(z)
+    if act == 'gelu':
+        return 0.5 * z * (1 + torch.erf(z * math.sqrt(0.5)))
+    return z
+
+
+def _dact(z, act):
+    if act == 'relu':
+        return (z > 0).to(z.dtype)
+    if act == 'tanh':
+        return 1 - torch.tanh(z) ** 2
+    if act == 'silu':
+        s = torch.sigmoid(z)
+        return s * (1 + z * (1 - s))
+    if act == 'gelu':
+        return 0.5 * (1 + torch.erf(z * math.sqrt(0.5))) + z * torch.exp(-0.5 * z * z) * (1 / math.sqrt(2 * math.pi))
+    return torch.ones_like(z)
+
+
+def _linear(st):
+    c, dt = st['case'], st['x'].dtype
+    x, w = st['x'].float(), st['w'].float()
+    z = x @ w.t()
+    if c['bias']:
+        z = z + st['b'].float()
+    y = _act(z, c['act'])
+    if c['residual']:
+        y = y + st['r'].float()
+    out = dict(y=y.to(dt))
+    if c['train']:
+        dz = st['dy'].float() * _dact(z, c['act']) if c['act'] != 'none' else st['dy'].float()
+        out['dx'], out['dw'] = (dz @ w).to(dt), (dz.t() @ x).to(dt)
+        if c['bias']:
+            out['db'] = dz.sum(0).to(dt)
+    return out
+
+
+def _prefix(a, b):
+    """h_t = a_t h_{t-1} + b_t over the first axis by doubling: log2(T) passes instead of T."""
+    d = 1
+    while d < a.shape[0]:
+        b = torch.cat((b[:d], b[d:] + a[d:] * b[:-d]))
+        a = torch.cat((a[:d], a[d:] * a[:-d]))
+        d *= 2
+    return b
+
+
+def _scan(st):
+    c, dt, h = st['case'], st['proj'].dtype, st['case']['h']
+    g, v = st['proj'][..., :h].float(), st['proj'][..., h:].float()
+    m = st['masks'][..., None]
+    f, nf = torch.sigmoid(g), torch.sigmoid(-g)
+    if c['step']:
+        new = f[0] * (m[0] * st['h0']) + nf[0] * v[0]
+        st['h0'].copy_(new)
+        return dict(out=new.to(dt), state=st['h0'])
+    a, b = m * f, nf * v
+    hs = _prefix(a, torch.cat(((b[0] + a[0] * st['h0'])[None], b[1:])))
+    prev = m * torch.cat((st['h0'][None], hs[:-1]))
+    dout = st['dout'].float()
+    dout = torch.cat((dout[:-1], (dout[-1] + st['dlast'])[None]))
+    nxt = torch.cat((a[1:], torch.zeros_like(a[:1])))       # what multiplies the gradient of the step behind
+    d = _prefix(nxt.flip(0), dout.flip(0)).flip(0)
+    dproj = torch.cat((d * (prev - v) * f * nf, d * nf), -1)
+    return dict(out=hs.to(dt), last=hs[-1], dproj=dproj.to(dt), dh0=a[0] * d[0])
+
+
+def _table(signed):
+    """Values of the 256 codes of a moment in 8 bits, for a scale of 1: 4 exponent bits and a sign, or 5 exponent bits; 3 mantissa bits."""
+    c = torch.arange(256, device='cuda')
+    top = 15 if signed else 31
+    e, k = (c >> 3) & top, (c & 7).float()
+    mag = torch.where(e > 0, torch.ldexp(8 + k, e - 1), k) * 2.0 ** (-2 - top)
+    return torch.where(c > 127, -mag, mag) if signed else mag
+
+
+def _bits(x):
+    """A 32-bit mixing function (multiply and xor-shift), on int32 whose products wrap."""
+    x = (x ^ ((x >> 16) & 0xffff)) * 0x7feb352d
+    x = (x ^ ((x >> 15) & 0x1ffff)) * (0x846ca68b - (1 << 32))
+    return x ^ ((x >> 16) & 0xffff)
+
+
+def _encode(x, rnd, signed):
+    """8-bit codes of x (rows of BLOCK share a power of two as scale), rounded up with the probability that rnd's 20 bits give."""
+    top = 15 if signed else 31
+    x = x.view(-1, BLOCK)
+    e = x.abs().amax(1, keepdim=True).view(torch.int32) >> 23
+    ok = (e > 0) & (e < 253)
+    scale = torch.where(ok, (e + 1) << 23, torch.zeros_like(e)).view(torch.float32)
+    inv = torch.where(ok, (253 - e) << 23, torch.zeros_like(e)).view(torch.float32)
+    y = x * inv
+    a = y.abs()
+    small = a < 2.0 ** (1 - top)
+    b = (torch.where(small, a + 2.0 ** (1 - top), a).view(torch.int32) + rnd.view(-1, BLOCK)) >> 20
+    b = b - ((127 - top) << 3) - small.to(torch.int32) * 8
+    b = torch.where(y < 0, b + 128, b) if signed else torch.where((b == 0) & (y > 0), torch.ones_like(b), b)
+    return b.to(torch.uint8).view(-1), scale
+
+
+def _decode(code, scale, table):
+    return (table[code.int()].view(-1, BLOCK) * scale).view(-1)
+
+
+def _adamw(st):
+    c = st['case']
+    st['t'] += 1
+    t, g = st['t'], st['g'].float()
+    if c['clip']:
+        norm = g.double().square().sum().sqrt()             # a long sum: in 64 bits
+        g = g * (c['clip'] / (norm + 1e-6)).clamp(max=1.0).float()
+    b1, b2 = BETAS
+    if c['bits'] == 32:
+        m, v = st['m'], st['v']
+    else:
+        m, v = _decode(st['m'], st['ms'], st['mtab']), _decode(st['v'], st['vs'], st['vtab'])
+    m = m * b1 + g * (1 - b1)
+    v = v * b2 + (g * g) * (1 - b2)
+    denom = v.sqrt() * (1 / math.sqrt(1 - b2 ** t)) + EPS
+    p = st['p'] * (1 - LR * DECAY) - (m / denom) * (LR / (1 - b1 ** t))
+    st['p'].copy_(p)
+    if c['copy']:
+        st['copy'].copy_(p)
+    if c['bits'] == 32:
+        st['m'], st['v'] = m, v
+    else:
+        key = _bits(torch.full((1,), (st['seed'] + t * 0x9e3779b9 + (1 << 31)) % (1 << 32) - (1 << 31), device='cuda', dtype=torch.int32))
+        rnd = _bits(torch.arange(p.numel(), device='cuda', dtype=torch.int32) ^ key)
+        st['m'], st['ms'] = _encode(m, rnd & 0xfffff, True)
+        st['v'], st['vs'] = _encode(v, (rnd >> 12) & 0xfffff, False)
+        m, v = _decode(st['m'], st['ms'], st['mtab']), _decode(st['v'], st['vs'], st['vtab'])
+    return dict(p=st['p'], m=m, v=v, copy=st['copy'])
+
+
+# ------------------------------------------------------------------------------------------------- one pass
+def run(st):
+    c = st['case']
+    if not own:
+        return {'linear': _linear, 'scan': _scan, 'adamw': _adamw}[c['op']](st)
+    _, ops = _framework()
+    if c['op'] == 'linear':
+        act, x, w = c['act'], st['x'], st['w']
+        pre = None
+        if c['train'] and act != 'none':
+            pre = torch.empty(c['m'], c['n'], dtype=x.dtype, device=x.device)
+        out = dict(y=ops.linear_act_fwd(x, w, st['b'], act=act, residual=st['r'], pre=pre))
+        if c['train']:
+            dx, dw, db = ops.linear_act_bwd(st['dy'], x, w, pre=pre, act=act, need_db=c['bias'])
+            out.update(dx=dx, dw=dw)
+            if c['bias']:
+                out['db'] = db
+        return out
+    if c['op'] == 'scan':
+        h = c['h']
+        gate, value = st['proj'][..., :h], st['proj'][..., h:]
+        if c['step']:
+            return dict(out=ops.gated_scan_step(gate[0], value[0], st['h0'], st['masks'][0]), state=st['h0'])
+        out, last, saved = ops.gated_scan_fwd(gate, value, st['h0'], st['masks'], save=True)
+        dproj = torch.empty_like(st['proj'])
+        _, _, dh0 = ops.gated_scan_bwd(st['dout'], gate, value, st['h0'], st['masks'], saved=saved, dlast=st['dlast'],
+                                       dgate=dproj[..., :h], dvalue=dproj[..., h:])
+        return dict(out=out, last=last, dproj=dproj, dh0=dh0)
+    st['opt'].step()
+    m, v = st['opt'].moments()
+    return dict(p=st['p'], m=m, v=v, copy=st['copy'])
+
+
+# ------------------------------------------------------------------------------------------------- what a pass cannot do without
+def work(case):
+    if case['op'] == 'linear':
+        e, m, n, k = SIZE[case['dtype']], case['m'], case['n'], case['k']
+        b = e * (m * k + n * k + m * n * (2 if case['residual'] else 1) + n * case['bias'])
+        fl = 2.0 * m * n * k
+        if case['train']:                                   # dy read, dx and dw written; x and w are counted above
+            b += e * (m * n + m * k + n * k + n * case['bias'])
+            fl *= 3
+        return dict(bytes=b, flops=fl)
+    if case['op'] == 'scan':
+        e, c = SIZE[case['dtype']], case['n'] * case['h']
+        b = case['t'] * (3 * e * c + 4 * case['n']) + 8 * c
+        if not case['step']:                                # dout read, both gradients written, the state's gradient
+            b += case['t'] * 3 * e * c + 8 * c
+        return dict(bytes=b, flops=case['t'] * c * (10.0 if case['step'] else 30.0))
+    n = sum(math.prod(s) for s in _shapes(case))
+    per = 8 + SIZE[case['grad']] + (2 if case['copy'] else 0) + (16 if case['bits'] == 32 else 4 + 8)   # 8 bits: values read back
+    return dict(bytes=n * per, flops=n * 20.0)
+
+
+# ------------------------------------------------------------------------------------------------- the definitions in 64 bits
+def _exact_linear(case, st):
+    f64 = torch.float64
+    x, w = st['x'].to(f64), st['w'].to(f64)
+    z = torch.matmul(x, w.transpose(0, 1))
+    if st['b'] is not None:
+        z += st['b'].to(f64)
+    act = case['act']
+    sig, cdf = 1 / (1 + torch.exp(-z)), 0.5 * torch.special.erfc(-z / math.sqrt(2))
+    val = dict(none=lambda: z, relu=lambda: z.clamp(min=0), tanh=lambda: z.tanh(), silu=lambda: z * sig, gelu=lambda: z * cdf)[act]()
+    res = {'y': val if st['r'] is None else val + st['r'].to(f64)}
+    if case['train']:
+        slope = dict(none=lambda: torch.ones_like(z), relu=lambda: torch.heaviside(z, torch.zeros_like(z)),
+                     tanh=lambda: 1 / z.cosh() ** 2, silu=lambda: sig + z * sig * (1 - sig),
+                     gelu=lambda: cdf + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi))[act]()
+        dz = st['dy'].to(f64) * slope
+        res['dx'], res['dw'] = torch.matmul(dz, w), torch.matmul(dz.transpose(0, 1), x)
+        if st['b'] is not None:
+            res['db'] = dz.sum(dim=0)
+    return res
+
+
+def _exact_scan(case, st):
+    f64, t, h = torch.float64, case['t'], case['h']
+    gate, val = (q.to(f64) for q in st['proj'].split(h, dim=-1))
+    keep = 1 / (1 + torch.exp(-gate))
+    take = 1 / (1 + torch.exp(gate))
+    mask, cur = st['masks'].to(f64).unsqueeze(-1), st['h0'].to(f64)
+    decay, add = mask * keep, take * val
+    seq = torch.empty_like(add)
+    for i in range(t):                                      # step by step, as the definition reads
+        cur = torch.addcmul(add[i], decay[i], cur)
+        seq[i] = cur
+    if case['step']:
+        return {'out': seq[0], 'state': seq[0]}
+    grad, back = st['dout'].to(f64), torch.empty_like(add)
+    cur = st['dlast'].to(f64)
+    for i in range(t - 1, -1, -1):
+        cur = grad[i] + cur
+        back[i] = cur
+        cur = decay[i] * cur
+    before = torch.empty_like(seq)
+    before[0], before[1:] = st['h0'].to(f64), seq[:-1]
+    dgate = back * (mask * before - val) * keep * take
+    return {'out': seq, 'last': seq[-1], 'dproj': torch.cat([dgate, back * take], dim=-1), 'dh0': cur}
+
+
+def _exact_adamw(case, st):
+    # the first step from moments that are zero; in 8 bits they have no value of their own, and the parameters do not depend on
+    # how the moments are kept afterwards
+    f64 = torch.float64
+    p, g = st['p'].to(f64), st['g'].to(f64)
+    if case['clip']:
+        total = math.sqrt(float((g * g).sum()))
+        g = g * min(1.0, case['clip'] / (total + 1e-6))
+    b1, b2 = BETAS
+    first, second = (1 - b1) * g, (1 - b2) * g * g
+    new = p - LR * DECAY * p - LR * (first / (1 - b1)) / (torch.sqrt(second / (1 - b2)) + EPS)
+    eight = case['bits'] == 8
+    return {'p': new, 'm': None if eight else first, 'v': None if eight else second, 'copy': new if case['copy'] else None}
+
+
+def exact(case, seed):
+    global own
+    was, own = own, False
+    try:
+        st = prepare(case, seed)
+    finally:
+        own = was
+    return {'linear': _exact_linear, 'scan': _exact_scan, 'adamw': _exact_adamw}[case['op']](case, st)
