@@ -242,11 +242,10 @@ def _scan(st):
 
 def _table(signed):
     """Values of the 256 codes of a moment in 8 bits, for a scale of 1: 4 exponent bits and a sign, or 5 exponent bits; 3 mantissa bits."""
-    c = torch.arange(256, device='cuda')
-    top = 15 if signed else 31
-    e, k = (c >> 3) & top, (c & 7).float()
-    mag = torch.where(e > 0, torch.ldexp(8 + k, e - 1), k) * 2.0 ** (-2 - top)
-    return torch.where(c > 127, -mag, mag) if signed else mag
+    top = 15 if signed else 31                              # (Python's powers of two: the device's pow is not exact)
+    code = [(c >> 3 & top, c & 7, c > 127) for c in range(256)]
+    mag = [((8 + k) * 2.0 ** (e - 1) if e else k) * 2.0 ** (-2 - top) for e, k, _ in code]
+    return torch.tensor([-v if signed and n else v for v, (_, _, n) in zip(mag, code)], device='cuda')
 
 
 def _bits(x):
