@@ -542,6 +542,81 @@ int acktr_gru_step_bwd_f32(const float* dout, const float* m_next, float* rzn_dg
                            const float* dgh_next, const float* w_hh_t, float* carry, int last, int N, int H, void* stream);
 int acktr_transpose_f32(const float* src, int rows, int cols, float* dst, void* stream);
 
+/* ---- gated recurrent core (no counterpart in the reference: a recurrent base that is parallel in time beside nn.GRU) ----------
+ * Storage types of the entries below: fp32, bf16 or fp16 (one of the codes for every operand of a call unless said otherwise);
+ * arithmetic, sums and states are fp32, rounded once where they are stored. */
+#define ACKTR_F32 0
+#define ACKTR_BF16 1
+#define ACKTR_F16 2
+
+#define ACKTR_ACT_NONE 0
+#define ACKTR_ACT_RELU 1
+#define ACKTR_ACT_TANH 2
+#define ACKTR_ACT_SILU 3            /* z / (1 + e^-z) */
+#define ACKTR_ACT_GELU 4            /* z Phi(z), Phi the normal distribution function */
+
+/* y[M, N] = act(x[M, K] w[N, K]^T + bias[N]) + residual[M, N]; bias and residual nullable.  pre (nullable, [M, N] of the
+ * storage type's size) receives what the backward pass needs of the pre-activations z = x w^T + bias: the slopes act'(z), as fp32 or,
+ * for 16-bit storage, as 16-bit fixed-point numbers in steps of 2^-14 (-32768: not a number).  ld*: row strides in
+ * elements, at least the row length, below 2^21.  Any alignment and width is taken: operands whose rows do not start at 16-byte
+ * boundaries or are no multiple of 16 bytes long are copied into the workspace first.  M may be 0.  y and pre must not overlap an
+ * input; y may be the residual itself (same pointer and stride).  workspace: ..._workspace_bytes() for the same
+ * operands (it looks at their alignment, not at their values), 16-byte aligned; may be NULL where that is 0. */
+long acktr_linear_act_fwd_workspace_bytes(const void* x, long ldx, const void* w, long ldw, long M, long N, long K, int dtype);
+int acktr_linear_act_fwd(const void* x, long ldx, const void* w, long ldw, const void* bias, const void* residual, long ldr, void* y,
+                         long ldy, void* pre, long ldp, long M, long N, long K, int dtype, int act, void* workspace,
+                         long workspace_bytes, void* stream);
+/* dz = dy act'(z) with the slopes in pre, dx[M, K] = dz w, dw[N, K] = dz^T x, db[N] = sum of dz over rows; dx, dw, db nullable (not computed then; w is
+ * needed for dx only, x for dw only).  dw and db are dense.  dz is rounded to the storage type before the products.  The residual's
+ * gradient is dy itself.  With M = 0, dw and db are zero.  Sums over rows are in a fixed order: results repeat bit for bit. */
+long acktr_linear_act_bwd_workspace_bytes(const void* dy, long lddy, const void* x, long ldx, const void* w, long ldw, const void* pre,
+                                          long ldp, int dx, int dw, int db, long M, long N, long K, int dtype, int act);
+int acktr_linear_act_bwd(const void* dy, long lddy, const void* x, long ldx, const void* w, long ldw, const void* pre, long ldp,
+                         void* dx, long lddx, void* dw, void* db, long M, long N, long K, int dtype, int act, void* workspace,
+                         long workspace_bytes, void* stream);
+
+/* Gated linear recurrence over T steps of N sequences of H channels, f = sigmoid(gate):
+ *   h_t = f_t (m_t h_{t-1}) + (1 - f_t) value_t,  h_{-1} = h0 (fp32 [N, H], nullable: zeros),  m = masks (fp32 [T, N], nullable: ones)
+ * A mask of 0 drops the state before it, finite or not.  out[T, N, H]: the states; last (fp32 [N, H], nullable): the final state,
+ * unrounded.  saved (fp32 [ceil(T / interval), N, H], nullable): the states the backward pass starts from,
+ * interval = acktr_gated_scan_save_interval().  Strides over t and n are in elements, channels are contiguous; out must not overlap
+ * the inputs.  T = 0: last = h0.  workspace: ..._workspace_bytes(), 16-byte aligned (for the backward pass too). */
+int acktr_gated_scan_save_interval(void);
+long acktr_gated_scan_workspace_bytes(long T, long N, long H, int dtype);
+int acktr_gated_scan_fwd(const void* gate, long gate_t, long gate_n, const void* value, long value_t, long value_n, const float* h0,
+                         const float* masks, void* out, long out_t, long out_n, float* last, float* saved, long T, long N, long H,
+                         int dtype, void* workspace, long workspace_bytes, void* stream);
+/* Gradients of a loss whose derivatives are dout (by out) and dlast (by last; fp32 [N, H], nullable): dgate, dvalue, and dh0 (fp32
+ * [N, H], nullable).  saved: from the forward pass; may be NULL up to `interval` steps.  T = 0: dh0 = dlast (zeros without). */
+int acktr_gated_scan_bwd(const void* dout, long dout_t, long dout_n, const void* gate, long gate_t, long gate_n, const void* value,
+                         long value_t, long value_n, const float* h0, const float* masks, const float* saved, const float* dlast,
+                         void* dgate, long dgate_t, long dgate_n, void* dvalue, long dvalue_t, long dvalue_n, float* dh0, long T,
+                         long N, long H, int dtype, void* workspace, long workspace_bytes, void* stream);
+/* One step: state (fp32 [N, H]) is updated in place, out[N, H] receives it rounded.  masks: fp32 [N], nullable. */
+int acktr_gated_scan_step(const void* gate, long gate_n, const void* value, long value_n, float* state, const float* masks, void* out,
+                          long out_n, long N, long H, int dtype, void* stream);
+
+/* AdamW over many tensors (decoupled weight decay; csrc/adamw.hip has the formulas).  `tensors` (device array) lists them;
+ * `chunks` (device array of {tensor, chunk number}, nchunks pairs) cuts each into pieces of acktr_adamw_chunk() elements.  Moments lie
+ * in mom1 / mom2, tensor k's from element tensors[k].state on (a multiple of acktr_adamw_block(), with room for its length rounded
+ * up to that): fp32 (bits = 32) or one byte each (bits = 8) with scales[2 * (element / block)] for mom1 and the odd entries for mom2.
+ * `state` (device, acktr_adamw_state_bytes(), zeroed by the caller): first six doubles lr, beta1, beta2, eps, weight decay, clip norm;
+ * then two int64: steps done, seed.  The call increments the steps.  clip != 0: gradients are scaled by
+ * min(1, clip norm / (2-norm over all + 1e-6)) on the fly; they are only read.  Two calls on one `state` must not overlap. */
+typedef struct acktr_adamw_tensor {
+    void* p; const void* g; void* copy;          /* parameters (updated), gradients, 16-bit copy of the parameters (nullable) */
+    long n; long state;
+    int p_dtype, g_dtype, copy_dtype;
+    int vec;                                     /* bits 0, 1, 2: p, g, copy start at a multiple of four elements */
+} acktr_adamw_tensor;
+int acktr_adamw_chunk(void);
+int acktr_adamw_block(void);
+long acktr_adamw_state_bytes(void);
+int acktr_adamw_step(void* state, const acktr_adamw_tensor* tensors, const int* chunks, long nchunks, void* mom1, void* mom2,
+                     float* scales, int bits, int clip, void* stream);
+/* m[n], v[n] (fp32) = the values that 8-bit moments stand for; n a multiple of acktr_adamw_block(). */
+int acktr_adamw_read_moments(const void* mom1, const void* mom2, const float* scales, float* m, float* v, long n, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

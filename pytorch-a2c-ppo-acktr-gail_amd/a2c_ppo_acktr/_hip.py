@@ -81,6 +81,12 @@ class PrecondJob(ctypes.Structure):
                 ('v_out', c_p), ('OUT', c_i), ('IN', c_i), ('q_g', c_p), ('q_a', c_p)]
 
 
+class AdamwTensor(ctypes.Structure):
+    """struct acktr_adamw_tensor (include/acktr_hip.h)"""
+    _fields_ = [('p', c_p), ('g', c_p), ('copy', c_p), ('n', c_l), ('state', c_l),
+                ('p_dtype', c_i), ('g_dtype', c_i), ('copy_dtype', c_i), ('vec', c_i)]
+
+
 class EigJob(ctypes.Structure):
     """struct acktr_eig_job (include/acktr_hip.h)"""
     _fields_ = [('a_inout_qt', c_p), ('d', c_p), ('n', c_i), ('reserved', c_i)]
@@ -183,6 +189,20 @@ _PROTOS = {
     'acktr_gru_step_fwd_f32': (c_i, [c_p] * 8 + [c_i, c_i, c_p]),
     'acktr_gru_step_bwd_f32': (c_i, [c_p] * 8 + [c_i, c_i, c_i, c_p]),
     'acktr_transpose_f32': (c_i, [c_p, c_i, c_i, c_p, c_p]),
+    'acktr_linear_act_fwd_workspace_bytes': (c_l, [c_p, c_l, c_p, c_l, c_l, c_l, c_l, c_i]),
+    'acktr_linear_act_fwd': (c_i, [c_p, c_l, c_p, c_l, c_p, c_p, c_l, c_p, c_l, c_p, c_l, c_l, c_l, c_l, c_i, c_i, c_p, c_l, c_p]),
+    'acktr_linear_act_bwd_workspace_bytes': (c_l, [c_p, c_l] * 4 + [c_i] * 3 + [c_l] * 3 + [c_i] * 2),
+    'acktr_linear_act_bwd': (c_i, [c_p, c_l] * 5 + [c_p, c_p] + [c_l] * 3 + [c_i] * 2 + [c_p, c_l, c_p]),
+    'acktr_gated_scan_save_interval': (c_i, []),
+    'acktr_gated_scan_workspace_bytes': (c_l, [c_l, c_l, c_l, c_i]),
+    'acktr_gated_scan_fwd': (c_i, [c_p, c_l, c_l] * 2 + [c_p, c_p] + [c_p, c_l, c_l] + [c_p, c_p] + [c_l] * 3 + [c_i, c_p, c_l, c_p]),
+    'acktr_gated_scan_bwd': (c_i, [c_p, c_l, c_l] * 3 + [c_p] * 4 + [c_p, c_l, c_l] * 2 + [c_p] + [c_l] * 3 + [c_i, c_p, c_l, c_p]),
+    'acktr_gated_scan_step': (c_i, [c_p, c_l, c_p, c_l, c_p, c_p, c_p, c_l, c_l, c_l, c_i, c_p]),
+    'acktr_adamw_chunk': (c_i, []),
+    'acktr_adamw_block': (c_i, []),
+    'acktr_adamw_state_bytes': (c_l, []),
+    'acktr_adamw_step': (c_i, [c_p, c_p, c_p, c_l, c_p, c_p, c_p, c_i, c_i, c_p]),
+    'acktr_adamw_read_moments': (c_i, [c_p] * 5 + [c_l, c_p]),
 }
 
 

@@ -447,3 +447,296 @@ def gemm(a, b, out=None, trans_a=False, trans_b=False, alpha=1.0, accumulate=Fal
                                    float(alpha), 1 if accumulate else 0, _hip.cur_stream(a.device))
     _hip.check(rc, 'acktr_gemm_f32')
     return out
+
+
+# ----------------------------------------------------------------------------------------------
+# the gated recurrent core's operators (csrc/linear_act.hip, csrc/gated_scan.hip): bf16, fp16 or fp32 storage, fp32 arithmetic.
+# Rows may be slices of wider ones (only the last axis has to be contiguous).  Scratch memory comes from torch's allocator
+# per call, so calls on several streams, and graphs captured one after the other, do not share any.
+# ----------------------------------------------------------------------------------------------
+DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+LINEAR_ACT = {None: 0, 'none': 0, 'relu': 1, 'tanh': 2, 'silu': 3, 'gelu': 4}
+
+
+class _on(object):
+    """Kernels are launched on the operands' device, whichever device is current."""
+    __slots__ = ('guard',)
+
+    def __init__(self, device):
+        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *a):
+        if self.guard is not None:
+            self.guard.__exit__(*a)
+        return False
+
+
+def _need(t, name, shape, dtype, device):
+    """A GPU operand of the expected shape, type and device whose last axis is contiguous."""
+    if not t.is_cuda:
+        raise RuntimeError('%s must live on the MI355X device (got %s): this package has no CPU path' % (name, t.device))
+    if t.device != device:
+        raise RuntimeError('%s is on %s, expected %s' % (name, t.device, device))
+    if t.dtype != dtype:
+        raise RuntimeError('%s must be %s (got %s)' % (name, dtype, t.dtype))
+    if tuple(t.shape) != tuple(shape):
+        raise RuntimeError('%s must have shape %s (got %s)' % (name, tuple(shape), tuple(t.shape)))
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise RuntimeError("%s: the last axis must be contiguous (stride %d)" % (name, t.stride(-1)))
+    return t.data_ptr()
+
+
+def _rows(t, name, shape, dtype, device):
+    """(pointer, row stride in elements) of a matrix whose rows may be slices of wider ones."""
+    p = _need(t, name, shape, dtype, device)
+    return p, (t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1))
+
+
+def _dense(t, name, shape, dtype, device):
+    p = _need(t, name, shape, dtype, device)
+    if not t.is_contiguous():
+        raise RuntimeError('%s must be contiguous' % name)
+    return p
+
+
+def _dtype_code(t, name):
+    if not isinstance(t, torch.Tensor) or t.dtype not in DTYPE_CODE:
+        raise RuntimeError('%s must be a bfloat16, float16 or float32 tensor (got %s)' % (name, getattr(t, 'dtype', type(t))))
+    if not t.is_cuda:
+        raise RuntimeError('%s must live on the MI355X device (got %s): this package has no CPU path' % (name, t.device))
+    return DTYPE_CODE[t.dtype]
+
+
+def _act_code(act):
+    if act not in LINEAR_ACT:
+        raise RuntimeError('unknown activation %r (one of none, relu, tanh, silu, gelu)' % (act,))
+    return LINEAR_ACT[act]
+
+
+def _span(t):
+    reach = 1
+    for n, s in zip(t.shape, t.stride()):
+        if n == 0:
+            return 0, 0
+        reach += (n - 1) * s
+    p, e = t.data_ptr(), t.element_size()
+    return p, p + reach * e
+
+
+def _no_overlap(a, b, what):
+    """a (to be written) and b (read) share no element."""
+    if a is None or b is None:
+        return
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    if a0 < b1 and b0 < a1:
+        # two column slices of the same rows do not meet although their spans do
+        if a.dim() == b.dim() > 1 and a.stride() == b.stride() and a.element_size() == b.element_size():
+            steps, e = [s for n, s in zip(a.shape[:-1], a.stride()[:-1]) if n > 1], a.element_size()
+            if steps and min(steps) > 0 and (b0 - a0) % e == 0:
+                step = min(steps)
+                d = ((b0 - a0) // e) % step
+                if all(s % step == 0 for s in steps) and d >= a.shape[-1] and d + b.shape[-1] <= step:
+                    return
+        raise RuntimeError('%s must not overlap' % what)
+
+
+def _writable(t, name):
+    """Every element of a tensor that is written has a place of its own (an expanded tensor has not)."""
+    axes = sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1)
+    reach = 1
+    for s, n in axes:
+        if s < reach:
+            raise RuntimeError('%s: its elements share memory (strides %s)' % (name, tuple(t.stride())))
+        reach = s * (n - 1) + reach
+
+
+def _scratch(nbytes, device, what):
+    if nbytes < 0:
+        _hip.check(-1, what)
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def linear_act_fwd(x, w, bias=None, act=None, residual=None, out=None, pre=None):
+    """out = act(x w^T + bias) + residual; x [M, K], w [N, K], bias [N], residual / out / pre [M, N], all of one type (bf16, fp16 or
+    fp32), sums in fp32, rounded once.  act: None, 'relu', 'tanh', 'silu' or 'gelu'.  pre [M, N]: receives
+    what linear_act_bwd needs of the pre-activations (the activation's slopes, encoded).  out may be `residual` itself."""
+    code, act = _dtype_code(x, 'x'), _act_code(act)
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1] or x.shape[1] < 1 or w.shape[0] < 1:
+        raise RuntimeError('linear_act_fwd: x [M, K] and w [N, K] expected, got %s and %s' % (tuple(x.shape), tuple(w.shape)))
+    (M, K), N, dt, dev = x.shape, w.shape[0], x.dtype, x.device
+    given = out is not None
+    if out is None:
+        out = torch.empty(M, N, dtype=dt, device=dev)
+    px, ldx = _rows(x, 'x', (M, K), dt, dev)
+    pw, ldw = _rows(w, 'w', (N, K), dt, dev)
+    py, ldy = _rows(out, 'out', (M, N), dt, dev)
+    pb = _need(bias, 'bias', (N,), dt, dev) if bias is not None else None
+    pr, ldr = _rows(residual, 'residual', (M, N), dt, dev) if residual is not None else (None, 0)
+    pz, ldz = _rows(pre, 'pre', (M, N), dt, dev) if pre is not None else (None, 0)
+    for a, name in ((out if given else None, 'out'), (pre, 'pre')):
+        if a is not None:
+            _writable(a, name)
+            for b in (x, w, bias) + (() if a is out and residual is not None and pr == py and ldr == ldy else (residual,)):
+                _no_overlap(a, b, 'linear_act_fwd: %s and an input' % name)
+    if given:
+        _no_overlap(out, pre, 'linear_act_fwd: out and pre')
+    L = _hip.lib()
+    with _on(dev):
+        nb = L.acktr_linear_act_fwd_workspace_bytes(px, ldx, pw, ldw, M, N, K, code)
+        ws = _scratch(nb, dev, 'acktr_linear_act_fwd')
+        with _Timed('linear_act_fwd', 2.0 * M * N * K):
+            rc = L.acktr_linear_act_fwd(px, ldx, pw, ldw, pb, pr, ldr, py, ldy, pz, ldz, M, N, K, code, act,
+                                        ws.data_ptr() if ws is not None else None, nb, _hip.cur_stream(dev))
+    _hip.check(rc, 'acktr_linear_act_fwd')
+    return out
+
+
+def linear_act_bwd(dy, x, w, pre=None, act=None, dx=None, dw=None, db=None, need_dx=True, need_dw=True, need_db=True):
+    """(dx, dw, db) of linear_act_fwd for dy [M, N] = the derivative by its output (the residual's gradient is dy itself).
+    pre: what the forward pass left there (not needed without an activation).  Gradients that are not needed are None."""
+    code, act = _dtype_code(dy, 'dy'), _act_code(act)
+    if dy.dim() != 2 or x.dim() != 2 or w.dim() != 2 or x.shape[0] != dy.shape[0] or tuple(w.shape) != (dy.shape[1], x.shape[1]):
+        raise RuntimeError('linear_act_bwd: dy [M, N], x [M, K] and w [N, K] expected, got %s, %s and %s'
+                           % (tuple(dy.shape), tuple(x.shape), tuple(w.shape)))
+    (M, N), K, dt, dev = dy.shape, x.shape[1], dy.dtype, dy.device
+    if act and pre is None:
+        raise RuntimeError("linear_act_bwd: an activation's gradient needs `pre` of the forward pass")
+    if not act:
+        pre = None
+    given = [t for t, need in ((dx, need_dx), (dw, need_dw), (db, need_db)) if need and t is not None]
+    new = lambda need, t, *s: torch.empty(*s, dtype=dt, device=dev) if need and t is None else (t if need else None)
+    dx, dw, db = new(need_dx, dx, M, K), new(need_dw, dw, N, K), new(need_db, db, N)
+    pg, ldg = _rows(dy, 'dy', (M, N), dt, dev)
+    px, ldx = _rows(x, 'x', (M, K), dt, dev)
+    pw, ldw = _rows(w, 'w', (N, K), dt, dev)
+    pz, ldz = _rows(pre, 'pre', (M, N), dt, dev) if pre is not None else (None, 0)
+    qx, ldq = _rows(dx, 'dx', (M, K), dt, dev) if dx is not None else (None, 0)
+    qw = _dense(dw, 'dw', (N, K), dt, dev) if dw is not None else None
+    qb = _need(db, 'db', (N,), dt, dev) if db is not None else None
+    for i, a in enumerate(given):
+        _writable(a, 'a gradient')
+        for b in (dy, x, w, pre) + tuple(given[:i]):
+            _no_overlap(a, b, 'linear_act_bwd: a gradient and another operand')
+    L = _hip.lib()
+    with _on(dev):
+        nb = L.acktr_linear_act_bwd_workspace_bytes(pg, ldg, px, ldx, pw, ldw, pz, ldz, dx is not None, dw is not None, db is not None,
+                                                    M, N, K, code, act)
+        ws = _scratch(nb, dev, 'acktr_linear_act_bwd')
+        with _Timed('linear_act_bwd', 2.0 * M * N * K * ((dx is not None) + (dw is not None))):
+            rc = L.acktr_linear_act_bwd(pg, ldg, px, ldx, pw, ldw, pz, ldz, qx, ldq, qw, qb, M, N, K, code, act,
+                                        ws.data_ptr() if ws is not None else None, nb, _hip.cur_stream(dev))
+    _hip.check(rc, 'acktr_linear_act_bwd')
+    return dx, dw, db
+
+
+def _steps(t, name, shape, dtype, device):
+    """(pointer, stride over steps, stride over sequences) of a [T, N, H] operand; axes of one element take a packed stride."""
+    p = _need(t, name, shape, dtype, device)
+    T, N, H = shape
+    return p, (t.stride(0) if T > 1 else N * H), (t.stride(1) if N > 1 else H)
+
+
+def _masks(masks, T, N, dev):
+    if masks is None:
+        return None
+    if masks.dim() == 3 and masks.shape[-1] == 1:
+        masks = masks[..., 0]
+    return _dense(masks, 'masks', (T, N), f32, dev)
+
+
+def gated_scan_fwd(gate, value, h0=None, masks=None, out=None, save=False):
+    """(out, last, saved) of the gated linear recurrence h_t = f_t (m_t h_{t-1}) + (1 - f_t) value_t, f = sigmoid(gate).
+    gate, value, out [T, N, H] (one type; any strides over T and N: halves of one projection, batch-first views); h0 [N, H] fp32 or
+    None (zeros); masks [T, N] or [T, N, 1] fp32 or None (ones): where it is 0 nothing before counts.  last [N, H] fp32: the final
+    state.  save=True: the states that gated_scan_bwd starts from, else None."""
+    code = _dtype_code(gate, 'gate')
+    if gate.dim() != 3 or gate.shape[2] < 1:
+        raise RuntimeError('gated_scan_fwd: gate [T, N, H] expected, got %s' % (tuple(gate.shape),))
+    (T, N, H), dt, dev = gate.shape, gate.dtype, gate.device
+    given = out is not None
+    if out is None:
+        out = torch.empty(T, N, H, dtype=dt, device=dev)
+    pg, pv, po = (_steps(t, n, (T, N, H), dt, dev) for t, n in ((gate, 'gate'), (value, 'value'), (out, 'out')))
+    ph = _dense(h0, 'h0', (N, H), f32, dev) if h0 is not None else None
+    pm = _masks(masks, T, N, dev)
+    if given:
+        _writable(out, 'out')
+        for b in (gate, value, h0, masks):
+            _no_overlap(out, b, 'gated_scan_fwd: out and an input')
+    L = _hip.lib()
+    last = torch.empty(N, H, dtype=f32, device=dev)
+    saved = torch.empty(-(-T // L.acktr_gated_scan_save_interval()), N, H, dtype=f32, device=dev) if save else None
+    with _on(dev):
+        nb = L.acktr_gated_scan_workspace_bytes(T, N, H, code)
+        ws = _scratch(nb, dev, 'acktr_gated_scan_fwd')
+        with _Timed('gated_scan_fwd', 10.0 * T * N * H):
+            rc = L.acktr_gated_scan_fwd(*pg, *pv, ph, pm, *po, last.data_ptr(), saved.data_ptr() if save else None, T, N, H, code,
+                                        ws.data_ptr() if ws is not None else None, nb, _hip.cur_stream(dev))
+    _hip.check(rc, 'acktr_gated_scan_fwd')
+    return out, last, saved
+
+
+def gated_scan_bwd(dout, gate, value, h0=None, masks=None, saved=None, dlast=None, dgate=None, dvalue=None, need_dh0=True):
+    """(dgate, dvalue, dh0) for dout [T, N, H] = the derivative by the states and dlast [N, H] fp32 (or None) by the final one;
+    the other operands are those of gated_scan_fwd(save=True) and what it saved."""
+    code = _dtype_code(gate, 'gate')
+    if gate.dim() != 3 or gate.shape[2] < 1:
+        raise RuntimeError('gated_scan_bwd: gate [T, N, H] expected, got %s' % (tuple(gate.shape),))
+    (T, N, H), dt, dev = gate.shape, gate.dtype, gate.device
+    given = [t for t in (dgate, dvalue) if t is not None]
+    dgate = torch.empty(T, N, H, dtype=dt, device=dev) if dgate is None else dgate
+    dvalue = torch.empty(T, N, H, dtype=dt, device=dev) if dvalue is None else dvalue
+    pd, pg, pv, qg, qv = (_steps(t, n, (T, N, H), dt, dev) for t, n in
+                          ((dout, 'dout'), (gate, 'gate'), (value, 'value'), (dgate, 'dgate'), (dvalue, 'dvalue')))
+    L = _hip.lib()
+    every = L.acktr_gated_scan_save_interval()
+    ph = _dense(h0, 'h0', (N, H), f32, dev) if h0 is not None else None
+    pm = _masks(masks, T, N, dev)
+    ps = _dense(saved, 'saved', (-(-T // every), N, H), f32, dev) if saved is not None and T else None
+    pl = _dense(dlast, 'dlast', (N, H), f32, dev) if dlast is not None else None
+    if T > every and saved is None:
+        raise RuntimeError('gated_scan_bwd: more than %d steps need what gated_scan_fwd(save=True) saved' % every)
+    for a in given:
+        _writable(a, 'a gradient')
+        for b in (dout, gate, value, h0, masks, saved, dlast):
+            _no_overlap(a, b, 'gated_scan_bwd: a gradient and an input')
+    if len(given) == 2:
+        _no_overlap(dgate, dvalue, 'gated_scan_bwd: dgate and dvalue')
+    dh0 = torch.empty(N, H, dtype=f32, device=dev) if need_dh0 else None
+    with _on(dev):
+        nb = L.acktr_gated_scan_workspace_bytes(T, N, H, code)
+        ws = _scratch(nb, dev, 'acktr_gated_scan_bwd')
+        with _Timed('gated_scan_bwd', 20.0 * T * N * H):
+            rc = L.acktr_gated_scan_bwd(*pd, *pg, *pv, ph, pm, ps, pl, *qg, *qv, dh0.data_ptr() if need_dh0 else None, T, N, H, code,
+                                        ws.data_ptr() if ws is not None else None, nb, _hip.cur_stream(dev))
+    _hip.check(rc, 'acktr_gated_scan_bwd')
+    return dgate, dvalue, dh0
+
+
+def gated_scan_step(gate, value, state, masks=None, out=None):
+    """One step of the recurrence: state [N, H] fp32 is updated IN PLACE, the result is returned rounded to gate's type.
+    gate, value, out [N, H]; masks [N] or [N, 1] fp32 or None."""
+    code = _dtype_code(gate, 'gate')
+    if gate.dim() != 2 or gate.shape[1] < 1:
+        raise RuntimeError('gated_scan_step: gate [N, H] expected, got %s' % (tuple(gate.shape),))
+    (N, H), dt, dev = gate.shape, gate.dtype, gate.device
+    given = out is not None
+    if out is None:
+        out = torch.empty(N, H, dtype=dt, device=dev)
+    (pg, gn), (pv, vn), (po, on) = (_rows(t, n, (N, H), dt, dev) for t, n in ((gate, 'gate'), (value, 'value'), (out, 'out')))
+    ps = _dense(state, 'state', (N, H), f32, dev)
+    pm = _masks(masks.reshape(1, -1), 1, N, dev) if masks is not None else None
+    if given:
+        _writable(out, 'out')
+        for b in (gate, value, state, masks):
+            _no_overlap(out, b, 'gated_scan_step: out and an input')
+    for b in (gate, value, masks):
+        _no_overlap(state, b, 'gated_scan_step: state and an input')
+    with _on(dev):
+        rc = _hip.lib().acktr_gated_scan_step(pg, gn, pv, vn, ps, pm, po, on, N, H, code, _hip.cur_stream(dev))
+    _hip.check(rc, 'acktr_gated_scan_step')
+    return out

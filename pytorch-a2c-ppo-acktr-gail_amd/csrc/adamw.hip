@@ -1,0 +1,315 @@
+// AdamW over many tensors:
+//   g <- g min(1, c / (|g| + 1e-6))            (|g|: 2-norm over all tensors; only with a clip)
+//   m <- b1 m + (1 - b1) g,  v <- b2 v + (1 - b2) g^2
+//   p <- p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+// One launch walks all tensors: their elements are cut into chunks of 2048, a table gives each workgroup its chunk.  The step counter
+// and the hyperparameters live in device memory, so a captured launch sequence replays with the right bias corrections.
+//
+// Moments are fp32 or 8-bit.  In 8 bits, 256 elements share a power of two as scale (just above the largest magnitude, so dividing by
+// it is exact) and a value is sign + 4 exponent + 3 mantissa bits (m) or 5 exponent + 3 mantissa bits (v; a running mean of squares
+// spans twice the octaves).  Rounding is stochastic: with b2 = 0.999 a step changes v by at most 0.1 % of its distance to g^2, far
+// below half a code's spacing of 6 %, so rounding to nearest would freeze v; rounding up with the probability of the cut-off bits
+// keeps its expectation.  The random bits are a function of (seed, step, element), so runs repeat.  A positive v never becomes 0:
+// m may survive where v would not, and m / eps is no step.
+#include "half_types.hpp"
+
+#pragma clang fp contract(off)
+
+namespace acktr {
+
+constexpr int AW_THREADS = 256, AW_CHUNK = 2048, AW_BLOCK = 256, AW_PARTIALS = 1024;
+
+// device copy of the optimiser's state that is not per element (acktr_adamw_state_bytes)
+struct AwState {
+    double lr, b1, b2, eps, wd, max_norm;      // written by the host when they change
+    long long step, seed;
+    // written by the first launch of a step for the second
+    float coef, keep, step_size, inv_bc2, b1f, nb1f, b2f, nb2f, epsf;
+    unsigned key;
+    unsigned done;                             // finished workgroups of the norm launch; back at 0 when it ends
+    float norm;
+    double partial[AW_PARTIALS];
+};
+
+__device__ __forceinline__ unsigned mix32(unsigned x) {
+    x = (x ^ (x >> 16)) * 0x7feb352du;
+    x = (x ^ (x >> 15)) * 0x846ca68bu;
+    return x ^ (x >> 16);
+}
+
+// scalars of the next step; one lane
+__device__ __forceinline__ void aw_begin(AwState* st, double sumsq, bool clip) {
+    const long long t = st->step + 1;
+    st->step = t;
+    double c = 1.0;
+    if (clip) {
+        const double norm = sqrt(sumsq);
+        c = st->max_norm / (norm + 1e-6);
+        if (c > 1.0) c = 1.0;                  // (a norm that is not a number stays one)
+        st->norm = (float)norm;
+    }
+    st->coef = (float)c;
+    st->keep = (float)(1.0 - st->lr * st->wd);
+    st->step_size = (float)(st->lr / (1.0 - pow(st->b1, (double)t)));
+    st->inv_bc2 = (float)(1.0 / sqrt(1.0 - pow(st->b2, (double)t)));
+    st->b1f = (float)st->b1;
+    st->nb1f = (float)(1.0 - st->b1);
+    st->b2f = (float)st->b2;
+    st->nb2f = (float)(1.0 - st->b2);
+    st->epsf = (float)st->eps;
+    st->key = mix32((unsigned)st->seed + (unsigned)t * 0x9e3779b9u);
+}
+
+// 4 consecutive values from element i of a tensor of n; nothing behind the end is touched
+template <class T>
+__device__ __forceinline__ f32v4 ld4_as(const void* p, long i, long n, bool vec) {
+    f32v4 r = {0.f, 0.f, 0.f, 0.f};
+    if (vec && i + 4 <= n) {
+        const vec_t<T, 4> v = *reinterpret_cast<const vec_t<T, 4>*>((const T*)p + i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) r[k] = to_f32(v[k]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (i + k < n) r[k] = to_f32(((const T*)p)[i + k]);
+    }
+    return r;
+}
+template <class T>
+__device__ __forceinline__ void st4_as(void* p, long i, long n, bool vec, const f32v4& v) {
+    if (vec && i + 4 <= n) {
+        vec_t<T, 4> o;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = from_f32<T>(v[k]);
+        *reinterpret_cast<vec_t<T, 4>*>((T*)p + i) = o;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (i + k < n) ((T*)p)[i + k] = from_f32<T>(v[k]);
+    }
+}
+__device__ __forceinline__ f32v4 ld4(const void* p, int dt, long i, long n, bool vec) {
+    return dt == ACKTR_F32 ? ld4_as<float>(p, i, n, vec) : dt == ACKTR_BF16 ? ld4_as<__bf16>(p, i, n, vec) : ld4_as<_Float16>(p, i, n, vec);
+}
+__device__ __forceinline__ void st4(void* p, int dt, long i, long n, bool vec, const f32v4& v) {
+    if (dt == ACKTR_F32) st4_as<float>(p, i, n, vec, v);
+    else if (dt == ACKTR_BF16) st4_as<__bf16>(p, i, n, vec, v);
+    else st4_as<_Float16>(p, i, n, vec, v);
+}
+
+__global__ __launch_bounds__(AW_THREADS) void adamw_norm_kernel(AwState* st, const acktr_adamw_tensor* tensors, const int2* chunks, int nchunks) {
+    __shared__ double sm[16];
+    __shared__ bool last;
+    double s = 0.0;
+    for (int q = blockIdx.x; q < nchunks; q += gridDim.x) {
+        const int2 ck = chunks[q];
+        const acktr_adamw_tensor t = tensors[ck.x];
+        const long base = (long)ck.y * AW_CHUNK;
+#pragma unroll
+        for (int k = 0; k < AW_CHUNK / AW_THREADS / 4; ++k) {
+            const long i = base + (k * AW_THREADS + threadIdx.x) * 4;
+            if (i >= t.n) break;
+            const f32v4 g = ld4(t.g, t.g_dtype, i, t.n, t.vec & 2);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s += (double)g[j] * (double)g[j];
+        }
+    }
+    s = block_sum(s, sm);
+    if (threadIdx.x == 0) {
+        __hip_atomic_store(&st->partial[blockIdx.x], s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last = __hip_atomic_fetch_add(&st->done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    // the last workgroup to finish sums the partial sums, always in the same order
+    double v = 0.0;
+    for (int i = threadIdx.x; i < (int)gridDim.x; i += AW_THREADS) v += __hip_atomic_load(&st->partial[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    v = block_sum(v, sm);
+    if (threadIdx.x == 0) {
+        aw_begin(st, v, true);
+        st->done = 0;
+    }
+}
+__global__ void adamw_begin_kernel(AwState* st) { aw_begin(st, 0.0, false); }
+
+// magnitude of a code of `TOP` as largest exponent field, for a scale of 1
+template <int TOP>
+__device__ __forceinline__ float code_value(unsigned c) {
+    const float x = __uint_as_float((c << 20) + ((127u - TOP) << 23));
+    return c < 8 ? 2.f * x - __uint_as_float((128u - TOP) << 23) : x;
+}
+// code of 0 <= y <= 1, rounded up with probability (cut-off bits) / 2^20; below the smallest exponent the codes are evenly spaced
+template <int TOP>
+__device__ __forceinline__ unsigned code_of(float y, unsigned rnd) {
+    const float low = __uint_as_float((128u - TOP) << 23);
+    const bool small = y < low;
+    const unsigned b = (__float_as_uint(small ? y + low : y) + rnd) >> 20;
+    return b - ((127u - TOP) << 3) - (small ? 8u : 0u);
+}
+// power-of-two scale above a block's largest magnitude and its inverse; 0 for a block of zeros (or below 2^-126), a NaN scale marks
+// a block with values that are not finite (or 2^126 and more)
+__device__ __forceinline__ void block_scale(float most, bool bad, float& scale, float& inv) {
+    const unsigned e = __float_as_uint(most) >> 23;
+    const bool ok = e > 0 && e < 253;
+    scale = bad || e >= 253 ? __uint_as_float(0x7fc00000u) : ok ? __uint_as_float((e + 1) << 23) : 0.f;
+    inv = ok && !bad ? __uint_as_float((253 - e) << 23) : 0.f;
+}
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+
+template <int BITS>
+__global__ __launch_bounds__(AW_THREADS) void adamw_update_kernel(const AwState* __restrict__ st, const acktr_adamw_tensor* __restrict__ tensors,
+                                                                  const int2* __restrict__ chunks, void* mom1, void* mom2, float* scales) {
+    const int2 ck = chunks[blockIdx.x];
+    const acktr_adamw_tensor t = tensors[ck.x];
+    const long base = (long)ck.y * AW_CHUNK;
+    const float coef = st->coef, keep = st->keep, step_size = st->step_size, inv_bc2 = st->inv_bc2, epsf = st->epsf;
+    const float b1 = st->b1f, nb1 = st->nb1f, b2 = st->b2f, nb2 = st->nb2f;
+    const unsigned key = st->key;
+    constexpr int IT = AW_CHUNK / AW_THREADS / 4;
+    f32v4 pv[IT], gv[IT];
+    f32v4 mv[IT], vv[IT];
+    unsigned mc[IT], vc[IT];
+    float ms[IT], vs[IT];
+    // all loads of the thread first
+#pragma unroll
+    for (int k = 0; k < IT; ++k) {
+        const long i = base + (k * AW_THREADS + threadIdx.x) * 4, si = t.state + i;      // a wave covers one block of 256 elements
+        if (base + (k * AW_THREADS + (threadIdx.x & ~63)) * 4 >= t.n) break;
+        pv[k] = ld4(t.p, t.p_dtype, i, t.n, t.vec & 1);
+        gv[k] = ld4(t.g, t.g_dtype, i, t.n, t.vec & 2);
+        if (BITS == 32) {
+            mv[k] = *reinterpret_cast<const f32v4*>((const float*)mom1 + si);
+            vv[k] = *reinterpret_cast<const f32v4*>((const float*)mom2 + si);
+        } else {
+            mc[k] = *reinterpret_cast<const unsigned*>((const uint8_t*)mom1 + si);
+            vc[k] = *reinterpret_cast<const unsigned*>((const uint8_t*)mom2 + si);
+            ms[k] = scales[si / AW_BLOCK * 2];
+            vs[k] = scales[si / AW_BLOCK * 2 + 1];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < IT; ++k) {
+        const long i = base + (k * AW_THREADS + threadIdx.x) * 4, si = t.state + i;
+        if (base + (k * AW_THREADS + (threadIdx.x & ~63)) * 4 >= t.n) break;             // the whole wave leaves
+        if (BITS == 8) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const unsigned a = (mc[k] >> (8 * j)) & 255u, b = (vc[k] >> (8 * j)) & 255u;
+                const float x = code_value<15>(a & 127u) * ms[k];
+                mv[k][j] = a & 128u ? -x : x;
+                vv[k][j] = code_value<31>(b) * vs[k];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float g = gv[k][j] * coef;
+            const float m = mv[k][j] * b1 + g * nb1;
+            const float v = vv[k][j] * b2 + (g * g) * nb2;
+            const float denom = sqrtf(v) * inv_bc2 + epsf;
+            pv[k][j] = pv[k][j] * keep - (m / denom) * step_size;
+            mv[k][j] = m;
+            vv[k][j] = v;
+        }
+        st4(t.p, t.p_dtype, i, t.n, t.vec & 1, pv[k]);
+        if (t.copy) st4(t.copy, t.copy_dtype, i, t.n, t.vec & 4, pv[k]);
+        if (BITS == 32) {
+            *reinterpret_cast<f32v4*>((float*)mom1 + si) = mv[k];
+            *reinterpret_cast<f32v4*>((float*)mom2 + si) = vv[k];
+        } else {
+            float mm = 0.f, vm = 0.f;
+            bool bad = false;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (i + j >= t.n) mv[k][j] = 0.f, vv[k][j] = 0.f;    // what lies behind a tensor's end has no state
+                mm = fmaxf(mm, fabsf(mv[k][j]));
+                vm = fmaxf(vm, vv[k][j]);
+                bad = bad || !(fabsf(mv[k][j]) < INFINITY) || !(vv[k][j] < INFINITY);
+            }
+            mm = wave_max(mm);
+            vm = wave_max(vm);
+            bad = __any(bad);
+            float sm, im, sv, iv;
+            block_scale(mm, bad, sm, im);
+            block_scale(vm, bad, sv, iv);
+            unsigned ma = 0, va = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const unsigned r = mix32((unsigned)(si + j) ^ key);
+                const float y = mv[k][j] * im, z = vv[k][j] * iv;
+                unsigned a = code_of<15>(fabsf(y), r & 0xfffffu), b = code_of<31>(z, r >> 12);
+                if (y < 0.f) a += 128u;
+                if (b == 0 && z > 0.f) b = 1;
+                ma |= (bad ? 0u : a) << (8 * j);
+                va |= (bad ? 0u : b) << (8 * j);
+            }
+            *reinterpret_cast<unsigned*>((uint8_t*)mom1 + si) = ma;
+            *reinterpret_cast<unsigned*>((uint8_t*)mom2 + si) = va;
+            if ((threadIdx.x & 63) == 0) {
+                scales[si / AW_BLOCK * 2] = sm;
+                scales[si / AW_BLOCK * 2 + 1] = sv;
+            }
+        }
+    }
+}
+
+// the values that 8-bit moments stand for
+__global__ __launch_bounds__(256) void adamw_read_kernel(const uint8_t* __restrict__ mom1, const uint8_t* __restrict__ mom2,
+                                                         const float* __restrict__ scales, float* __restrict__ m, float* __restrict__ v, long n) {
+    for (long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (long)gridDim.x * 1024) {
+        const unsigned a4 = *reinterpret_cast<const unsigned*>(mom1 + i), b4 = *reinterpret_cast<const unsigned*>(mom2 + i);
+        const float ms = scales[i / AW_BLOCK * 2], vs = scales[i / AW_BLOCK * 2 + 1];
+        f32v4 om, ov;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const unsigned a = (a4 >> (8 * j)) & 255u, b = (b4 >> (8 * j)) & 255u;
+            const float x = code_value<15>(a & 127u) * ms;
+            om[j] = a & 128u ? -x : x;
+            ov[j] = code_value<31>(b) * vs;
+        }
+        *reinterpret_cast<f32v4*>(m + i) = om;
+        *reinterpret_cast<f32v4*>(v + i) = ov;
+    }
+}
+
+}  // namespace acktr
+
+using namespace acktr;
+
+extern "C" int acktr_adamw_chunk(void) { return AW_CHUNK; }
+extern "C" int acktr_adamw_block(void) { return AW_BLOCK; }
+extern "C" long acktr_adamw_state_bytes(void) { return (long)sizeof(AwState); }
+
+extern "C" int acktr_adamw_step(void* state, const acktr_adamw_tensor* tensors, const int* chunks, long nchunks, void* mom1, void* mom2,
+                                float* scales, int bits, int clip, void* stream) {
+    ACKTR_ARG(bits == 32 || bits == 8, "adamw: moments are held in 32 or 8 bits (got %d)", bits);
+    ACKTR_ARG(nchunks >= 0 && nchunks < (1L << 31), "adamw: too many chunks (%ld)", nchunks);
+    ACKTR_ARG(state && (nchunks == 0 || (tensors && chunks && mom1 && mom2)) && (bits == 32 || nchunks == 0 || scales), "adamw: null buffer");
+    ACKTR_ARG((((uintptr_t)state | (uintptr_t)mom1 | (uintptr_t)mom2) & 15) == 0 && (((uintptr_t)tensors | (uintptr_t)chunks) & 7) == 0,
+              "adamw: buffers must be 16-byte aligned");
+    hipStream_t s = (hipStream_t)stream;
+    AwState* st = (AwState*)state;
+    if (clip && nchunks) {
+        adamw_norm_kernel<<<(int)min(nchunks, (long)AW_PARTIALS), AW_THREADS, 0, s>>>(st, tensors, (const int2*)chunks, (int)nchunks);
+    } else {
+        adamw_begin_kernel<<<1, 1, 0, s>>>(st);
+    }
+    ACKTR_LAUNCH_CHECK();
+    if (!nchunks) return 0;
+    if (bits == 32) adamw_update_kernel<32><<<(int)nchunks, AW_THREADS, 0, s>>>(st, tensors, (const int2*)chunks, mom1, mom2, scales);
+    else adamw_update_kernel<8><<<(int)nchunks, AW_THREADS, 0, s>>>(st, tensors, (const int2*)chunks, mom1, mom2, scales);
+    ACKTR_LAUNCH_CHECK();
+    return 0;
+}
+
+extern "C" int acktr_adamw_read_moments(const void* mom1, const void* mom2, const float* scales, float* m, float* v, long n, void* stream) {
+    ACKTR_ARG(n >= 0 && n % AW_BLOCK == 0, "adamw: the moments' length must be a multiple of %d (got %ld)", AW_BLOCK, n);
+    if (n == 0) return 0;
+    ACKTR_ARG(mom1 && mom2 && scales && m && v, "adamw: null buffer");
+    adamw_read_kernel<<<(int)min((n + 1023) / 1024, 8192L), 256, 0, (hipStream_t)stream>>>((const uint8_t*)mom1, (const uint8_t*)mom2, scales, m, v, n);
+    ACKTR_LAUNCH_CHECK();
+    return 0;
+}

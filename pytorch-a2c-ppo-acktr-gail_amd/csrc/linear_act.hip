@@ -1,0 +1,503 @@
+// y = act(x w^T + b) + r with bf16, fp16 or fp32 operands and fp32 sums, and its backward pass:
+//   dz = dy act'(z),  dx = dz w,  dw = dz^T x,  db = sum over rows of dz
+// Three products over the same tile kernel (tile_gemm.hpp), which reads each operand as it lies: forward k | k contiguous, input
+// gradient k | rows, weight gradient rows | rows.
+#include "act_terms.hpp"
+#include "tile_gemm.hpp"
+
+namespace acktr {
+
+struct LinArgs {
+    const void *a, *b;                  // A: M x K, B: N x K
+    long lda, ldb;
+    int M, N, K;
+    void* y;
+    long ldy;
+    const void *bias, *res;             // nullable
+    void* pre;                          // slopes for the backward pass; nullable
+    long ldr, ldp;
+    int act, vec;                       // vec: 16-byte stores of 8 columns are possible everywhere
+    float* slabs;                       // split reduction: fp32 partial products [slices][M][N] instead of y
+    int kslice;                         // k per slice (a multiple of the K step), K without a split
+    int tiles_m, tiles_n;
+};
+
+// act(v + bias) + res for 8 columns n.. of row m, and their stores.  v: the product.
+template <class T, int ACT, bool SLOPE>
+__device__ __forceinline__ void finish8(const LinArgs& p, int m, int n, float (&v)[8]) {
+    typedef vec_t<T, 8> v8;
+    typedef typename SlopeOf<T>::type ST;
+    typedef vec_t<ST, 8> s8;
+    if (p.vec) {                                             // N is a multiple of 8 then
+        if (p.bias) {
+            const v8 b = *reinterpret_cast<const v8*>((const T*)p.bias + n);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] += to_f32(b[i]);
+        }
+        v8 r, y;
+        s8 z;
+        if (p.res) r = *reinterpret_cast<const v8*>((const T*)p.res + (long)m * p.ldr + n);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float slope;
+            float o = act_of<ACT, SLOPE>(v[i], slope);
+            if (p.res) o += to_f32(r[i]);
+            y[i] = from_f32<T>(o);
+            if (SLOPE) {
+                ST c;
+                put_slope(c, slope);
+                z[i] = c;
+            }
+        }
+        *reinterpret_cast<v8*>((T*)p.y + (long)m * p.ldy + n) = y;
+        if (SLOPE) *reinterpret_cast<s8*>((ST*)p.pre + (long)m * p.ldp + n) = z;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (n + i >= p.N) break;
+            float z = v[i], slope;
+            if (p.bias) z += to_f32(((const T*)p.bias)[n + i]);
+            float o = act_of<ACT, SLOPE>(z, slope);
+            if (p.res) o += to_f32(((const T*)p.res)[(long)m * p.ldr + n + i]);
+            ((T*)p.y)[(long)m * p.ldy + n + i] = from_f32<T>(o);
+            if (SLOPE) put_slope(((ST*)p.pre)[(long)m * p.ldp + n + i], slope);
+        }
+    }
+}
+template <class T>
+__device__ __forceinline__ void finish_any(const LinArgs& p, int m, int n, float (&v)[8]) {
+    if (p.pre) {
+        switch (p.act) {
+            case ACKTR_ACT_RELU: finish8<T, ACKTR_ACT_RELU, true>(p, m, n, v); break;
+            case ACKTR_ACT_TANH: finish8<T, ACKTR_ACT_TANH, true>(p, m, n, v); break;
+            case ACKTR_ACT_SILU: finish8<T, ACKTR_ACT_SILU, true>(p, m, n, v); break;
+            case ACKTR_ACT_GELU: finish8<T, ACKTR_ACT_GELU, true>(p, m, n, v); break;
+            default: finish8<T, ACKTR_ACT_NONE, true>(p, m, n, v);
+        }
+    } else {
+        switch (p.act) {
+            case ACKTR_ACT_RELU: finish8<T, ACKTR_ACT_RELU, false>(p, m, n, v); break;
+            case ACKTR_ACT_TANH: finish8<T, ACKTR_ACT_TANH, false>(p, m, n, v); break;
+            case ACKTR_ACT_SILU: finish8<T, ACKTR_ACT_SILU, false>(p, m, n, v); break;
+            case ACKTR_ACT_GELU: finish8<T, ACKTR_ACT_GELU, false>(p, m, n, v); break;
+            default: finish8<T, ACKTR_ACT_NONE, false>(p, m, n, v);
+        }
+    }
+}
+
+// FULL: bias / activation / residual; otherwise the product is stored as it is.
+template <class T, bool AKC, bool BKC, int BM, int BN, int WM, int WN, bool FULL>
+__global__ __launch_bounds__(WM * WN * 64, (BM * BN > 128 * 128 ? WM * WN / 4 : 2)) void linear_tile_kernel(const LinArgs p) {
+    typedef TileGemm<T, AKC, BKC, BM, BN, WM, WN> G;
+    extern __shared__ char smem[];
+    ACKTR_LDS char* sm = (ACKTR_LDS char*)smem;
+    // Neighbouring tiles share operand rows, so each of the 8 L2 caches (workgroups go to them in turn) gets a contiguous piece
+    // of the tile order, and the order walks blocks of 8 row tiles.
+    const int total = p.tiles_m * p.tiles_n, id = blockIdx.x;
+    const int per = (total + 7) / 8, full = total - 8 * (per - 1);            // XCDs 0 .. full-1 have `per` tiles, the others per-1
+    const int x = id & 7, q = id >> 3;
+    const int t = x < full ? x * per + q : full * per + (x - full) * (per - 1) + q;
+    const int band = t / (8 * p.tiles_n), inband = t % (8 * p.tiles_n);
+    const int rows_in = min(8, p.tiles_m - band * 8);
+    const int tm = band * 8 + inband % rows_in, tn = inband / rows_in;
+    const int m0 = tm * BM, n0 = tn * BN;
+    const int k0 = blockIdx.y * p.kslice, k1 = min(p.K, k0 + p.kslice);
+
+    G g;
+    g.run(p.a, p.lda, m0, p.M, p.b, p.ldb, n0, p.N, k0, k1, sm);
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = m0 + (wave / WN) * (BM / WM), wn = n0 + (wave % WN) * (BN / WN);
+    // The accumulators pass through a wave's own piece of LDS (P row blocks at a time) and come back as 8 consecutive columns of a
+    // row, so stores cover whole lines and the epilogue is one loop.  Row pitch + 4 floats: 16 rows meet 16 different bank groups.
+    constexpr int WTN = BN / WN, PITCH = WTN + 4, BLK = 16 * PITCH * 4;
+    constexpr int FIT = G::LDS / (WM * WN) / BLK;
+    constexpr int P = FIT >= G::MI ? G::MI : FIT >= 4 && G::MI % 4 == 0 ? 4 : FIT >= 2 && G::MI % 2 == 0 ? 2 : 1;
+    static_assert(FIT >= 1, "epilogue block");
+    constexpr int LPR = WTN / 8, RPI = 64 / LPR;                              // lanes a row, rows an iteration
+    __syncthreads();
+    ACKTR_LDS float* mine = reinterpret_cast<ACKTR_LDS float*>(sm) + wave * (P * BLK / 4);
+#pragma unroll
+    for (int base = 0; base < G::MI; base += P) {
+#pragma unroll
+        for (int i = 0; i < P; ++i)
+#pragma unroll
+            for (int j = 0; j < G::NI; ++j)
+                *reinterpret_cast<ACKTR_LDS f32v4*>(mine + (i * 16 + (lane & 15)) * PITCH + j * 16 + 4 * (lane >> 4)) = g.acc[base + i][j];
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                    // the wave's own piece: no barrier
+#pragma unroll 1
+        for (int r = lane / LPR; r < P * 16; r += RPI) {
+            const int m = wm + base * 16 + r, n = wn + (lane % LPR) * 8;
+            const f32v4 lo = *reinterpret_cast<ACKTR_LDS f32v4*>(mine + r * PITCH + (lane % LPR) * 8);
+            const f32v4 hi = *reinterpret_cast<ACKTR_LDS f32v4*>(mine + r * PITCH + (lane % LPR) * 8 + 4);
+            if (m >= p.M || n >= p.N) continue;
+            float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            if (p.slabs) {
+                float* s = p.slabs + ((long)blockIdx.y * p.M + m) * p.N + n;
+                if (p.vec) {
+                    *reinterpret_cast<f32v4*>(s) = lo;
+                    *reinterpret_cast<f32v4*>(s + 4) = hi;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (n + i < p.N) s[i] = v[i];
+                }
+            } else if constexpr (FULL) {
+                finish_any<T>(p, m, n, v);
+            } else {
+                finish8<T, ACKTR_ACT_NONE, false>(p, m, n, v);
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+}
+
+// Sum of the slices of a split reduction in slice order, then the epilogue.
+template <class T>
+__global__ __launch_bounds__(256) void linear_slabs_kernel(const LinArgs p, int slices) {
+    const int groups = (p.N + 7) / 8;
+    const long total = (long)p.M * groups;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
+        const int m = (int)(i / groups), n = (int)(i % groups) * 8;
+        const float* s = p.slabs + (long)m * p.N + n;
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (int z = 0; z < slices; ++z, s += (long)p.M * p.N) {
+            if (p.vec) {
+                const f32v4 lo = *reinterpret_cast<const f32v4*>(s), hi = *reinterpret_cast<const f32v4*>(s + 4);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] += lo[j], v[4 + j] += hi[j];
+            } else {
+                for (int j = 0; j < 8 && n + j < p.N; ++j) v[j] += s[j];
+            }
+        }
+        finish_any<T>(p, m, n, v);
+    }
+}
+
+// dst[r][c] = src[r][c] for c < cols, 0 up to ldd: a copy whose rows start at 16-byte boundaries, for operands that do not
+// (an odd width, a slice of a wider row).  It costs one pass over the operand; reading such rows element by element in the
+// product would cost a fetch per element of every tile that uses it.
+template <class T>
+__global__ __launch_bounds__(256) void pack_rows_kernel(const T* __restrict__ src, long lds, int rows, int cols, T* __restrict__ dst, int ldd) {
+    typedef vec_t<T, 16 / sizeof(T)> vv;
+    constexpr int V = 16 / sizeof(T);
+    const int groups = ldd / V;
+    const long total = (long)rows * groups;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
+        const long r = i / groups;
+        const int c = (int)(i % groups) * V;
+        vv o;
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = c + j < cols ? src[r * lds + c + j] : (T)0.f;
+        *reinterpret_cast<vv*>(dst + r * ldd + c) = o;
+    }
+}
+
+// dz = dy slope (ACT; dz null: not wanted; without ACT dz is dy itself) and, per block of rows, the column sums of dz.
+// A thread holds one group of V columns and walks the block's rows in steps of 8; sums[block][N] (nullable).
+template <class T, bool ACT, int V>
+__global__ __launch_bounds__(256) void act_bwd_kernel(const T* __restrict__ dy, long lddy, const void* __restrict__ pre, long ldp,
+                                                      T* __restrict__ dz, long lddz, int M, int N, int rows_per, float* __restrict__ sums) {
+    typedef vec_t<T, V> vv;
+    typedef typename SlopeOf<T>::type ST;
+    typedef vec_t<ST, V> sv;
+    const int cg = threadIdx.x & 31, rg = threadIdx.x >> 5;
+    const int n = (blockIdx.x * 32 + cg) * V;
+    const int r0 = blockIdx.y * rows_per, r1 = min(M, r0 + rows_per);
+    float s[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[i] = 0.f;
+    if (n < N) {
+#pragma unroll 4
+        for (int r = r0 + rg; r < r1; r += 8) {
+            const vv g = *reinterpret_cast<const vv*>(dy + r * lddy + n);
+            sv z;
+            vv o;
+            if (ACT) z = *reinterpret_cast<const sv*>((const ST*)pre + r * ldp + n);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float d = to_f32(g[i]);
+                if (ACT) d *= get_slope(z[i]);
+                s[i] += d;
+                o[i] = from_f32<T>(d);
+            }
+            if (ACT && dz) *reinterpret_cast<vv*>(dz + r * lddz + n) = o;
+        }
+    } else if (ACT && V == 1 && dz && n < lddz) {            // the padding columns of aligned dz rows, which the products read
+        for (int r = r0 + rg; r < r1; r += 8) dz[r * lddz + n] = from_f32<T>(0.f);
+    }
+    if (!sums) return;
+    __shared__ float part[8][32 * V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) part[rg][cg * V + i] = s[i];
+    __syncthreads();
+    for (int c = threadIdx.x; c < 32 * V; c += 256) {
+        const int col = blockIdx.x * 32 * V + c;
+        if (col >= N) continue;
+        float t = 0.f;
+        for (int j = 0; j < 8; ++j) t += part[j][c];
+        sums[(long)blockIdx.y * N + col] = t;
+    }
+}
+// db = sum of the row blocks' sums, 8 partial sums a column (each over every eighth block), in fixed order
+template <class T>
+__global__ __launch_bounds__(256) void col_sums_kernel(const float* __restrict__ sums, int blocks, int N, T* __restrict__ db) {
+    __shared__ float part[8][32];
+    const int c = threadIdx.x & 31, j = threadIdx.x >> 5, col = blockIdx.x * 32 + c;
+    float t = 0.f;
+    if (col < N)
+        for (int b = j; b < blocks; b += 8) t += sums[(long)b * N + col];
+    part[j][c] = t;
+    __syncthreads();
+    if (j == 0 && col < N) {
+        for (int i = 1; i < 8; ++i) t += part[i][c];
+        db[col] = from_f32<T>(t);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------- host side
+constexpr int KSTEP_BYTES = 128, MAX_SLICES = 32, SUM_BLOCKS = 256;
+
+static inline long up(long v, long a) { return (v + a - 1) / a * a; }
+static inline bool rows16(const void* p, long ld, long e) { return ((uintptr_t)p & 15) == 0 && ld * e % 16 == 0; }
+
+// Tile and reduction split of an M x N x K product.
+struct Plan { int bm, bn, slices; long kslice; };
+static Plan plan_of(long M, long N, long K, int e) {
+    const long kt = KSTEP_BYTES / e, steps = (K + kt - 1) / kt;
+    Plan p{64, 64, 1, up(K, kt)};
+    const long t64 = (long)cdiv(M, 64) * cdiv(N, 64);
+    long want = 1;
+    if (t64 < 256 && steps > 8) want = min(min((long)cdiv(512, t64), steps / 4), (long)MAX_SLICES);
+    if (want > 1) {
+        p.kslice = up((steps + want - 1) / want, 1) * kt;
+        p.slices = cdiv(K, p.kslice);
+    }
+    return p;
+}
+
+template <class T, bool AKC, bool BKC, int BM, int BN, int WM, int WN, bool FULL>
+static int launch_tile(LinArgs& p, const Plan& pl, hipStream_t s) {
+    auto kern = linear_tile_kernel<T, AKC, BKC, BM, BN, WM, WN, FULL>;
+    constexpr int lds = TileGemm<T, AKC, BKC, BM, BN, WM, WN>::LDS;
+    if (lds > 65536) {
+        hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) {
+            set_error("linear_act: %d bytes of LDS refused: %s", lds, hipGetErrorString(e));
+            return (int)e;
+        }
+    }
+    p.tiles_m = cdiv(p.M, BM);
+    p.tiles_n = cdiv(p.N, BN);
+    kern<<<dim3((unsigned)(p.tiles_m * p.tiles_n), pl.slices), dim3(WM * WN * 64), lds, s>>>(p);
+    ACKTR_LAUNCH_CHECK();
+    return 0;
+}
+
+// One product with its epilogue; `slabs` holds the slices of a split reduction.
+template <class T, bool AKC, bool BKC, bool FULL>
+static int product(LinArgs p, float* slabs, hipStream_t s) {
+    const Plan pl = plan_of(p.M, p.N, p.K, sizeof(T));
+    p.kslice = (int)pl.kslice;
+    p.slabs = pl.slices > 1 ? slabs : nullptr;
+    const int rc = launch_tile<T, AKC, BKC, 64, 64, 2, 2, FULL>(p, pl, s);
+    if (rc || pl.slices == 1) return rc;
+    linear_slabs_kernel<T><<<min(cdiv((long)p.M * ((p.N + 7) / 8), 256), 2048), 256, 0, s>>>(p, pl.slices);
+    ACKTR_LAUNCH_CHECK();
+    return 0;
+}
+static long slab_bytes(long M, long N, long K, int e) {
+    const Plan pl = plan_of(M, N, K, e);
+    return pl.slices > 1 ? up(4 * M * N * pl.slices, 256) : 0;
+}
+
+template <class T>
+static int pack(const void* src, long lds, int rows, int cols, void* dst, int ldd, hipStream_t s) {
+    pack_rows_kernel<T><<<min(cdiv((long)rows * (ldd * sizeof(T) / 16), 256), 4096), 256, 0, s>>>((const T*)src, lds, rows, cols, (T*)dst, ldd);
+    ACKTR_LAUNCH_CHECK();
+    return 0;
+}
+
+static int check_dims(long M, long K, long N, int dtype, int act) {
+    ACKTR_ARG(dtype_ok(dtype), "linear_act: unknown dtype code %d", dtype);
+    ACKTR_ARG(act >= 0 && act <= ACKTR_ACT_GELU, "linear_act: unknown activation code %d", act);
+    ACKTR_ARG(M >= 0 && N >= 1 && K >= 1, "linear_act: sizes must be M >= 0, N >= 1, K >= 1 (got M %ld, N %ld, K %ld)", M, N, K);
+    ACKTR_ARG(M < (1L << 31) - 256 && N <= (1 << 20) && K <= (1 << 20), "linear_act: M below 2^31 - 256, N and K at most 2^20 (got M %ld, N %ld, K %ld)", M, N, K);
+    ACKTR_ARG((long)cdiv(M, 64) * cdiv(N, 64) < (1L << 31) - 8, "linear_act: too many tiles (M %ld, N %ld)", M, N);
+    return 0;
+}
+static int check_ld(const char* what, long ld, long cols) {
+    ACKTR_ARG(ld >= cols && ld < (1 << 21), "linear_act: row stride of %s must be at least its %ld columns and below 2^21 (got %ld)", what, cols, ld);
+    return 0;
+}
+
+static constexpr int V_OF(int e) { return 16 / e; }
+
+}  // namespace acktr
+
+using namespace acktr;
+
+// Where the parts of a workspace lie (byte offsets; a part that is not needed has no bytes).
+struct FwdSpace { bool px, pw; long x, w, slabs, bytes; };
+static FwdSpace fwd_space(const void* x, long ldx, const void* w, long ldw, long M, long N, long K, int e) {
+    FwdSpace f;
+    const bool whole = K % V_OF(e) == 0;
+    const long kp = up(K, V_OF(e));
+    f.px = !whole || !rows16(x, ldx, e);
+    f.pw = !whole || !rows16(w, ldw, e);
+    f.x = 0;
+    f.w = f.px ? up(M * kp * e, 256) : 0;
+    f.slabs = f.w + (f.pw ? up(N * kp * e, 256) : 0);
+    f.bytes = f.slabs + slab_bytes(M, N, kp, e);
+    return f;
+}
+struct BwdSpace { bool aligned, pdy, px, pw; long dz, x, w, sums, slabs, bytes; };
+static BwdSpace bwd_space(const void* dy, long lddy, const void* x, long ldx, const void* w, long ldw, const void* pre, long ldp, bool dx, bool dw,
+                          bool db, long M, long N, long K, int e, int act) {
+    BwdSpace f;
+    const int V = V_OF(e);
+    const long np = up(N, V), kp = up(K, V);
+    f.aligned = N % V == 0 && rows16(dy, lddy, e) && (act == ACKTR_ACT_NONE || rows16(pre, ldp, e));
+    f.pdy = act == ACKTR_ACT_NONE && (dx || dw) && (N % V != 0 || !rows16(dy, lddy, e));
+    f.px = dw && (K % V != 0 || !rows16(x, ldx, e));
+    f.pw = dx && (K % V != 0 || !rows16(w, ldw, e));
+    f.dz = 0;
+    f.x = act != ACKTR_ACT_NONE || f.pdy ? up(M * np * e, 256) : 0;
+    f.w = f.x + (f.px ? up(M * kp * e, 256) : 0);
+    f.sums = f.w + (f.pw ? up(N * kp * e, 256) : 0);
+    f.slabs = f.sums + (db ? up(4L * SUM_BLOCKS * N, 256) : 0);
+    long most = dx ? slab_bytes(M, K, N, e) : 0;
+    if (dw) most = max(most, slab_bytes(N, K, M, e));
+    f.bytes = f.slabs + most;
+    return f;
+}
+
+extern "C" long acktr_linear_act_fwd_workspace_bytes(const void* x, long ldx, const void* w, long ldw, long M, long N, long K, int dtype) {
+    if (check_dims(M, K, N, dtype, 0)) return -1;
+    return fwd_space(x, ldx, w, ldw, M, N, K, (int)elem_bytes(dtype)).bytes;
+}
+
+extern "C" int acktr_linear_act_fwd(const void* x, long ldx, const void* w, long ldw, const void* bias, const void* residual, long ldr,
+                                    void* y, long ldy, void* pre, long ldp, long M, long N, long K, int dtype, int act,
+                                    void* workspace, long workspace_bytes, void* stream) {
+    if (int rc = check_dims(M, K, N, dtype, act)) return rc;
+    if (check_ld("x", ldx, K) || check_ld("w", ldw, K) || check_ld("y", ldy, N)) return -1;
+    if ((residual && check_ld("residual", ldr, N)) || (pre && check_ld("pre", ldp, N))) return -1;
+    ACKTR_ARG(M == 0 || (x && w && y), "linear_act_fwd: x, w and y are required");
+    if (M == 0) return 0;
+    const FwdSpace sp = fwd_space(x, ldx, w, ldw, M, N, K, (int)elem_bytes(dtype));
+    ACKTR_ARG(workspace_bytes >= sp.bytes && ((uintptr_t)workspace & 15) == 0 && (workspace || !sp.bytes),
+              "linear_act_fwd: workspace of %ld bytes, %ld with 16-byte alignment are needed", workspace_bytes, sp.bytes);
+    hipStream_t s = (hipStream_t)stream;
+    return with_dtype(dtype, [&](auto t) -> int {
+        typedef decltype(t) T;
+        constexpr int e = sizeof(T);
+        LinArgs p{};
+        p.a = x, p.lda = ldx, p.b = w, p.ldb = ldw;
+        p.M = (int)M, p.N = (int)N, p.K = (int)K;
+        p.y = y, p.ldy = ldy, p.bias = bias, p.res = residual, p.ldr = ldr, p.pre = pre, p.ldp = ldp, p.act = act;
+        p.vec = N % 8 == 0 && rows16(y, ldy, e) && (!bias || ((uintptr_t)bias & 15) == 0) && (!residual || rows16(residual, ldr, e)) &&
+                (!pre || rows16(pre, ldp, e));
+        char* ws = (char*)workspace;
+        const int kp = (int)up(K, V_OF(e));
+        if (sp.px) {
+            if (int rc = pack<T>(x, ldx, (int)M, (int)K, ws + sp.x, kp, s)) return rc;
+            p.a = ws + sp.x, p.lda = kp;
+        }
+        if (sp.pw) {
+            if (int rc = pack<T>(w, ldw, (int)N, (int)K, ws + sp.w, kp, s)) return rc;
+            p.b = ws + sp.w, p.ldb = kp;
+        }
+        p.K = kp;
+        return product<T, true, true, true>(p, (float*)(ws + sp.slabs), s);
+    });
+}
+
+extern "C" long acktr_linear_act_bwd_workspace_bytes(const void* dy, long lddy, const void* x, long ldx, const void* w, long ldw,
+                                                     const void* pre, long ldp, int dx, int dw, int db, long M, long N, long K, int dtype,
+                                                     int act) {
+    if (check_dims(M, K, N, dtype, act)) return -1;
+    return bwd_space(dy, lddy, x, ldx, w, ldw, pre, ldp, dx != 0, dw != 0, db != 0, M, N, K, (int)elem_bytes(dtype), act).bytes;
+}
+
+extern "C" int acktr_linear_act_bwd(const void* dy, long lddy, const void* x, long ldx, const void* w, long ldw, const void* pre, long ldp,
+                                    void* dx, long lddx, void* dw, void* db, long M, long N, long K, int dtype, int act, void* workspace,
+                                    long workspace_bytes, void* stream) {
+    if (int rc = check_dims(M, K, N, dtype, act)) return rc;
+    if (check_ld("dy", lddy, N)) return -1;
+    ACKTR_ARG(!dx || w, "linear_act_bwd: dx needs w");
+    ACKTR_ARG(!dw || x || M == 0, "linear_act_bwd: dw needs x");
+    if ((dx && (check_ld("w", ldw, K) || check_ld("dx", lddx, K))) || (dw && check_ld("x", ldx, K))) return -1;
+    ACKTR_ARG(act == ACKTR_ACT_NONE || pre || M == 0, "linear_act_bwd: an activation's gradient needs what the forward pass left in `pre`");
+    if (act != ACKTR_ACT_NONE && check_ld("pre", ldp, N)) return -1;
+    ACKTR_ARG(M == 0 || dy, "linear_act_bwd: dy is required");
+    const BwdSpace sp = bwd_space(dy, lddy, x, ldx, w, ldw, pre, ldp, dx, dw, db, M, N, K, (int)elem_bytes(dtype), act);
+    ACKTR_ARG(workspace_bytes >= sp.bytes && ((uintptr_t)workspace & 15) == 0 && (workspace || !sp.bytes),
+              "linear_act_bwd: workspace of %ld bytes, %ld with 16-byte alignment are needed", workspace_bytes, sp.bytes);
+    hipStream_t s = (hipStream_t)stream;
+    return with_dtype(dtype, [&](auto t) -> int {
+        typedef decltype(t) T;
+        constexpr int e = sizeof(T), V = V_OF(e);
+        const int np = (int)up(N, V), kp = (int)up(K, V);
+        char* ws = (char*)workspace;
+        T *dz_ws = (T*)(ws + sp.dz), *x_ws = (T*)(ws + sp.x), *w_ws = (T*)(ws + sp.w);
+        float *sums = (float*)(ws + sp.sums), *slabs = (float*)(ws + sp.slabs);
+
+        // dz and the column sums.  Rows of dy (or pre) that do not start at 16 bytes, or end inside 16, are taken value by value;
+        // dz itself is written into aligned rows, which the two products read.
+        const void* dz = dy;
+        long lddz = lddy;
+        const bool write = act != ACKTR_ACT_NONE && M > 0;
+        if (write) dz = dz_ws, lddz = np;
+        if (M > 0 && (write || db)) {
+            const int cols = sp.aligned ? 32 * V : 32;
+            const int gx = cdiv(N, cols);
+            const int want = max(1, min(SUM_BLOCKS, 2048 / gx));
+            const int rows_per = (int)up(max(16, cdiv(M, want)), 8), gy = cdiv(M, rows_per);
+            auto launch = [&](auto act_c, auto v_c) {
+                act_bwd_kernel<T, decltype(act_c)::value, decltype(v_c)::value><<<dim3(gx, gy), 256, 0, s>>>(
+                    (const T*)dy, lddy, pre, ldp, dz_ws, np, (int)M, (int)N, rows_per, db ? sums : nullptr);
+            };
+            using std::integral_constant;
+            if (write && sp.aligned) launch(std::true_type{}, integral_constant<int, V>{});
+            else if (write) launch(std::true_type{}, integral_constant<int, 1>{});
+            else if (sp.aligned) launch(std::false_type{}, integral_constant<int, V>{});
+            else launch(std::false_type{}, integral_constant<int, 1>{});
+            ACKTR_LAUNCH_CHECK();
+            if (db) {
+                col_sums_kernel<T><<<cdiv(N, 32), 256, 0, s>>>(sums, gy, (int)N, (T*)db);
+                ACKTR_LAUNCH_CHECK();
+            }
+        } else if (db) {                                     // no rows: the gradient of the bias is zero
+            col_sums_kernel<T><<<cdiv(N, 32), 256, 0, s>>>(sums, 0, (int)N, (T*)db);
+            ACKTR_LAUNCH_CHECK();
+        }
+        if (M > 0 && sp.pdy) {                               // no activation: dy itself, in aligned rows
+            if (int rc = pack<T>(dy, lddy, (int)M, (int)N, dz_ws, np, s)) return rc;
+            dz = dz_ws, lddz = np;
+        }
+        if (dx && M > 0) {                                   // dx[M, K] = dz[M, N] w[N, K]: sum over N
+            LinArgs p{};
+            p.a = dz, p.lda = lddz, p.b = w, p.ldb = ldw;
+            if (sp.pw) {
+                if (int rc = pack<T>(w, ldw, (int)N, (int)K, w_ws, kp, s)) return rc;
+                p.b = w_ws, p.ldb = kp;
+            }
+            p.M = (int)M, p.N = (int)K, p.K = (int)N;
+            p.y = dx, p.ldy = lddx, p.vec = K % 8 == 0 && rows16(dx, lddx, e);
+            if (int rc = product<T, true, false, false>(p, slabs, s)) return rc;
+        }
+        if (dw) {                                            // dw[N, K] = dz^T x: sum over M
+            LinArgs p{};
+            p.a = dz, p.lda = lddz, p.b = x, p.ldb = ldx;
+            if (M > 0 && sp.px) {
+                if (int rc = pack<T>(x, ldx, (int)M, (int)K, x_ws, kp, s)) return rc;
+                p.b = x_ws, p.ldb = kp;
+            }
+            p.M = (int)N, p.N = (int)K, p.K = (int)M;
+            p.y = dw, p.ldy = K, p.vec = K % 8 == 0 && rows16(dw, K, e);
+            if (int rc = product<T, false, false, false>(p, slabs, s)) return rc;
+        }
+        return 0;
+    });
+}

@@ -1,0 +1,207 @@
+// Matrix-core tile product for bf16 / fp16 / fp32 operands that are read as they lie in memory.
+//
+//   D(m, n) = sum_k A(m, k) B(n, k)         A: M x K, B: N x K, each with either k or its own row index contiguous
+//
+// * Tiles go from memory straight into LDS (16 bytes a lane, no registers in between).  A lane's LDS place is fixed by the
+//   instruction (base + 16 * lane), so bank conflicts are kept away by choosing which 16 bytes of memory a lane FETCHES:
+//     k contiguous   : the tile is [rows][128 bytes]; chunk c of row r lies at c ^ ((r >> 1) & 7).  A fragment read (16 rows, one
+//                      chunk each) then covers all 64 banks once.
+//     rows contiguous: the tile is [k][rows]; 32-byte unit u of line k lies at u ^ ((k & 3) | (k >> 1 & 4)) (as many of these
+//                      bits as the line has units).  16-bit fragments are
+//                      read with the transposing ds_read_b64_tr_b16 (a group of 16 lanes reads 4 lines x 16 rows and gets 4
+//                      consecutive k of its row each); fp32 fragments with one ds_read_b32 per k.
+// * A K step is 128 bytes of k (64 16-bit or 32 fp32 values), cut into two halves that alternate in registers: while the
+//   matrix cores work on one half, the other half is read from LDS; the next K step's memory loads are in flight for a
+//   whole K step.  One barrier per K step.
+// * The products are formed transposed (B's rows on the matrix instruction's row side), so that a lane ends up with four
+//   consecutive n of one m.  fp32 uses v_mfma_f32_16x16x4 on the same fragments: a lane group's four consecutive k are four
+//   instructions, each pairing the same k of A and B.
+// * Memory loads are written as inline assembly because the compiler, which cannot tell the LDS stages apart, would wait for
+//   all of them in front of every LDS read.  They write no register; tile_sync() waits for them.
+#pragma once
+#include "half_types.hpp"
+
+namespace acktr {
+
+#define ACKTR_LDS __attribute__((address_space(3)))
+
+typedef short s16v4 __attribute__((ext_vector_type(4)));
+typedef short s16v8 __attribute__((ext_vector_type(8)));
+
+// 16 zero bytes of the reduction's tail
+__device__ const uint4 g_tile_zero = {0, 0, 0, 0};
+
+// memory -> LDS, 16 bytes a lane: from `base` (uniform) + off (per lane); to lds (uniform) + 16 * lane
+__device__ __forceinline__ void dma16(const void* base, unsigned off, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+}
+__device__ __forceinline__ void dma16_ptr(const void* p, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory");
+}
+// every load and LDS access of this wave is done, then the workgroup's
+__device__ __forceinline__ void tile_sync() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+__device__ __forceinline__ f32v4 mfma_half(const s16v8& a, const s16v8& b, const f32v4& c, __bf16) {
+    typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32v4 mfma_half(const s16v8& a, const s16v8& b, const f32v4& c, _Float16) {
+    typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32v4 mfma_half(const s16v8& a, const s16v8& b, f32v4 c, float) {
+    const f32v4 x = __builtin_bit_cast(f32v4, a), y = __builtin_bit_cast(f32v4, b);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
+    return c;
+}
+
+// One operand's tile: R rows x 128 bytes of k per K step.  KC: k contiguous.
+template <class T, bool KC, int R, int NT>
+struct TileOperand {
+    static constexpr int E = sizeof(T), V = 16 / E;              // values in 16 bytes
+    static constexpr int KT = 128 / E;                           // k per K step
+    static constexpr int BYTES = R * 128;                        // either layout
+    static constexpr int CHUNKS = BYTES / 16, ITERS = CHUNKS / NT;
+    static constexpr int LINE = KC ? 128 : R * E;                // bytes of an LDS line
+    static_assert(CHUNKS % NT == 0, "whole loads");
+    // the unit permutation of line k (rows contiguous)
+    __device__ static __forceinline__ int twist(int k) { return ((k & 3) | ((k >> 1) & 4)) & (LINE / 32 - 1); }
+
+    unsigned off[ITERS];      // per lane, from the tile's base
+    int kk[ITERS];            // first k of the lane's chunk within the K step
+    const char* base;         // uniform: tile's first row, current K step
+    long step;                // bytes from one K step to the next
+
+    // rows [row0, row0 + R) of `rows`, first K step at k0; ld in elements
+    __device__ __forceinline__ void init(const void* p, long ld, int row0, int rows, int k0, int tid) {
+        if constexpr (KC) {
+            base = (const char*)p + ((long)row0 * ld + k0) * E;
+            step = 128;
+        } else {
+            base = (const char*)p + ((long)k0 * ld + row0) * E;
+            step = (long)KT * ld * E;
+        }
+#pragma unroll
+        for (int i = 0; i < ITERS; ++i) {
+            const int id = i * NT + tid;
+            if constexpr (KC) {
+                const int r = id >> 3, c = (id & 7) ^ ((r >> 1) & 7);
+                int rr = row0 + r < rows ? r : rows - 1 - row0;   // rows behind the last one: the last one's values, never stored
+                off[i] = (unsigned)((long)rr * ld * E) + c * 16;
+                kk[i] = c * V;
+            } else {
+                constexpr int CPL = LINE / 16;                   // chunks in a line
+                const int k = id / CPL, c = id % CPL, f = twist(k);
+                int g = (((c >> 1) ^ f) << 1 | (c & 1)) * V;     // first row of the fetched chunk
+                if (row0 + g >= rows) g = (rows - 1 - row0) / V * V;
+                off[i] = (unsigned)((long)k * ld * E) + g * E;
+                kk[i] = k;
+            }
+        }
+    }
+    // kleft: k that are left at this K step; lds: uniform address of the stage
+    __device__ __forceinline__ void load(int kleft, unsigned lds, int wave) {
+        if (kleft >= KT) {
+#pragma unroll
+            for (int i = 0; i < ITERS; ++i) dma16(base, off[i], lds + (i * NT + wave * 64) * 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < ITERS; ++i)
+                dma16_ptr(kk[i] < kleft ? (const void*)(base + off[i]) : (const void*)&g_tile_zero, lds + (i * NT + wave * 64) * 16);
+        }
+        base += step;
+    }
+    // fragment of rows [r0, r0 + 16), half h of the K step at LDS stage s
+    __device__ static __forceinline__ s16v8 frag(const ACKTR_LDS char* s, int r0, int h, int lane) {
+        if constexpr (KC) {
+            const int r = r0 + (lane & 15), c = (h * 4 + (lane >> 4)) ^ ((r >> 1) & 7);
+            return *reinterpret_cast<const ACKTR_LDS s16v8*>(s + r * 128 + c * 16);
+        } else if constexpr (E == 2) {
+            const int k = h * 32 + 8 * (lane >> 4) + ((lane & 15) >> 2);
+            // k + 4 has the same (k & 3) and (k >> 3 & 1): both reads sit in the same unit
+            const int u = (r0 >> 4) ^ twist(k);
+            ACKTR_LDS char* p = const_cast<ACKTR_LDS char*>(s) + k * LINE + u * 32 + (lane & 3) * 8;
+            const s16v4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<ACKTR_LDS s16v4*>(p));
+            const s16v4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<ACKTR_LDS s16v4*>(p + 4 * LINE));
+            return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+            f32v4 v;
+            const int r = r0 + (lane & 15);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int k = h * 16 + 4 * (lane >> 4) + j;
+                const int u = (r >> 3) ^ twist(k);
+                v[j] = *reinterpret_cast<const ACKTR_LDS float*>(s + k * LINE + u * 32 + (r & 7) * 4);
+            }
+            return __builtin_bit_cast(s16v8, v);
+        }
+    }
+};
+
+// A workgroup's BM x BN tile by WM x WN waves.  After run(): lane holds acc[mi][ni][i] = D(m, n) with
+// m = wave's first row + 16 mi + lane % 16, n = wave's first column + 16 ni + 4 (lane / 16) + i.
+template <class T, bool AKC, bool BKC, int BM, int BN, int WM, int WN>
+struct TileGemm {
+    static constexpr int NT = WM * WN * 64, MI = BM / WM / 16, NI = BN / WN / 16;
+    typedef TileOperand<T, AKC, BM, NT> OpA;
+    typedef TileOperand<T, BKC, BN, NT> OpB;
+    static constexpr int KT = OpA::KT, STAGE = OpA::BYTES + OpB::BYTES, LDS = 2 * STAGE;
+
+    f32v4 acc[MI][NI];
+
+    __device__ __forceinline__ void frags(const ACKTR_LDS char* s, int h, int wm, int wn, int lane, s16v8 (&fa)[MI], s16v8 (&fb)[NI]) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) fa[i] = OpA::frag(s, wm + 16 * i, h, lane);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) fb[i] = OpB::frag(s + OpA::BYTES, wn + 16 * i, h, lane);
+    }
+    __device__ __forceinline__ void products(const s16v8 (&fa)[MI], const s16v8 (&fb)[NI]) {
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+            for (int i = 0; i < MI; ++i) acc[i][j] = mfma_half(fb[j], fa[i], acc[i][j], T{});
+    }
+    __device__ __forceinline__ void run(const void* a, long lda, int m0, int M, const void* b, long ldb, int n0, int N, int k0, int k1,
+                                        ACKTR_LDS char* sm) {
+        const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
+        const unsigned lds = (unsigned)(uintptr_t)sm;
+        OpA oa;
+        OpB ob;
+        oa.init(a, lda, m0, M, k0, tid);
+        ob.init(b, ldb, n0, N, k0, tid);
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) acc[i][j] = f32v4{0.f, 0.f, 0.f, 0.f};
+        int left = k1 - k0;                              // k not yet requested
+        auto request = [&](unsigned stage) {
+            oa.load(left, lds + stage, wave);
+            ob.load(left, lds + stage + OpA::BYTES, wave);
+            left -= KT;
+        };
+        const int steps = (k1 - k0 + KT - 1) / KT;
+        if (steps <= 0) return;
+        s16v8 fa0[MI], fb0[NI], fa1[MI], fb1[NI];
+        request(0);
+        tile_sync();
+        if (steps > 1) request(STAGE);
+        frags(sm, 0, wm, wn, lane, fa0, fb0);
+        unsigned cur = 0;
+        for (int t = 0; t + 1 < steps; ++t) {
+            frags(sm + cur, 1, wm, wn, lane, fa1, fb1);
+            products(fa0, fb0);
+            tile_sync();                                 // this stage is read, the other one has arrived
+            if (t + 2 < steps) request(cur);
+            cur ^= STAGE;
+            frags(sm + cur, 0, wm, wn, lane, fa0, fb0);
+            products(fa1, fb1);
+        }
+        frags(sm + cur, 1, wm, wn, lane, fa1, fb1);
+        products(fa0, fb0);
+        products(fa1, fb1);
+    }
+};
+
+}  // namespace acktr

@@ -1,0 +1,70 @@
+"""CPU: the gated core's operators refuse what they cannot take, before anything is launched."""
+import ctypes
+
+import pytest
+import torch
+
+
+def lib():
+    from a2c_ppo_acktr import _hip
+    return _hip.lib()
+
+
+def err():
+    return lib().acktr_last_error().decode()
+
+
+def test_no_cpu_path():
+    from a2c_ppo_acktr import algo, ops
+    x, w = torch.zeros(4, 8), torch.zeros(3, 8)
+    s = torch.zeros(5, 2, 8)
+    for f in (lambda: ops.linear_act_fwd(x, w), lambda: ops.linear_act_bwd(torch.zeros(4, 3), x, w), lambda: ops.gated_scan_fwd(s, s),
+              lambda: ops.gated_scan_bwd(s, s, s), lambda: ops.gated_scan_step(s[0], s[0], torch.zeros(2, 8)),
+              lambda: algo.AdamW([x], lr=1.0, grads=[x]).step()):
+        with pytest.raises(RuntimeError):
+            f()
+
+
+def test_linear_entry_arguments():
+    L, one = lib(), ctypes.c_void_p(256)
+    fwd = lambda M=4, N=8, K=8, ldx=8, ldw=8, ldy=8, dt=1, act=0, x=one, ws=one, nb=1 << 20: L.acktr_linear_act_fwd(
+        x, ldx, one, ldw, None, None, 0, one, ldy, None, 0, M, N, K, dt, act, ws, nb, None)
+    for kw in (dict(dt=3), dict(act=5), dict(act=-1), dict(M=-1), dict(N=0), dict(K=0), dict(K=(1 << 20) + 1, ldx=1 << 21), dict(ldx=7), dict(ldw=4),
+               dict(ldy=7), dict(ldx=1 << 21), dict(x=None), dict(K=7, ldx=7, nb=16), dict(K=7, ldx=7, ws=None), dict(K=7, ldx=7, ws=ctypes.c_void_p(264))):
+        assert fwd(**kw) == -1 and err(), kw
+    assert fwd(M=0) == 0
+    assert L.acktr_linear_act_fwd_workspace_bytes(one, 8, one, 8, 4, 8, 8, 9) == -1
+    bwd = lambda act=0, pre=None, dy=one, x=one, w=one, dx=one, dw=one, ldp=8, lddx=8, dt=1, nb=1 << 20: L.acktr_linear_act_bwd(
+        dy, 8, x, 8, w, 8, pre, ldp, dx, lddx, dw, None, 4, 8, 8, dt, act, one, nb, None)
+    for kw in (dict(act=2), dict(act=2, pre=one, ldp=7), dict(dy=None), dict(x=None), dict(w=None), dict(lddx=3), dict(dt=-1), dict(act=2, pre=one, nb=0)):
+        assert bwd(**kw) == -1 and err(), kw
+
+
+def test_scan_entry_arguments():
+    L, one = lib(), ctypes.c_void_p(256)
+    fwd = lambda T=4, N=2, H=8, dt=1, g=one, nb=1 << 30: L.acktr_gated_scan_fwd(g, 16, 8, one, 16, 8, None, None, one, 16, 8, None, None, T, N, H, dt,
+                                                                                one, nb, None)
+    for kw in (dict(dt=4), dict(T=-1), dict(N=-1), dict(H=0), dict(T=1 << 30), dict(N=1 << 20, H=1 << 20), dict(g=None), dict(nb=0, T=4000)):
+        assert fwd(**kw) == -1 and err(), kw
+    assert fwd(N=0) == 0 and fwd(T=0) == 0
+    bwd = lambda T=4, d=one, saved=None, nb=1 << 30: L.acktr_gated_scan_bwd(d, 16, 8, one, 16, 8, one, 16, 8, None, None, saved, None, one, 16, 8, one, 16, 8,
+                                                                            None, T, 2, 8, 1, one, nb, None)
+    for kw in (dict(d=None), dict(T=65), dict(T=4000, saved=one, nb=0)):
+        assert bwd(**kw) == -1 and err(), kw
+    assert L.acktr_gated_scan_step(None, 8, one, 8, one, None, one, 8, 2, 8, 1, None) == -1
+    assert L.acktr_gated_scan_step(one, 8, one, 8, one, None, one, 8, 2, 8, 7, None) == -1
+    assert L.acktr_gated_scan_workspace_bytes(4, 2, 0, 1) == -1
+
+
+def test_adamw_entry_arguments():
+    L, one = lib(), ctypes.c_void_p(256)
+    call = lambda st=one, n=4, m=one, sc=one, bits=32, t=one: L.acktr_adamw_step(st, t, one, n, m, one, sc, bits, 0, None)
+    for kw in (dict(st=None), dict(n=-1), dict(m=None), dict(bits=16), dict(bits=8, sc=None), dict(t=None), dict(m=ctypes.c_void_p(260))):
+        assert call(**kw) == -1 and err(), kw
+    assert L.acktr_adamw_read_moments(one, one, one, one, one, 100, None) == -1
+    assert L.acktr_adamw_read_moments(None, one, one, one, one, 256, None) == -1
+
+
+def test_struct_matches_the_header():
+    from a2c_ppo_acktr import _hip
+    assert ctypes.sizeof(_hip.AdamwTensor) == 56 and _hip.AdamwTensor.vec.offset == 52

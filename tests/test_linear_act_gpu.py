@@ -1,0 +1,218 @@
+"""linear_act_fwd / linear_act_bwd against a 64-bit evaluation (gated_refs.py derives the tolerances)."""
+import pytest
+import torch
+
+from gated_refs import ACTS, check, linear64, linear_grads64
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda:0'
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def rnd(seed, *shape, scale=1.0, dtype=F32):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    return (torch.randn(*shape, device=DEV, generator=g) * scale).to(dtype)
+
+
+def run(M, N, K, dt, act, bias=True, res=True, pad=0, seed=0, big=1.0):
+    from a2c_ppo_acktr import ops
+    cut = lambda s, r, c, k=1.0: rnd(seed + s, r, c + pad, scale=k, dtype=dt)[:, :c]
+    x, w = cut(1, M, K, big), cut(2, N, K, 1.5 / K ** 0.5)
+    b = rnd(seed + 3, N, scale=0.5, dtype=dt) if bias else None
+    r = cut(4, M, N) if res else None
+    dy = cut(5, M, N, 0.1)
+    pre = torch.empty(M, N, dtype=dt, device=DEV) if act != 'none' else None
+    y = ops.linear_act_fwd(x, w, b, act=act, residual=r, pre=pre)
+    dx, dw, db = ops.linear_act_bwd(dy, x, w, pre=pre, act=act)
+    ry, ty, slope, ts = linear64(x, w, b, act, r)
+    gx, gw, gb = linear_grads64(dy, x, w, slope, ts)
+    check(y, (ry, ty), 'y')
+    check(dx, gx, 'dx')
+    check(dw, gw, 'dw')
+    check(db, gb, 'db')
+    # without pre the same values come out
+    assert torch.equal(ops.linear_act_fwd(x, w, b, act=act, residual=r), y)
+    # and again, bit for bit
+    again = ops.linear_act_bwd(dy, x, w, pre=pre, act=act)
+    assert all(torch.equal(p, q) for p, q in zip(again, (dx, dw, db)))
+
+
+SIZES = [(1, 1, 1), (1, 8, 8), (3, 5, 7), (2, 64, 64), (16, 16, 32), (17, 33, 65), (32, 1024, 512), (33, 40, 200), (64, 64, 64), (65, 129, 8),
+         (128, 256, 72), (130, 264, 136), (255, 257, 96), (300, 96, 1000), (1011, 390, 777), (512, 512, 512), (1000, 16, 2048)]
+
+
+@pytest.mark.parametrize('dt', [BF, HF, F32])
+@pytest.mark.parametrize('M,N,K', SIZES)
+def test_sizes(M, N, K, dt):
+    run(M, N, K, dt, 'tanh')
+
+
+@pytest.mark.parametrize('dt', [BF, HF, F32])
+@pytest.mark.parametrize('act', ACTS)
+@pytest.mark.parametrize('bias,res', [(False, False), (True, False), (False, True)])
+def test_epilogues(act, dt, bias, res):
+    run(200, 136, 96, dt, act, bias, res)
+    run(70, 37, 51, dt, act, bias, res, seed=50)
+
+
+@pytest.mark.parametrize('dt', [BF, HF, F32])
+@pytest.mark.parametrize('pad', [1, 3, 4, 8, 40])
+def test_rows_of_wider_tensors(dt, pad):
+    run(140, 72, 104, dt, 'silu', pad=pad)
+
+
+@pytest.mark.parametrize('dt', [BF, F32])
+@pytest.mark.parametrize('M,N,K', [(4096, 512, 1568), (2048, 1024, 512), (8200, 260, 136), (16, 2048, 2048), (5000, 8, 40), (20000, 24, 16)])
+def test_larger(dt, M, N, K):
+    run(M, N, K, dt, 'gelu')
+
+
+def test_large_pre_activations():
+    """tails of every activation: values far from zero"""
+    for act in ACTS:
+        run(96, 64, 64, F32, act, big=30.0)
+
+
+def test_slices_at_odd_offsets():
+    """operands that start in the middle of 16 bytes"""
+    from a2c_ppo_acktr import ops
+    for off in (1, 2, 5):
+        x = rnd(1, 50 * 64 + 16, dtype=BF)[off:off + 50 * 64].view(50, 64)
+        w = rnd(2, 24 * 64 + 16, scale=0.1, dtype=BF)[off:off + 24 * 64].view(24, 64)
+        out = torch.full((50 * 24 + 16,), 7.0, dtype=BF, device=DEV)
+        o = out[off:off + 50 * 24].view(50, 24)
+        assert ops.linear_act_fwd(x, w, act='relu', out=o).data_ptr() == o.data_ptr()
+        y, t, _, _ = linear64(x, w, None, 'relu')
+        check(o, (y, t), 'y')
+        assert bool((out[:off] == 7).all()) and bool((out[off + 50 * 24:] == 7).all())      # nothing beside it
+
+
+def test_rows_beside_the_output_stay():
+    from a2c_ppo_acktr import ops
+    for M, N, ld in ((70, 37, 64), (130, 64, 80), (5, 24, 25)):
+        big = torch.full((M + 3, ld), 5.0, dtype=BF, device=DEV)
+        ops.linear_act_fwd(rnd(1, M, 40, dtype=BF), rnd(2, N, 40, dtype=BF), out=big[:M, :N])
+        assert bool((big[M:] == 5).all()) and bool((big[:, N:] == 5).all())
+
+
+def test_no_rows():
+    from a2c_ppo_acktr import ops
+    x, w = torch.empty(0, 24, dtype=BF, device=DEV), rnd(1, 16, 24, dtype=BF)
+    assert ops.linear_act_fwd(x, w, act='gelu').shape == (0, 16)
+    pre, dy = torch.empty(0, 16, dtype=BF, device=DEV), torch.empty(0, 16, dtype=BF, device=DEV)
+    dx, dw, db = ops.linear_act_bwd(dy, x, w, pre=pre, act='gelu')
+    assert dx.shape == (0, 24) and not dw.any() and not db.any()
+
+
+def test_residual_in_place():
+    from a2c_ppo_acktr import ops
+    for M, N, K in ((64, 64, 64), (513, 200, 96), (40, 8, 2048)):
+        x, w, r = rnd(1, M, K, dtype=BF), rnd(2, N, K, scale=0.1, dtype=BF), rnd(3, M, N, dtype=BF)
+        want = ops.linear_act_fwd(x, w, act='silu', residual=r)
+        assert torch.equal(ops.linear_act_fwd(x, w, act='silu', residual=r, out=r), want)
+
+
+def test_only_what_is_needed():
+    from a2c_ppo_acktr import ops
+    x, w, dy = rnd(1, 100, 72, dtype=BF), rnd(2, 40, 72, dtype=BF), rnd(3, 100, 40, dtype=BF)
+    pre = torch.empty(100, 40, dtype=BF, device=DEV)
+    ops.linear_act_fwd(x, w, act='tanh', pre=pre)
+    full = ops.linear_act_bwd(dy, x, w, pre=pre, act='tanh')
+    for k in range(3):
+        need = [i == k for i in range(3)]
+        part = ops.linear_act_bwd(dy, x, w, pre=pre, act='tanh', need_dx=need[0], need_dw=need[1], need_db=need[2])
+        for i in range(3):
+            assert (part[i] is None) if i != k else torch.equal(part[i], full[i])
+
+
+def test_values_that_are_not_finite_stay_in_their_rows():
+    from a2c_ppo_acktr import ops
+    x, w = rnd(1, 150, 64, dtype=BF), rnd(2, 72, 64, dtype=BF)
+    clean = ops.linear_act_fwd(x, w, act='silu')
+    x2 = x.clone()
+    x2[7, 3], x2[149, 63] = float('nan'), float('inf')
+    got = ops.linear_act_fwd(x2, w, act='silu')
+    keep = [i for i in range(150) if i not in (7, 149)]
+    assert torch.equal(got[keep], clean[keep])
+    assert bool(got[7].isnan().all()) and not bool(got[149].isfinite().all())
+    assert bool(ops.linear_act_fwd(x2, w, act='relu')[7].isnan().all())
+
+
+def test_gradient_against_differences():
+    """fp32: (L(p + h) - L(p - h)) / 2h with L in 64 bits, against the operator's gradients along random directions.  The central
+    difference is off by h^2 / 6 times the third derivative, here below 1e-5 of the gradient's scale, the operator by 1e-5."""
+    from a2c_ppo_acktr import ops
+    for act in ('tanh', 'silu', 'gelu'):
+        x, w, b, r = rnd(1, 40, 24), rnd(2, 16, 24, scale=0.3), rnd(3, 16), rnd(4, 40, 16)
+        dy = rnd(5, 40, 16)
+        pre = torch.empty(40, 16, device=DEV)
+        ops.linear_act_fwd(x, w, b, act=act, residual=r, pre=pre)
+        dx, dw, db = ops.linear_act_bwd(dy, x, w, pre=pre, act=act)
+        loss = lambda x, w, b: float((linear64(x, w, b, act)[0] * dy.double()).sum())
+        for i, (p, g) in enumerate(((x, dx), (w, dw), (b, db))):
+            v = rnd(10 + i, *p.shape).double()
+            h = 1e-4
+            args = [x.double(), w.double(), b.double()]
+            up, dn = list(args), list(args)
+            up[i], dn[i] = args[i] + h * v, args[i] - h * v
+            num = (loss(*up) - loss(*dn)) / (2 * h)
+            ana = float((g.double() * v).sum())
+            assert abs(num - ana) <= 2e-5 * float(g.double().norm() * v.norm()), (act, i, num, ana)
+
+
+def test_captured_and_replayed():
+    from a2c_ppo_acktr import ops
+    M, N, K = 260, 136, 72
+    x, w, b, dy = rnd(1, M, K, dtype=BF), rnd(2, N, K, dtype=BF), rnd(3, N, dtype=BF), rnd(4, M, N, dtype=BF)
+    pre = torch.empty(M, N, dtype=BF, device=DEV)
+
+    def step():
+        y = ops.linear_act_fwd(x, w, b, act='gelu', pre=pre)
+        return (y,) + ops.linear_act_bwd(dy, x, w, pre=pre, act='gelu')
+    step()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):                                     # two graphs, replayed in turn: neither uses the other's scratch
+        g = torch.cuda.CUDAGraph()
+        with ops.graph_capture(g):
+            out = step()
+        graphs.append((g, out))
+    for k in range(4):
+        x.copy_(rnd(20 + k, M, K, dtype=BF))
+        want = [t.clone() for t in step()]
+        for g, out in graphs:
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(out, want)), k
+
+
+def test_two_streams():
+    from a2c_ppo_acktr import ops
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    x, w = rnd(1, 900, 777, dtype=BF), rnd(2, 390, 777, dtype=BF)
+    x2, w2 = rnd(3, 900, 777, dtype=BF), rnd(4, 390, 777, dtype=BF)
+    want, want2 = ops.linear_act_fwd(x, w, act='silu'), ops.linear_act_fwd(x2, w2, act='silu')
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        with torch.cuda.stream(a):
+            got.append((ops.linear_act_fwd(x, w, act='silu'), want))
+        with torch.cuda.stream(b):
+            got.append((ops.linear_act_fwd(x2, w2, act='silu'), want2))
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in got)
+
+
+def test_refusals_on_the_device():
+    from a2c_ppo_acktr import ops
+    x, w = rnd(1, 8, 16, dtype=BF), rnd(2, 4, 16, dtype=BF)
+    bad = [lambda: ops.linear_act_fwd(x, w.half()), lambda: ops.linear_act_fwd(x, w[:, :8]), lambda: ops.linear_act_fwd(x, w, act='elu'),
+           lambda: ops.linear_act_fwd(x, w, bias=rnd(3, 5, dtype=BF)), lambda: ops.linear_act_fwd(x, w, residual=rnd(3, 8, 5, dtype=BF)),
+           lambda: ops.linear_act_fwd(x.t(), w.t()), lambda: ops.linear_act_fwd(x.double(), w.double()),
+           lambda: ops.linear_act_fwd(x, w, out=x[:, :4]), lambda: ops.linear_act_fwd(x, w, out=rnd(3, 1, 4, dtype=BF).expand(8, 4)),
+           lambda: ops.linear_act_fwd(x[:1].expand(8, 16), w), lambda: ops.linear_act_bwd(rnd(3, 8, 4, dtype=BF), x, w, act='tanh'),
+           lambda: ops.linear_act_bwd(rnd(3, 8, 5, dtype=BF), x, w), lambda: ops.linear_act_bwd(rnd(3, 8, 4, dtype=BF), x, w, dx=x)]
+    for f in bad:
+        with pytest.raises(RuntimeError):
+            f()
