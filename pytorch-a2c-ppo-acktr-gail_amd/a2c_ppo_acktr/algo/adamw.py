@@ -128,6 +128,8 @@ class AdamW(object):
         replay when a hyperparameter changed."""
         self._check_hyper()
         dev = self.params[0].device
+        if dev.type == 'cuda' and dev.index is None:
+            dev = torch.device('cuda', torch.cuda.current_device())
         if self._dev is None or self._dev != dev:
             if dev.type != 'cuda':
                 raise RuntimeError('AdamW: parameters must live on the MI355X device (got %s): this package has no CPU path' % dev)
@@ -162,7 +164,7 @@ class AdamW(object):
         """One step on all tensors: two launches."""
         self.prepare()
         L = _hip.lib()
-        with ops._on(self._dev):
+        with ops._on(self._dev.index):
             rc = L.acktr_adamw_step(self._state.data_ptr(), self._tensors.data_ptr(), self._chunks.data_ptr(), self._chunks.shape[0],
                                     self.mom1.data_ptr(), self.mom2.data_ptr(), self.scales.data_ptr() if self.scales is not None else None,
                                     self.state_bits, 1 if self._hyper[5] > 0 else 0, _hip.cur_stream(self._dev))
@@ -177,7 +179,7 @@ class AdamW(object):
         if self.state_bits == 32:
             return self.mom1, self.mom2
         m, v = torch.empty(self._total, dtype=f32, device=self._dev), torch.empty(self._total, dtype=f32, device=self._dev)
-        with ops._on(self._dev):
+        with ops._on(self._dev.index):
             rc = _hip.lib().acktr_adamw_read_moments(self.mom1.data_ptr(), self.mom2.data_ptr(), self.scales.data_ptr(), m.data_ptr(),
                                                      v.data_ptr(), self._total, _hip.cur_stream(self._dev))
         _hip.check(rc, 'acktr_adamw_read_moments')

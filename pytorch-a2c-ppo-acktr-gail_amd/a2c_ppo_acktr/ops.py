@@ -462,8 +462,8 @@ class _on(object):
     """Kernels are launched on the operands' device, whichever device is current."""
     __slots__ = ('guard',)
 
-    def __init__(self, device):
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    def __init__(self, index):
+        self.guard = None if index == torch.cuda.current_device() else torch.cuda.device(index)
 
     def __enter__(self):
         if self.guard is not None:
@@ -475,32 +475,53 @@ class _on(object):
         return False
 
 
-def _need(t, name, shape, dtype, device):
-    """A GPU operand of the expected shape, type and device whose last axis is contiguous."""
+def _launch(fn, args, index, what, work):
+    """fn(*args, stream) on device `index`, timed when the profiler is on."""
+    stream = _hip.cur_stream(index)
+    if profiler is None and index == torch.cuda.current_device():
+        rc = fn(*args, stream)
+    else:
+        with _on(index), _Timed(what, work):
+            rc = fn(*args, stream)
+    if rc:
+        _hip.check(rc, 'acktr_' + what)
+
+
+def _refuse(t, name, shape, dtype, index):
+    """Says what is wrong with an operand that is not a GPU tensor of this shape, type and device with a contiguous last axis."""
     if not t.is_cuda:
         raise RuntimeError('%s must live on the MI355X device (got %s): this package has no CPU path' % (name, t.device))
-    if t.device != device:
-        raise RuntimeError('%s is on %s, expected %s' % (name, t.device, device))
+    if t.get_device() != index:
+        raise RuntimeError('%s is on %s, expected cuda:%d' % (name, t.device, index))
     if t.dtype != dtype:
         raise RuntimeError('%s must be %s (got %s)' % (name, dtype, t.dtype))
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise RuntimeError('%s must have shape %s (got %s)' % (name, tuple(shape), tuple(t.shape)))
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise RuntimeError("%s: the last axis must be contiguous (stride %d)" % (name, t.stride(-1)))
+    raise RuntimeError('%s: the last axis must be contiguous (strides %s)' % (name, tuple(t.stride())))
+
+
+def _vec(t, name, n, dtype, index):
+    if t.dtype is not dtype or t.get_device() != index or t.shape != (n,) or (n > 1 and t.stride(0) != 1):
+        _refuse(t, name, (n,), dtype, index)
     return t.data_ptr()
 
 
-def _rows(t, name, shape, dtype, device):
+def _rows(t, name, shape, dtype, index):
     """(pointer, row stride in elements) of a matrix whose rows may be slices of wider ones."""
-    p = _need(t, name, shape, dtype, device)
-    return p, (t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1))
+    if t.dtype is not dtype or t.get_device() != index or t.shape != shape:
+        _refuse(t, name, shape, dtype, index)
+    ld, inner = t.stride()
+    if inner != 1 and shape[1] > 1:
+        _refuse(t, name, shape, dtype, index)
+    return t.data_ptr(), (ld if shape[0] > 1 else max(shape[1], 1))
 
 
-def _dense(t, name, shape, dtype, device):
-    p = _need(t, name, shape, dtype, device)
+def _dense(t, name, shape, dtype, index):
+    if t.dtype is not dtype or t.get_device() != index or t.shape != shape:
+        _refuse(t, name, shape, dtype, index)
     if not t.is_contiguous():
         raise RuntimeError('%s must be contiguous' % name)
-    return p
+    return t.data_ptr()
 
 
 def _dtype_code(t, name):
@@ -518,6 +539,9 @@ def _act_code(act):
 
 
 def _span(t):
+    if t.is_contiguous():
+        p = t.data_ptr()
+        return p, p + t.nbytes
     reach = 1
     for n, s in zip(t.shape, t.stride()):
         if n == 0:
@@ -546,6 +570,8 @@ def _no_overlap(a, b, what):
 
 def _writable(t, name):
     """Every element of a tensor that is written has a place of its own (an expanded tensor has not)."""
+    if t.is_contiguous():
+        return
     axes = sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1)
     reach = 1
     for s, n in axes:
@@ -554,10 +580,10 @@ def _writable(t, name):
         reach = s * (n - 1) + reach
 
 
-def _scratch(nbytes, device, what):
+def _scratch(nbytes, like, what):
     if nbytes < 0:
         _hip.check(-1, what)
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    return like.new_empty(nbytes, dtype=torch.uint8)
 
 
 def linear_act_fwd(x, w, bias=None, act=None, residual=None, out=None, pre=None):
@@ -567,31 +593,31 @@ def linear_act_fwd(x, w, bias=None, act=None, residual=None, out=None, pre=None)
     code, act = _dtype_code(x, 'x'), _act_code(act)
     if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1] or x.shape[1] < 1 or w.shape[0] < 1:
         raise RuntimeError('linear_act_fwd: x [M, K] and w [N, K] expected, got %s and %s' % (tuple(x.shape), tuple(w.shape)))
-    (M, K), N, dt, dev = x.shape, w.shape[0], x.dtype, x.device
+    (M, K), N, dt, at = x.shape, w.shape[0], x.dtype, x.get_device()
+    mn = (M, N)
     given = out is not None
-    if out is None:
-        out = torch.empty(M, N, dtype=dt, device=dev)
-    px, ldx = _rows(x, 'x', (M, K), dt, dev)
-    pw, ldw = _rows(w, 'w', (N, K), dt, dev)
-    py, ldy = _rows(out, 'out', (M, N), dt, dev)
-    pb = _need(bias, 'bias', (N,), dt, dev) if bias is not None else None
-    pr, ldr = _rows(residual, 'residual', (M, N), dt, dev) if residual is not None else (None, 0)
-    pz, ldz = _rows(pre, 'pre', (M, N), dt, dev) if pre is not None else (None, 0)
-    for a, name in ((out if given else None, 'out'), (pre, 'pre')):
-        if a is not None:
-            _writable(a, name)
-            for b in (x, w, bias) + (() if a is out and residual is not None and pr == py and ldr == ldy else (residual,)):
-                _no_overlap(a, b, 'linear_act_fwd: %s and an input' % name)
+    if not given:
+        out = x.new_empty(mn)
+    px, ldx = _rows(x, 'x', (M, K), dt, at)
+    pw, ldw = _rows(w, 'w', (N, K), dt, at)
+    py, ldy = _rows(out, 'out', mn, dt, at)
+    pb = _vec(bias, 'bias', N, dt, at) if bias is not None else None
+    pr, ldr = _rows(residual, 'residual', mn, dt, at) if residual is not None else (None, 0)
+    pz, ldz = None, 0
+    if pre is not None:
+        pz, ldz = _rows(pre, 'pre', mn, dt, at)
+        _writable(pre, 'pre')
+        for b in (x, w, bias, residual, out if given else None):
+            _no_overlap(pre, b, 'linear_act_fwd: pre and another operand')
     if given:
-        _no_overlap(out, pre, 'linear_act_fwd: out and pre')
+        _writable(out, 'out')
+        for b in (x, w, bias, None if pr == py and ldr == ldy else residual):
+            _no_overlap(out, b, 'linear_act_fwd: out and an input')
     L = _hip.lib()
-    with _on(dev):
-        nb = L.acktr_linear_act_fwd_workspace_bytes(px, ldx, pw, ldw, M, N, K, code)
-        ws = _scratch(nb, dev, 'acktr_linear_act_fwd')
-        with _Timed('linear_act_fwd', 2.0 * M * N * K):
-            rc = L.acktr_linear_act_fwd(px, ldx, pw, ldw, pb, pr, ldr, py, ldy, pz, ldz, M, N, K, code, act,
-                                        ws.data_ptr() if ws is not None else None, nb, _hip.cur_stream(dev))
-    _hip.check(rc, 'acktr_linear_act_fwd')
+    nb = L.acktr_linear_act_fwd_workspace_bytes(px, ldx, pw, ldw, M, N, K, code)
+    ws = _scratch(nb, x, 'acktr_linear_act_fwd') if nb else None
+    _launch(L.acktr_linear_act_fwd, (px, ldx, pw, ldw, pb, pr, ldr, py, ldy, pz, ldz, M, N, K, code, act, ws.data_ptr() if nb else None, nb),
+            at, 'linear_act_fwd', 2.0 * M * N * K)
     return out
 
 
@@ -602,50 +628,57 @@ def linear_act_bwd(dy, x, w, pre=None, act=None, dx=None, dw=None, db=None, need
     if dy.dim() != 2 or x.dim() != 2 or w.dim() != 2 or x.shape[0] != dy.shape[0] or tuple(w.shape) != (dy.shape[1], x.shape[1]):
         raise RuntimeError('linear_act_bwd: dy [M, N], x [M, K] and w [N, K] expected, got %s, %s and %s'
                            % (tuple(dy.shape), tuple(x.shape), tuple(w.shape)))
-    (M, N), K, dt, dev = dy.shape, x.shape[1], dy.dtype, dy.device
+    (M, N), K, dt, at = dy.shape, x.shape[1], dy.dtype, dy.get_device()
     if act and pre is None:
         raise RuntimeError("linear_act_bwd: an activation's gradient needs `pre` of the forward pass")
     if not act:
         pre = None
     given = [t for t, need in ((dx, need_dx), (dw, need_dw), (db, need_db)) if need and t is not None]
-    new = lambda need, t, *s: torch.empty(*s, dtype=dt, device=dev) if need and t is None else (t if need else None)
-    dx, dw, db = new(need_dx, dx, M, K), new(need_dw, dw, N, K), new(need_db, db, N)
-    pg, ldg = _rows(dy, 'dy', (M, N), dt, dev)
-    px, ldx = _rows(x, 'x', (M, K), dt, dev)
-    pw, ldw = _rows(w, 'w', (N, K), dt, dev)
-    pz, ldz = _rows(pre, 'pre', (M, N), dt, dev) if pre is not None else (None, 0)
-    qx, ldq = _rows(dx, 'dx', (M, K), dt, dev) if dx is not None else (None, 0)
-    qw = _dense(dw, 'dw', (N, K), dt, dev) if dw is not None else None
-    qb = _need(db, 'db', (N,), dt, dev) if db is not None else None
+    pg, ldg = _rows(dy, 'dy', (M, N), dt, at)
+    px, ldx = _rows(x, 'x', (M, K), dt, at)
+    pw, ldw = _rows(w, 'w', (N, K), dt, at)
+    pz, ldz = _rows(pre, 'pre', (M, N), dt, at) if pre is not None else (None, 0)
+    qx = qw = qb = None
+    ldq = 0
+    if need_dx:
+        dx = dy.new_empty((M, K)) if dx is None else dx
+        qx, ldq = _rows(dx, 'dx', (M, K), dt, at)
+    if need_dw:
+        dw = dy.new_empty((N, K)) if dw is None else dw
+        qw = _dense(dw, 'dw', (N, K), dt, at)
+    if need_db:
+        db = dy.new_empty(N) if db is None else db
+        qb = _vec(db, 'db', N, dt, at)
     for i, a in enumerate(given):
         _writable(a, 'a gradient')
         for b in (dy, x, w, pre) + tuple(given[:i]):
             _no_overlap(a, b, 'linear_act_bwd: a gradient and another operand')
     L = _hip.lib()
-    with _on(dev):
-        nb = L.acktr_linear_act_bwd_workspace_bytes(pg, ldg, px, ldx, pw, ldw, pz, ldz, dx is not None, dw is not None, db is not None,
-                                                    M, N, K, code, act)
-        ws = _scratch(nb, dev, 'acktr_linear_act_bwd')
-        with _Timed('linear_act_bwd', 2.0 * M * N * K * ((dx is not None) + (dw is not None))):
-            rc = L.acktr_linear_act_bwd(pg, ldg, px, ldx, pw, ldw, pz, ldz, qx, ldq, qw, qb, M, N, K, code, act,
-                                        ws.data_ptr() if ws is not None else None, nb, _hip.cur_stream(dev))
-    _hip.check(rc, 'acktr_linear_act_bwd')
-    return dx, dw, db
+    nb = L.acktr_linear_act_bwd_workspace_bytes(pg, ldg, px, ldx, pw, ldw, pz, ldz, need_dx, need_dw, need_db, M, N, K, code, act)
+    ws = _scratch(nb, dy, 'acktr_linear_act_bwd') if nb else None
+    _launch(L.acktr_linear_act_bwd, (pg, ldg, px, ldx, pw, ldw, pz, ldz, qx, ldq, qw, qb, M, N, K, code, act, ws.data_ptr() if nb else None, nb),
+            at, 'linear_act_bwd', 2.0 * M * N * K * (bool(need_dx) + bool(need_dw)))
+    return dx if need_dx else None, dw if need_dw else None, db if need_db else None
 
 
-def _steps(t, name, shape, dtype, device):
+def _steps(t, name, shape, dtype, index):
     """(pointer, stride over steps, stride over sequences) of a [T, N, H] operand; axes of one element take a packed stride."""
-    p = _need(t, name, shape, dtype, device)
+    if t.dtype is not dtype or t.get_device() != index or t.shape != shape:
+        _refuse(t, name, shape, dtype, index)
+    st, sn, inner = t.stride()
     T, N, H = shape
-    return p, (t.stride(0) if T > 1 else N * H), (t.stride(1) if N > 1 else H)
+    if inner != 1 and H > 1:
+        _refuse(t, name, shape, dtype, index)
+    return t.data_ptr(), (st if T > 1 else N * H), (sn if N > 1 else H)
 
 
-def _masks(masks, T, N, dev):
+def _masks(masks, shape, index):
+    """[T, N] fp32 or the rollout's [T, N, 1]"""
     if masks is None:
         return None
-    if masks.dim() == 3 and masks.shape[-1] == 1:
-        masks = masks[..., 0]
-    return _dense(masks, 'masks', (T, N), f32, dev)
+    if masks.dim() == len(shape) + 1 and masks.shape[-1] == 1:
+        masks = masks.squeeze(-1)
+    return _dense(masks, 'masks', shape, f32, index)
 
 
 def gated_scan_fwd(gate, value, h0=None, masks=None, out=None, save=False):
@@ -656,27 +689,25 @@ def gated_scan_fwd(gate, value, h0=None, masks=None, out=None, save=False):
     code = _dtype_code(gate, 'gate')
     if gate.dim() != 3 or gate.shape[2] < 1:
         raise RuntimeError('gated_scan_fwd: gate [T, N, H] expected, got %s' % (tuple(gate.shape),))
-    (T, N, H), dt, dev = gate.shape, gate.dtype, gate.device
+    shape, dt, at = gate.shape, gate.dtype, gate.get_device()
+    T, N, H = shape
     given = out is not None
-    if out is None:
-        out = torch.empty(T, N, H, dtype=dt, device=dev)
-    pg, pv, po = (_steps(t, n, (T, N, H), dt, dev) for t, n in ((gate, 'gate'), (value, 'value'), (out, 'out')))
-    ph = _dense(h0, 'h0', (N, H), f32, dev) if h0 is not None else None
-    pm = _masks(masks, T, N, dev)
+    if not given:
+        out = gate.new_empty(shape)
+    pg, pv, po = _steps(gate, 'gate', shape, dt, at), _steps(value, 'value', shape, dt, at), _steps(out, 'out', shape, dt, at)
+    ph = _dense(h0, 'h0', (N, H), f32, at) if h0 is not None else None
+    pm = _masks(masks, (T, N), at)
     if given:
         _writable(out, 'out')
         for b in (gate, value, h0, masks):
             _no_overlap(out, b, 'gated_scan_fwd: out and an input')
     L = _hip.lib()
-    last = torch.empty(N, H, dtype=f32, device=dev)
-    saved = torch.empty(-(-T // L.acktr_gated_scan_save_interval()), N, H, dtype=f32, device=dev) if save else None
-    with _on(dev):
-        nb = L.acktr_gated_scan_workspace_bytes(T, N, H, code)
-        ws = _scratch(nb, dev, 'acktr_gated_scan_fwd')
-        with _Timed('gated_scan_fwd', 10.0 * T * N * H):
-            rc = L.acktr_gated_scan_fwd(*pg, *pv, ph, pm, *po, last.data_ptr(), saved.data_ptr() if save else None, T, N, H, code,
-                                        ws.data_ptr() if ws is not None else None, nb, _hip.cur_stream(dev))
-    _hip.check(rc, 'acktr_gated_scan_fwd')
+    last = gate.new_empty((N, H), dtype=f32)
+    saved = gate.new_empty((-(-T // L.acktr_gated_scan_save_interval()), N, H), dtype=f32) if save else None
+    nb = L.acktr_gated_scan_workspace_bytes(T, N, H, code)
+    ws = _scratch(nb, gate, 'acktr_gated_scan_fwd') if nb else None
+    _launch(L.acktr_gated_scan_fwd, (*pg, *pv, ph, pm, *po, last.data_ptr(), saved.data_ptr() if save else None, T, N, H, code,
+                                     ws.data_ptr() if nb else None, nb), at, 'gated_scan_fwd', 10.0 * T * N * H)
     return out, last, saved
 
 
@@ -686,18 +717,19 @@ def gated_scan_bwd(dout, gate, value, h0=None, masks=None, saved=None, dlast=Non
     code = _dtype_code(gate, 'gate')
     if gate.dim() != 3 or gate.shape[2] < 1:
         raise RuntimeError('gated_scan_bwd: gate [T, N, H] expected, got %s' % (tuple(gate.shape),))
-    (T, N, H), dt, dev = gate.shape, gate.dtype, gate.device
+    shape, dt, at = gate.shape, gate.dtype, gate.get_device()
+    T, N, H = shape
     given = [t for t in (dgate, dvalue) if t is not None]
-    dgate = torch.empty(T, N, H, dtype=dt, device=dev) if dgate is None else dgate
-    dvalue = torch.empty(T, N, H, dtype=dt, device=dev) if dvalue is None else dvalue
-    pd, pg, pv, qg, qv = (_steps(t, n, (T, N, H), dt, dev) for t, n in
-                          ((dout, 'dout'), (gate, 'gate'), (value, 'value'), (dgate, 'dgate'), (dvalue, 'dvalue')))
+    dgate = gate.new_empty(shape) if dgate is None else dgate
+    dvalue = gate.new_empty(shape) if dvalue is None else dvalue
+    pd, pg, pv = _steps(dout, 'dout', shape, dt, at), _steps(gate, 'gate', shape, dt, at), _steps(value, 'value', shape, dt, at)
+    qg, qv = _steps(dgate, 'dgate', shape, dt, at), _steps(dvalue, 'dvalue', shape, dt, at)
     L = _hip.lib()
     every = L.acktr_gated_scan_save_interval()
-    ph = _dense(h0, 'h0', (N, H), f32, dev) if h0 is not None else None
-    pm = _masks(masks, T, N, dev)
-    ps = _dense(saved, 'saved', (-(-T // every), N, H), f32, dev) if saved is not None and T else None
-    pl = _dense(dlast, 'dlast', (N, H), f32, dev) if dlast is not None else None
+    ph = _dense(h0, 'h0', (N, H), f32, at) if h0 is not None else None
+    pm = _masks(masks, (T, N), at)
+    ps = _dense(saved, 'saved', (-(-T // every), N, H), f32, at) if saved is not None and T else None
+    pl = _dense(dlast, 'dlast', (N, H), f32, at) if dlast is not None else None
     if T > every and saved is None:
         raise RuntimeError('gated_scan_bwd: more than %d steps need what gated_scan_fwd(save=True) saved' % every)
     for a in given:
@@ -706,14 +738,11 @@ def gated_scan_bwd(dout, gate, value, h0=None, masks=None, saved=None, dlast=Non
             _no_overlap(a, b, 'gated_scan_bwd: a gradient and an input')
     if len(given) == 2:
         _no_overlap(dgate, dvalue, 'gated_scan_bwd: dgate and dvalue')
-    dh0 = torch.empty(N, H, dtype=f32, device=dev) if need_dh0 else None
-    with _on(dev):
-        nb = L.acktr_gated_scan_workspace_bytes(T, N, H, code)
-        ws = _scratch(nb, dev, 'acktr_gated_scan_bwd')
-        with _Timed('gated_scan_bwd', 20.0 * T * N * H):
-            rc = L.acktr_gated_scan_bwd(*pd, *pg, *pv, ph, pm, ps, pl, *qg, *qv, dh0.data_ptr() if need_dh0 else None, T, N, H, code,
-                                        ws.data_ptr() if ws is not None else None, nb, _hip.cur_stream(dev))
-    _hip.check(rc, 'acktr_gated_scan_bwd')
+    dh0 = gate.new_empty((N, H), dtype=f32) if need_dh0 else None
+    nb = L.acktr_gated_scan_workspace_bytes(T, N, H, code)
+    ws = _scratch(nb, gate, 'acktr_gated_scan_bwd') if nb else None
+    _launch(L.acktr_gated_scan_bwd, (*pd, *pg, *pv, ph, pm, ps, pl, *qg, *qv, dh0.data_ptr() if need_dh0 else None, T, N, H, code,
+                                     ws.data_ptr() if nb else None, nb), at, 'gated_scan_bwd', 20.0 * T * N * H)
     return dgate, dvalue, dh0
 
 
@@ -723,20 +752,19 @@ def gated_scan_step(gate, value, state, masks=None, out=None):
     code = _dtype_code(gate, 'gate')
     if gate.dim() != 2 or gate.shape[1] < 1:
         raise RuntimeError('gated_scan_step: gate [N, H] expected, got %s' % (tuple(gate.shape),))
-    (N, H), dt, dev = gate.shape, gate.dtype, gate.device
+    shape, dt, at = gate.shape, gate.dtype, gate.get_device()
+    N, H = shape
     given = out is not None
-    if out is None:
-        out = torch.empty(N, H, dtype=dt, device=dev)
-    (pg, gn), (pv, vn), (po, on) = (_rows(t, n, (N, H), dt, dev) for t, n in ((gate, 'gate'), (value, 'value'), (out, 'out')))
-    ps = _dense(state, 'state', (N, H), f32, dev)
-    pm = _masks(masks.reshape(1, -1), 1, N, dev) if masks is not None else None
+    if not given:
+        out = gate.new_empty(shape)
+    (pg, gn), (pv, vn), (po, on) = _rows(gate, 'gate', shape, dt, at), _rows(value, 'value', shape, dt, at), _rows(out, 'out', shape, dt, at)
+    ps = _dense(state, 'state', shape, f32, at)
+    pm = _masks(masks, (N,), at)
     if given:
         _writable(out, 'out')
         for b in (gate, value, state, masks):
             _no_overlap(out, b, 'gated_scan_step: out and an input')
     for b in (gate, value, masks):
         _no_overlap(state, b, 'gated_scan_step: state and an input')
-    with _on(dev):
-        rc = _hip.lib().acktr_gated_scan_step(pg, gn, pv, vn, ps, pm, po, on, N, H, code, _hip.cur_stream(dev))
-    _hip.check(rc, 'acktr_gated_scan_step')
+    _launch(_hip.lib().acktr_gated_scan_step, (pg, gn, pv, vn, ps, pm, po, on, N, H, code), at, 'gated_scan_step', 10.0 * N * H)
     return out

@@ -491,7 +491,7 @@ extern "C" long acktr_gated_scan_workspace_bytes(long T, long N, long H, int dty
         const ScanPlan p = scan_plan(T, N, H, (int)elem_bytes(dtype), wide != 0);
         if (p.blocks > 1) most = max(most, 8L * p.blocks * N * H);
     }
-    return most + 16;
+    return most;
 }
 
 extern "C" int acktr_gated_scan_fwd(const void* gate, long gt, long gn, const void* value, long vt, long vn, const float* h0,

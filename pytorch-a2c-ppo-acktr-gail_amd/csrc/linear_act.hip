@@ -3,176 +3,9 @@
 // Three products over the same tile kernel (tile_gemm.hpp), which reads each operand as it lies: forward k | k contiguous, input
 // gradient k | rows, weight gradient rows | rows.
 #include "act_terms.hpp"
-#include "tile_gemm.hpp"
+#include "linear_act.hpp"
 
 namespace acktr {
-
-struct LinArgs {
-    const void *a, *b;                  // A: M x K, B: N x K
-    long lda, ldb;
-    int M, N, K;
-    void* y;
-    long ldy;
-    const void *bias, *res;             // nullable
-    void* pre;                          // slopes for the backward pass; nullable
-    long ldr, ldp;
-    int act, vec;                       // vec: 16-byte stores of 8 columns are possible everywhere
-    float* slabs;                       // split reduction: fp32 partial products [slices][M][N] instead of y
-    int kslice;                         // k per slice (a multiple of the K step), K without a split
-    int tiles_m, tiles_n;
-};
-
-// act(v + bias) + res for 8 columns n.. of row m, and their stores.  v: the product.
-template <class T, int ACT, bool SLOPE>
-__device__ __forceinline__ void finish8(const LinArgs& p, int m, int n, float (&v)[8]) {
-    typedef vec_t<T, 8> v8;
-    typedef typename SlopeOf<T>::type ST;
-    typedef vec_t<ST, 8> s8;
-    if (p.vec) {                                             // N is a multiple of 8 then
-        if (p.bias) {
-            const v8 b = *reinterpret_cast<const v8*>((const T*)p.bias + n);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] += to_f32(b[i]);
-        }
-        v8 r, y;
-        s8 z;
-        if (p.res) r = *reinterpret_cast<const v8*>((const T*)p.res + (long)m * p.ldr + n);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            float slope;
-            float o = act_of<ACT, SLOPE>(v[i], slope);
-            if (p.res) o += to_f32(r[i]);
-            y[i] = from_f32<T>(o);
-            if (SLOPE) {
-                ST c;
-                put_slope(c, slope);
-                z[i] = c;
-            }
-        }
-        *reinterpret_cast<v8*>((T*)p.y + (long)m * p.ldy + n) = y;
-        if (SLOPE) *reinterpret_cast<s8*>((ST*)p.pre + (long)m * p.ldp + n) = z;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (n + i >= p.N) break;
-            float z = v[i], slope;
-            if (p.bias) z += to_f32(((const T*)p.bias)[n + i]);
-            float o = act_of<ACT, SLOPE>(z, slope);
-            if (p.res) o += to_f32(((const T*)p.res)[(long)m * p.ldr + n + i]);
-            ((T*)p.y)[(long)m * p.ldy + n + i] = from_f32<T>(o);
-            if (SLOPE) put_slope(((ST*)p.pre)[(long)m * p.ldp + n + i], slope);
-        }
-    }
-}
-template <class T>
-__device__ __forceinline__ void finish_any(const LinArgs& p, int m, int n, float (&v)[8]) {
-    if (p.pre) {
-        switch (p.act) {
-            case ACKTR_ACT_RELU: finish8<T, ACKTR_ACT_RELU, true>(p, m, n, v); break;
-            case ACKTR_ACT_TANH: finish8<T, ACKTR_ACT_TANH, true>(p, m, n, v); break;
-            case ACKTR_ACT_SILU: finish8<T, ACKTR_ACT_SILU, true>(p, m, n, v); break;
-            case ACKTR_ACT_GELU: finish8<T, ACKTR_ACT_GELU, true>(p, m, n, v); break;
-            default: finish8<T, ACKTR_ACT_NONE, true>(p, m, n, v);
-        }
-    } else {
-        switch (p.act) {
-            case ACKTR_ACT_RELU: finish8<T, ACKTR_ACT_RELU, false>(p, m, n, v); break;
-            case ACKTR_ACT_TANH: finish8<T, ACKTR_ACT_TANH, false>(p, m, n, v); break;
-            case ACKTR_ACT_SILU: finish8<T, ACKTR_ACT_SILU, false>(p, m, n, v); break;
-            case ACKTR_ACT_GELU: finish8<T, ACKTR_ACT_GELU, false>(p, m, n, v); break;
-            default: finish8<T, ACKTR_ACT_NONE, false>(p, m, n, v);
-        }
-    }
-}
-
-// FULL: bias / activation / residual; otherwise the product is stored as it is.
-template <class T, bool AKC, bool BKC, int BM, int BN, int WM, int WN, bool FULL>
-__global__ __launch_bounds__(WM * WN * 64, (BM * BN > 128 * 128 ? WM * WN / 4 : 2)) void linear_tile_kernel(const LinArgs p) {
-    typedef TileGemm<T, AKC, BKC, BM, BN, WM, WN> G;
-    extern __shared__ char smem[];
-    ACKTR_LDS char* sm = (ACKTR_LDS char*)smem;
-    // Neighbouring tiles share operand rows, so each of the 8 L2 caches (workgroups go to them in turn) gets a contiguous piece
-    // of the tile order, and the order walks blocks of 8 row tiles.
-    const int total = p.tiles_m * p.tiles_n, id = blockIdx.x;
-    const int per = (total + 7) / 8, full = total - 8 * (per - 1);            // XCDs 0 .. full-1 have `per` tiles, the others per-1
-    const int x = id & 7, q = id >> 3;
-    const int t = x < full ? x * per + q : full * per + (x - full) * (per - 1) + q;
-    const int band = t / (8 * p.tiles_n), inband = t % (8 * p.tiles_n);
-    const int rows_in = min(8, p.tiles_m - band * 8);
-    const int tm = band * 8 + inband % rows_in, tn = inband / rows_in;
-    const int m0 = tm * BM, n0 = tn * BN;
-    const int k0 = blockIdx.y * p.kslice, k1 = min(p.K, k0 + p.kslice);
-
-    G g;
-    g.run(p.a, p.lda, m0, p.M, p.b, p.ldb, n0, p.N, k0, k1, sm);
-
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = m0 + (wave / WN) * (BM / WM), wn = n0 + (wave % WN) * (BN / WN);
-    // The accumulators pass through a wave's own piece of LDS (P row blocks at a time) and come back as 8 consecutive columns of a
-    // row, so stores cover whole lines and the epilogue is one loop.  Row pitch + 4 floats: 16 rows meet 16 different bank groups.
-    constexpr int WTN = BN / WN, PITCH = WTN + 4, BLK = 16 * PITCH * 4;
-    constexpr int FIT = G::LDS / (WM * WN) / BLK;
-    constexpr int P = FIT >= G::MI ? G::MI : FIT >= 4 && G::MI % 4 == 0 ? 4 : FIT >= 2 && G::MI % 2 == 0 ? 2 : 1;
-    static_assert(FIT >= 1, "epilogue block");
-    constexpr int LPR = WTN / 8, RPI = 64 / LPR;                              // lanes a row, rows an iteration
-    __syncthreads();
-    ACKTR_LDS float* mine = reinterpret_cast<ACKTR_LDS float*>(sm) + wave * (P * BLK / 4);
-#pragma unroll
-    for (int base = 0; base < G::MI; base += P) {
-#pragma unroll
-        for (int i = 0; i < P; ++i)
-#pragma unroll
-            for (int j = 0; j < G::NI; ++j)
-                *reinterpret_cast<ACKTR_LDS f32v4*>(mine + (i * 16 + (lane & 15)) * PITCH + j * 16 + 4 * (lane >> 4)) = g.acc[base + i][j];
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                    // the wave's own piece: no barrier
-#pragma unroll 1
-        for (int r = lane / LPR; r < P * 16; r += RPI) {
-            const int m = wm + base * 16 + r, n = wn + (lane % LPR) * 8;
-            const f32v4 lo = *reinterpret_cast<ACKTR_LDS f32v4*>(mine + r * PITCH + (lane % LPR) * 8);
-            const f32v4 hi = *reinterpret_cast<ACKTR_LDS f32v4*>(mine + r * PITCH + (lane % LPR) * 8 + 4);
-            if (m >= p.M || n >= p.N) continue;
-            float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-            if (p.slabs) {
-                float* s = p.slabs + ((long)blockIdx.y * p.M + m) * p.N + n;
-                if (p.vec) {
-                    *reinterpret_cast<f32v4*>(s) = lo;
-                    *reinterpret_cast<f32v4*>(s + 4) = hi;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (n + i < p.N) s[i] = v[i];
-                }
-            } else if constexpr (FULL) {
-                finish_any<T>(p, m, n, v);
-            } else {
-                finish8<T, ACKTR_ACT_NONE, false>(p, m, n, v);
-            }
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    }
-}
-
-// Sum of the slices of a split reduction in slice order, then the epilogue.
-template <class T>
-__global__ __launch_bounds__(256) void linear_slabs_kernel(const LinArgs p, int slices) {
-    const int groups = (p.N + 7) / 8;
-    const long total = (long)p.M * groups;
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
-        const int m = (int)(i / groups), n = (int)(i % groups) * 8;
-        const float* s = p.slabs + (long)m * p.N + n;
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        for (int z = 0; z < slices; ++z, s += (long)p.M * p.N) {
-            if (p.vec) {
-                const f32v4 lo = *reinterpret_cast<const f32v4*>(s), hi = *reinterpret_cast<const f32v4*>(s + 4);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] += lo[j], v[4 + j] += hi[j];
-            } else {
-                for (int j = 0; j < 8 && n + j < p.N; ++j) v[j] += s[j];
-            }
-        }
-        finish_any<T>(p, m, n, v);
-    }
-}
 
 // dst[r][c] = src[r][c] for c < cols, 0 up to ldd: a copy whose rows start at 16-byte boundaries, for operands that do not
 // (an odd width, a slice of a wider row).  It costs one pass over the operand; reading such rows element by element in the
@@ -253,62 +86,6 @@ __global__ __launch_bounds__(256) void col_sums_kernel(const float* __restrict__
         for (int i = 1; i < 8; ++i) t += part[i][c];
         db[col] = from_f32<T>(t);
     }
-}
-
-// ---------------------------------------------------------------------------------------------------- host side
-constexpr int KSTEP_BYTES = 128, MAX_SLICES = 32, SUM_BLOCKS = 256;
-
-static inline long up(long v, long a) { return (v + a - 1) / a * a; }
-static inline bool rows16(const void* p, long ld, long e) { return ((uintptr_t)p & 15) == 0 && ld * e % 16 == 0; }
-
-// Tile and reduction split of an M x N x K product.
-struct Plan { int bm, bn, slices; long kslice; };
-static Plan plan_of(long M, long N, long K, int e) {
-    const long kt = KSTEP_BYTES / e, steps = (K + kt - 1) / kt;
-    Plan p{64, 64, 1, up(K, kt)};
-    const long t64 = (long)cdiv(M, 64) * cdiv(N, 64);
-    long want = 1;
-    if (t64 < 256 && steps > 8) want = min(min((long)cdiv(512, t64), steps / 4), (long)MAX_SLICES);
-    if (want > 1) {
-        p.kslice = up((steps + want - 1) / want, 1) * kt;
-        p.slices = cdiv(K, p.kslice);
-    }
-    return p;
-}
-
-template <class T, bool AKC, bool BKC, int BM, int BN, int WM, int WN, bool FULL>
-static int launch_tile(LinArgs& p, const Plan& pl, hipStream_t s) {
-    auto kern = linear_tile_kernel<T, AKC, BKC, BM, BN, WM, WN, FULL>;
-    constexpr int lds = TileGemm<T, AKC, BKC, BM, BN, WM, WN>::LDS;
-    if (lds > 65536) {
-        hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-        if (e != hipSuccess) {
-            set_error("linear_act: %d bytes of LDS refused: %s", lds, hipGetErrorString(e));
-            return (int)e;
-        }
-    }
-    p.tiles_m = cdiv(p.M, BM);
-    p.tiles_n = cdiv(p.N, BN);
-    kern<<<dim3((unsigned)(p.tiles_m * p.tiles_n), pl.slices), dim3(WM * WN * 64), lds, s>>>(p);
-    ACKTR_LAUNCH_CHECK();
-    return 0;
-}
-
-// One product with its epilogue; `slabs` holds the slices of a split reduction.
-template <class T, bool AKC, bool BKC, bool FULL>
-static int product(LinArgs p, float* slabs, hipStream_t s) {
-    const Plan pl = plan_of(p.M, p.N, p.K, sizeof(T));
-    p.kslice = (int)pl.kslice;
-    p.slabs = pl.slices > 1 ? slabs : nullptr;
-    const int rc = launch_tile<T, AKC, BKC, 64, 64, 2, 2, FULL>(p, pl, s);
-    if (rc || pl.slices == 1) return rc;
-    linear_slabs_kernel<T><<<min(cdiv((long)p.M * ((p.N + 7) / 8), 256), 2048), 256, 0, s>>>(p, pl.slices);
-    ACKTR_LAUNCH_CHECK();
-    return 0;
-}
-static long slab_bytes(long M, long N, long K, int e) {
-    const Plan pl = plan_of(M, N, K, e);
-    return pl.slices > 1 ? up(4 * M * N * pl.slices, 256) : 0;
 }
 
 template <class T>
@@ -409,7 +186,7 @@ extern "C" int acktr_linear_act_fwd(const void* x, long ldx, const void* w, long
             p.b = ws + sp.w, p.ldb = kp;
         }
         p.K = kp;
-        return product<T, true, true, true>(p, (float*)(ws + sp.slabs), s);
+        return linear_product<T>(LIN_FORWARD, p, (float*)(ws + sp.slabs), s);
     });
 }
 
@@ -485,7 +262,7 @@ extern "C" int acktr_linear_act_bwd(const void* dy, long lddy, const void* x, lo
             }
             p.M = (int)M, p.N = (int)K, p.K = (int)N;
             p.y = dx, p.ldy = lddx, p.vec = K % 8 == 0 && rows16(dx, lddx, e);
-            if (int rc = product<T, true, false, false>(p, slabs, s)) return rc;
+            if (int rc = linear_product<T>(LIN_DX, p, slabs, s)) return rc;
         }
         if (dw) {                                            // dw[N, K] = dz^T x: sum over M
             LinArgs p{};
@@ -496,7 +273,7 @@ extern "C" int acktr_linear_act_bwd(const void* dy, long lddy, const void* x, lo
             }
             p.M = (int)N, p.N = (int)K, p.K = (int)M;
             p.y = dw, p.ldy = K, p.vec = K % 8 == 0 && rows16(dw, K, e);
-            if (int rc = product<T, false, false, false>(p, slabs, s)) return rc;
+            if (int rc = linear_product<T>(LIN_DW, p, slabs, s)) return rc;
         }
         return 0;
     });

@@ -1,0 +1,6 @@
+// linear_act.hip's products on bf16 operands.
+#include "linear_act_kernels.hpp"
+
+namespace acktr {
+template int linear_product<__bf16>(LinKind, const LinArgs&, float*, hipStream_t);
+}

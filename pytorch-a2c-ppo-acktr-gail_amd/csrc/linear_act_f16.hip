@@ -1,0 +1,6 @@
+// linear_act.hip's products on fp16 operands.
+#include "linear_act_kernels.hpp"
+
+namespace acktr {
+template int linear_product<_Float16>(LinKind, const LinArgs&, float*, hipStream_t);
+}

@@ -1,0 +1,291 @@
+// Tile kernels of linear_act.hip and their launches.
+#pragma once
+#include <atomic>
+#include <type_traits>
+
+#include "act_terms.hpp"
+#include "linear_act.hpp"
+#include "tile_gemm.hpp"
+
+namespace acktr {
+
+// act(v + bias) + res for 8 columns n.. of row m, and their stores.  v: the product.  Vector form: N is a multiple of 8 and all rows
+// start at 16 bytes; bias and residual are already in registers (b, r; zero where there is none).
+template <class T, int ACT, bool SLOPE>
+__device__ __forceinline__ void finish8(const LinArgs& p, int m, int n, float (&v)[8], const float (&b)[8], const vec_t<T, 8>& r, bool res) {
+    typedef typename SlopeOf<T>::type ST;
+    vec_t<T, 8> y;
+    vec_t<ST, 8> z;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        float slope;
+        float o = act_of<ACT, SLOPE>(v[i] + b[i], slope);
+        if (res) o += to_f32(r[i]);
+        y[i] = from_f32<T>(o);
+        if (SLOPE) {
+            ST c;
+            put_slope(c, slope);
+            z[i] = c;
+        }
+    }
+    *reinterpret_cast<vec_t<T, 8>*>((T*)p.y + (long)m * p.ldy + n) = y;
+    if (SLOPE) *reinterpret_cast<vec_t<ST, 8>*>((ST*)p.pre + (long)m * p.ldp + n) = z;
+}
+// the same value by value, for widths and rows of any alignment
+template <class T, int ACT, bool SLOPE>
+__device__ __forceinline__ void finish8_any(const LinArgs& p, int m, int n, float (&v)[8]) {
+    typedef typename SlopeOf<T>::type ST;
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+        if (n + i >= p.N) break;
+        float z = v[0], slope;
+        if (p.bias) z += to_f32(((const T*)p.bias)[n + i]);
+        float o = act_of<ACT, SLOPE>(z, slope);
+        if (p.res) o += to_f32(((const T*)p.res)[(long)m * p.ldr + n + i]);
+        ((T*)p.y)[(long)m * p.ldy + n + i] = from_f32<T>(o);
+        if (SLOPE) put_slope(((ST*)p.pre)[(long)m * p.ldp + n + i], slope);
+#pragma unroll
+        for (int j = 0; j < 7; ++j) v[j] = v[j + 1];         // (the registers rotate: they have no address)
+    }
+}
+// f(activation code, whether slopes are wanted) as compile-time constants
+template <class F>
+__device__ __forceinline__ void with_act(const LinArgs& p, F&& f) {
+    using std::integral_constant;
+    auto both = [&](auto act) __attribute__((always_inline)) {
+        if (p.pre) f(act, std::true_type{});
+        else f(act, std::false_type{});
+    };
+    switch (p.act) {
+        case ACKTR_ACT_RELU: both(integral_constant<int, ACKTR_ACT_RELU>{}); break;
+        case ACKTR_ACT_TANH: both(integral_constant<int, ACKTR_ACT_TANH>{}); break;
+        case ACKTR_ACT_SILU: both(integral_constant<int, ACKTR_ACT_SILU>{}); break;
+        case ACKTR_ACT_GELU: both(integral_constant<int, ACKTR_ACT_GELU>{}); break;
+        default: both(integral_constant<int, ACKTR_ACT_NONE>{});
+    }
+}
+template <class T>
+__device__ __forceinline__ void load_bias8(const LinArgs& p, int n, float (&b)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) b[i] = 0.f;
+    if (p.bias && n < p.N) {
+        const vec_t<T, 8> x = *reinterpret_cast<const vec_t<T, 8>*>((const T*)p.bias + n);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b[i] = to_f32(x[i]);
+    }
+}
+
+// Row blocks [base, base + P) of the accumulators into LDS.  The registers of each turn are picked by comparison (they have no
+// address), so one copy of the epilogue serves all turns.
+template <class G, int P, int PITCH, int TURN>
+__device__ __forceinline__ void spill_turn(const f32v4 (&acc)[G::MI][G::NI], int base, ACKTR_LDS float* at) {
+    if (base == TURN) {
+#pragma unroll
+        for (int i = 0; i < P; ++i)
+#pragma unroll
+            for (int j = 0; j < G::NI; ++j) *reinterpret_cast<ACKTR_LDS f32v4*>(at + i * 16 * PITCH + j * 16) = acc[TURN + i][j];
+        asm volatile("; turn %0" ::"n"(TURN));               // keeps the turns' stores apart: merged, they would index the registers
+    }
+    if constexpr (TURN + P < G::MI) spill_turn<G, P, PITCH, TURN + P>(acc, base, at);
+}
+
+// FULL: bias / activation / residual; otherwise the product is stored as it is.
+template <class T, bool AKC, bool BKC, int BM, int BN, int WM, int WN, bool FULL>
+__global__ __launch_bounds__(WM * WN * 64, (BM * BN > 128 * 128 ? WM * WN / 4 : 2)) void linear_tile_kernel(const LinArgs p) {
+    typedef TileGemm<T, AKC, BKC, BM, BN, WM, WN> G;
+    extern __shared__ char smem[];
+    ACKTR_LDS char* sm = (ACKTR_LDS char*)smem;
+    // Neighbouring tiles share operand rows, so each of the 8 L2 caches (workgroups go to them in turn) gets a contiguous piece
+    // of the tile order, and the order walks blocks of 8 row tiles.
+    const int total = p.tiles_m * p.tiles_n, id = blockIdx.x;
+    const int per = (total + 7) / 8, full = total - 8 * (per - 1);            // XCDs 0 .. full-1 have `per` tiles, the others per-1
+    const int x = id & 7, q = id >> 3;
+    const int t = x < full ? x * per + q : full * per + (x - full) * (per - 1) + q;
+    const int band = t / (8 * p.tiles_n), inband = t % (8 * p.tiles_n);
+    const int rows_in = min(8, p.tiles_m - band * 8);
+    const int tm = band * 8 + inband % rows_in, tn = inband / rows_in;
+    const int m0 = tm * BM, n0 = tn * BN;
+    const int k0 = blockIdx.y * p.kslice, k1 = min(p.K, k0 + p.kslice);
+
+    G g;
+    g.run(p.a, p.lda, m0, p.M, p.b, p.ldb, n0, p.N, k0, k1, sm);
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = m0 + (wave / WN) * (BM / WM), wn = n0 + (wave % WN) * (BN / WN);
+    // The accumulators pass through a wave's own piece of LDS (P row blocks at a time) and come back as 8 consecutive columns of a
+    // row, so stores cover whole lines and the epilogue is one loop.  Row pitch + 4 floats: 16 rows meet 16 different bank groups.
+    constexpr int WTN = BN / WN, PITCH = WTN + 4, BLK = 16 * PITCH * 4;
+    constexpr int FIT = G::LDS / (WM * WN) / BLK;
+    constexpr int P = FIT >= G::MI ? G::MI : FIT >= 4 && G::MI % 4 == 0 ? 4 : FIT >= 2 && G::MI % 2 == 0 ? 2 : 1;
+    static_assert(FIT >= 1, "epilogue block");
+    constexpr int LPR = WTN / 8, RPI = 64 / LPR, IT = P * 16 / RPI;           // lanes a row, rows an iteration, iterations a turn
+    __syncthreads();
+    ACKTR_LDS float* mine = reinterpret_cast<ACKTR_LDS float*>(sm) + wave * (P * BLK / 4);
+    const int lr = lane / LPR, n = wn + (lane % LPR) * 8;
+    const ACKTR_LDS float* src = mine + lr * PITCH + (lane % LPR) * 8;
+    auto spill = [&](int base) __attribute__((always_inline)) {
+        spill_turn<G, P, PITCH, 0>(g.acc, base, mine + (lane & 15) * PITCH + 4 * (lane >> 4));
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                    // the wave's own piece: no barrier
+    };
+    auto fetch8 = [&](int k, float(&v)[8]) __attribute__((always_inline)) {
+        const f32v4 lo = *reinterpret_cast<const ACKTR_LDS f32v4*>(src + k * RPI * PITCH);
+        const f32v4 hi = *reinterpret_cast<const ACKTR_LDS f32v4*>(src + k * RPI * PITCH + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = lo[i], v[4 + i] = hi[i];
+    };
+    if (p.slabs || !p.vec) {
+#pragma unroll 1
+        for (int base = 0; base < G::MI; base += P) {
+            spill(base);
+#pragma unroll 1
+            for (int k = 0; k < IT; ++k) {
+                const int m = wm + base * 16 + k * RPI + lr;
+                float v[8];
+                fetch8(k, v);
+                if (m >= p.M || n >= p.N) continue;
+                if (p.slabs) {
+                    float* s = p.slabs + ((long)blockIdx.y * p.M + m) * p.N + n;
+                    if (p.vec) {
+                        *reinterpret_cast<f32v4*>(s) = f32v4{v[0], v[1], v[2], v[3]};
+                        *reinterpret_cast<f32v4*>(s + 4) = f32v4{v[4], v[5], v[6], v[7]};
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (n + i < p.N) s[i] = v[i];
+                    }
+                } else if constexpr (FULL) {
+                    with_act(p, [&](auto act, auto slope) { finish8_any<T, decltype(act)::value, decltype(slope)::value>(p, m, n, v); });
+                } else {
+                    finish8_any<T, ACKTR_ACT_NONE, false>(p, m, n, v);
+                }
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+        return;
+    }
+    auto finish = [&](auto act, auto slope) __attribute__((always_inline)) {
+        constexpr int ACT = decltype(act)::value;
+        constexpr bool SLOPE = decltype(slope)::value;
+        float b[8];
+        if constexpr (FULL) load_bias8<T>(p, n, b);
+        else
+            for (int i = 0; i < 8; ++i) b[i] = 0.f;
+        const bool res = FULL && p.res;
+        vec_t<T, 8> r[IT];
+        // a turn's residual rows are requested a turn ahead: their latency passes under the turn before
+        auto residual = [&](int base) __attribute__((always_inline)) {
+#pragma unroll
+            for (int k = 0; k < IT; ++k) {
+                const int m = wm + base * 16 + k * RPI + lr;
+                if (res && m < p.M && n < p.N) r[k] = *reinterpret_cast<const vec_t<T, 8>*>((const T*)p.res + (long)m * p.ldr + n);
+            }
+        };
+        residual(0);
+#pragma unroll 1
+        for (int base = 0; base < G::MI; base += P) {
+            spill(base);
+            vec_t<T, 8> now[IT];
+#pragma unroll
+            for (int k = 0; k < IT; ++k) now[k] = r[k];
+            if (base + P < G::MI) residual(base + P);
+#pragma unroll
+            for (int k = 0; k < IT; ++k) {
+                const int m = wm + base * 16 + k * RPI + lr;
+                float v[8];
+                fetch8(k, v);
+                if (m < p.M && n < p.N) finish8<T, ACT, SLOPE>(p, m, n, v, b, now[k], res);
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+    };
+    if constexpr (FULL) with_act(p, finish);
+    else finish(std::integral_constant<int, ACKTR_ACT_NONE>{}, std::false_type{});
+}
+
+// Sum of the slices of a split reduction in slice order, then the epilogue.
+template <class T>
+__global__ __launch_bounds__(256) void linear_slabs_kernel(const LinArgs p, int slices) {
+    const int groups = (p.N + 7) / 8;
+    const long total = (long)p.M * groups;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
+        const int m = (int)(i / groups), n = (int)(i % groups) * 8;
+        const float* s = p.slabs + (long)m * p.N + n;
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (int z = 0; z < slices; ++z, s += (long)p.M * p.N) {
+            if (p.vec) {
+                const f32v4 lo = *reinterpret_cast<const f32v4*>(s), hi = *reinterpret_cast<const f32v4*>(s + 4);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] += lo[j], v[4 + j] += hi[j];
+            } else {
+                for (int j = 0; j < 8 && n + j < p.N; ++j) v[j] += s[j];
+            }
+        }
+        if (p.vec) {
+            float b[8];
+            load_bias8<T>(p, n, b);
+            vec_t<T, 8> r;
+            if (p.res) r = *reinterpret_cast<const vec_t<T, 8>*>((const T*)p.res + (long)m * p.ldr + n);
+            with_act(p, [&](auto act, auto slope) { finish8<T, decltype(act)::value, decltype(slope)::value>(p, m, n, v, b, r, p.res); });
+        } else {
+            with_act(p, [&](auto act, auto slope) { finish8_any<T, decltype(act)::value, decltype(slope)::value>(p, m, n, v); });
+        }
+    }
+}
+
+template <class T, bool AKC, bool BKC, int BM, int BN, int WM, int WN, bool FULL>
+static int launch_tile(LinArgs& p, const Plan& pl, hipStream_t s) {
+    auto kern = linear_tile_kernel<T, AKC, BKC, BM, BN, WM, WN, FULL>;
+    constexpr int lds = TileGemm<T, AKC, BKC, BM, BN, WM, WN>::LDS;
+    if (lds > 65536) {                                       // once per kernel and device
+        static std::atomic<unsigned> allowed{0};
+        int dev = 0;
+        hipError_t e = hipGetDevice(&dev);
+        if (e == hipSuccess && !(allowed.load(std::memory_order_relaxed) >> (dev & 31) & 1u)) {
+            e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+            if (e == hipSuccess) allowed.fetch_or(1u << (dev & 31), std::memory_order_relaxed);
+        }
+        if (e != hipSuccess) {
+            set_error("linear_act: %d bytes of LDS refused: %s", lds, hipGetErrorString(e));
+            return (int)e;
+        }
+    }
+    p.tiles_m = cdiv(p.M, BM);
+    p.tiles_n = cdiv(p.N, BN);
+    kern<<<dim3((unsigned)(p.tiles_m * p.tiles_n), pl.slices), dim3(WM * WN * 64), lds, s>>>(p);
+    ACKTR_LAUNCH_CHECK();
+    return 0;
+}
+
+template <class T, bool AKC, bool BKC, bool FULL>
+static int product(LinArgs p, float* slabs, hipStream_t s) {
+    const Plan pl = plan_of(p.M, p.N, p.K, sizeof(T));
+    p.kslice = (int)pl.kslice;
+    p.slabs = pl.slices > 1 ? slabs : nullptr;
+    int rc;
+    if constexpr (sizeof(T) == 4) {
+        if (pl.tile == 0) rc = launch_tile<T, AKC, BKC, 64, 64, 2, 2, FULL>(p, pl, s);
+        else rc = launch_tile<T, AKC, BKC, 128, 64, 2, 2, FULL>(p, pl, s);
+    } else {
+        switch (pl.tile) {
+            case 0: rc = launch_tile<T, AKC, BKC, 64, 64, 2, 2, FULL>(p, pl, s); break;
+            case 1: rc = launch_tile<T, AKC, BKC, 128, 64, 2, 2, FULL>(p, pl, s); break;
+            case 2: rc = launch_tile<T, AKC, BKC, 128, 128, 2, 2, FULL>(p, pl, s); break;
+            default: rc = launch_tile<T, AKC, BKC, 256, 256, 2, 4, FULL>(p, pl, s);
+        }
+    }
+    if (rc || pl.slices == 1) return rc;
+    linear_slabs_kernel<T><<<min(cdiv((long)p.M * ((p.N + 7) / 8), 256), 2048), 256, 0, s>>>(p, pl.slices);
+    ACKTR_LAUNCH_CHECK();
+    return 0;
+}
+
+template <class T>
+int linear_product(LinKind kind, const LinArgs& p, float* slabs, hipStream_t s) {
+    switch (kind) {
+        case LIN_FORWARD: return product<T, true, true, true>(p, slabs, s);
+        case LIN_DX: return product<T, true, false, false>(p, slabs, s);
+        default: return product<T, false, false, false>(p, slabs, s);
+    }
+}
+
+}  // namespace acktr

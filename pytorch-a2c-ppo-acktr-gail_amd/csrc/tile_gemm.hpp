@@ -162,6 +162,19 @@ struct TileGemm {
 #pragma unroll
             for (int i = 0; i < MI; ++i) acc[i][j] = mfma_half(fb[j], fa[i], acc[i][j], T{});
     }
+    // Order of a half step: its LDS reads are spread over its products instead of being gathered where registers are scarcest
+    // (the compiler's own order leaves their latency in front of the next half).
+    __device__ __forceinline__ void interleave() {
+        constexpr int PER = sizeof(T) == 4 ? 4 : 1;
+        constexpr int READS = MI * (AKC ? 1 : sizeof(T) == 4 ? 4 : 2) + NI * (BKC ? 1 : sizeof(T) == 4 ? 4 : 2), PRODUCTS = MI * NI * PER;
+        constexpr int EACH = PRODUCTS >= 2 * READS ? PRODUCTS * 3 / 4 / READS : 1;
+#pragma unroll
+        for (int i = 0; i < READS; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS, 0);
+    }
     __device__ __forceinline__ void run(const void* a, long lda, int m0, int M, const void* b, long ldb, int n0, int N, int k0, int k1,
                                         ACKTR_LDS char* sm) {
         const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -192,11 +205,13 @@ struct TileGemm {
         for (int t = 0; t + 1 < steps; ++t) {
             frags(sm + cur, 1, wm, wn, lane, fa1, fb1);
             products(fa0, fb0);
+            interleave();
             tile_sync();                                 // this stage is read, the other one has arrived
             if (t + 2 < steps) request(cur);
             cur ^= STAGE;
             frags(sm + cur, 0, wm, wn, lane, fa0, fb0);
             products(fa1, fb1);
+            interleave();
         }
         frags(sm + cur, 1, wm, wn, lane, fa1, fb1);
         products(fa0, fb0);
