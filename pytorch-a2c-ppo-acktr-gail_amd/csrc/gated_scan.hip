@@ -6,38 +6,49 @@
 // into pieces that are composed in parallel, the pieces' states follow from a short scan over them, and a second walk over the
 // piece -- its inputs still in registers -- gives every state.  One read of each input, one write of each output.
 //
-// A workgroup owns CT = LC * V neighbouring channels (n, h flattened) and walks time in superchunks of NW * (64 / LC) * L steps: each
-// thread holds L consecutive steps of V channels.  States, products and sums are fp32 whatever the storage type.
+// A wave owns 64 * V neighbouring channels (n, h flattened; V a lane) and 16 consecutive steps; the waves of a workgroup follow one
+// another in time, and the workgroup walks on in superchunks of 16 steps a wave.  A whole wave per step keeps loads and stores in full
+// lines, addresses in scalar registers (one 32-bit offset a lane serves all steps) and the composition free of cross-lane traffic:
+// waves meet in LDS once a superchunk.  The next superchunk's inputs are requested before the present one is worked on.
+// States, products and sums are fp32 whatever the storage type.
+#include <type_traits>
+
 #include "act_terms.hpp"
 #include "half_types.hpp"
 
 namespace acktr {
 
-constexpr int SCAN_L = 8;
+constexpr int SCAN_L = 16;
+constexpr int SCAN_SAVE = 64;                       // steps between saved states; divides the superchunk of more than 64 steps
 
-// restart-safe product: a zero factor drops the other one even if it is not finite
-__device__ __forceinline__ float cut_mul(float a, float x) { return a == 0.f ? 0.f : a * x; }
+// A value as the compiler sees it for the first time: what was derived from it before is derived again rather than kept in a register.
+template <class X>
+__device__ __forceinline__ void forget(X& x) {
+    typedef typename std::conditional<sizeof(X) == 8, unsigned long, typename std::conditional<sizeof(X) == 4, unsigned, unsigned short>::type>::type U;
+    U u = __builtin_bit_cast(U, x);
+    asm volatile("" : "+v"(u));
+    x = __builtin_bit_cast(X, u);
+}
 
-// f = 1 / (1 + e^-x) and 1 - f without cancellation; e = exp(-|x|) <= 1 never overflows.  The product |x| log2(e) is carried
-// with its rounding error: without it e is off by |x| * 6e-8.
+// product that is 0 where a factor is, even if the other one is not finite: what a mask of 0 drops leaves no trace
+extern "C" __device__ float acktr_mul_legacy(float, float) __asm("llvm.amdgcn.fmul.legacy");      // v_mul_legacy_f32
+__device__ __forceinline__ float cut_mul(float a, float x) { return acktr_mul_legacy(a, x); }
+
+// f = 1 / (1 + e^-x) and 1 - f = e^-x f, both relative to their own size.  x is held above -87, where f is fp32's smallest normal number
+// and e^-x still finite (maximum() keeps a NaN).  ACC (fp32 storage): the product x log2(e) is carried with its rounding error,
+// without which e^-x is off by |x| 6e-8 -- nothing beside the rounding of a 16-bit x.
+template <bool ACC>
 __device__ __forceinline__ void gate_of(float x, float& f, float& nf) {
-    const float a = -fabsf(x), p = a * LOG2E, lo = fmaf(a, LOG2E, -p) + a * 1.92596299e-8f;
-    const float e0 = __builtin_amdgcn_exp2f(p), e = fmaf(e0, lo * 0.693147182f, e0), r = fast_rcp(1.f + e);
-    const float small = e * r;
-    f = x < 0.f ? small : r;
-    nf = x < 0.f ? r : small;
+    x = __builtin_elementwise_maximum(x, -87.f);
+    const float p = x * -LOG2E;
+    float e = __builtin_amdgcn_exp2f(p);
+    if (ACC) {
+        const float lo = fmaf(x, -LOG2E, -p) + x * -1.92596299e-8f;
+        e = fmaf(e, lo * 0.693147182f, e);
+    }
+    f = fast_rcp(1.f + e);
+    nf = e * f;
 }
-
-// both halves of a gate in one register: the smaller one, with the sign bit set where it is f
-__device__ __forceinline__ float gate_pack(float x, float f, float nf) { return x < 0.f ? -f : nf; }
-__device__ __forceinline__ void gate_unpack(float s, float& f, float& nf) {
-    const bool neg = __float_as_uint(s) >> 31;
-    const float a = fabsf(s), b = 1.f - a;
-    f = neg ? a : b;
-    nf = neg ? b : a;
-}
-
-constexpr int SCAN_SAVE = 64;                       // steps between saved states; divides every superchunk of more than 32 steps
 
 struct ScanArgs {
     const void *gate, *value, *dout;
@@ -53,184 +64,245 @@ struct ScanArgs {
     int T, N, H, blocks, block_steps;               // block_steps: a multiple of the superchunk
 };
 
-template <class T, int V, int LC, int NW>
-struct Scan {
-    static constexpr int NT = NW * 64, GW = 64 / LC, CT = LC * V, SC = NW * GW * SCAN_L;
-    typedef vec_t<T, V> vv;
+// How a tile's channels lie: WHOLE: all in one sequence (H is a multiple of the tile, or N is 1), so masks are scalars; MIXED: of
+// several; FAR: MIXED with offsets that need 64 bits.
+enum ScanMode { SCAN_WHOLE, SCAN_MIXED, SCAN_FAR };
 
-    int lane, wave, group, c, n, j, chl;            // chl: channel within the tile
+template <class T, int V, int NW, int MODE>
+struct Scan {
+    static constexpr bool FAR = MODE == SCAN_FAR;
+    static constexpr int CT = 64 * V, SC = NW * SCAN_L;
+    typedef vec_t<T, V> vv;
+    typedef vec_t<float, 2 * V> pairs;
+
+    int lane, wave, c, dn, j, n0;                    // n0: the tile's first sequence, dn: this lane's, counted from there
     bool live;
 
     __device__ __forceinline__ void place(const ScanArgs& p) {
         lane = threadIdx.x & 63;
-        wave = threadIdx.x >> 6;
-        group = wave * GW + lane / LC;
-        chl = (lane % LC) * V;
-        const long cc = (long)blockIdx.x * CT + chl;
-        live = cc < (long)p.N * p.H;
-        c = live ? (int)cc : 0;
-        n = c / p.H;
-        j = c - n * p.H;
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const long first = (long)blockIdx.x * CT, C = (long)p.N * p.H;
+        live = first + lane * V < C;
+        c = (int)(live ? first + lane * V : first);
+        n0 = (int)(first / p.H);
+        if constexpr (MODE == SCAN_WHOLE) {
+            dn = 0;
+            j = c - n0 * p.H;
+        } else {
+            const int n = c / p.H;
+            dn = n - n0;
+            j = c - n * p.H;
+        }
     }
-    __device__ __forceinline__ static vv load(const void* base, long off) { return *reinterpret_cast<const vv*>((const T*)base + off); }
-
-    // (A, B): this thread's composed piece, in group order (REV: in descending order).  Returns the state at the piece's start in `in`
-    // and moves `carry` behind the last piece.  sm: [NW][CT][2] floats; the caller alternates two of them.
-    template <bool REV>
-    __device__ __forceinline__ void exchange(float (&A)[V], float (&B)[V], float (&carry)[V], float (&in)[V], float* sm) {
+    // A [T, N, H] operand as this lane sees it, from step t on: a buffer whose base and step offsets are uniform (scalar registers), so
+    // that one 32-bit offset a lane is all the addressing there is; FAR: plain 64-bit addresses.
+    struct Rows {
+        const char* base;                            // uniform: sequence n0
+        long step;                                   // bytes a step
+        typename std::conditional<FAR, long, int>::type off;
+    };
+    struct Window {
+        __amdgpu_buffer_rsrc_t rsrc;
+        const char* base;
+        long step;
+        typename std::conditional<FAR, long, int>::type off;
+        __device__ __forceinline__ vv load(int l) const {
+            if constexpr (FAR) return *reinterpret_cast<const vv*>(base + l * step + off);
+            else if constexpr (sizeof(vv) == 2) return __builtin_bit_cast(vv, __builtin_amdgcn_raw_buffer_load_b16(rsrc, off, l * (int)step, 0));
+            else if constexpr (sizeof(vv) == 4) return __builtin_bit_cast(vv, __builtin_amdgcn_raw_buffer_load_b32(rsrc, off, l * (int)step, 0));
+            else return __builtin_bit_cast(vv, __builtin_amdgcn_raw_buffer_load_b64(rsrc, off, l * (int)step, 0));
+        }
+        __device__ __forceinline__ void store(int l, const vv& v) const {
+            typedef unsigned u2 __attribute__((ext_vector_type(2)));
+            if constexpr (FAR) *reinterpret_cast<vv*>(const_cast<char*>(base) + l * step + off) = v;
+            else if constexpr (sizeof(vv) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, v), rsrc, off, l * (int)step, 0);
+            else if constexpr (sizeof(vv) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), rsrc, off, l * (int)step, 0);
+            else __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u2, v), rsrc, off, l * (int)step, 0);
+        }
+    };
+    __device__ __forceinline__ Rows rows(const void* p, long st, long sn) const {
+        Rows r;
+        r.base = (const char*)p + n0 * sn * (long)sizeof(T);
+        r.step = st * (long)sizeof(T);
+        r.off = (typename std::conditional<FAR, long, int>::type)((dn * sn + j) * (long)sizeof(T));
+        return r;
+    }
+    __device__ __forceinline__ static Window at(const Rows& r, int t) {
+        Window w;
+        w.base = r.base + t * r.step;
+        w.step = r.step;
+        w.off = r.off;
+        if constexpr (!FAR) w.rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(w.base), 0, 0xffffffff, 0x00020000);
+        return w;
+    }
+    // steps [t, t + SCAN_L) of the inputs.  What lies behind the end (te), or in lanes without channels, becomes a step that changes
+    // nothing: a gate of 200 (f = 1, 1 - f = 0), a value, a derivative of 0, a mask of 1.
+    template <bool VALUES, bool DOUTS>
+    __device__ __forceinline__ void fetch(const ScanArgs& p, const Rows& rg, const Rows& rv, const Rows& rd, int t, int te, bool all,
+                                          vv (&g)[SCAN_L], vv (&v)[SCAN_L], vv (&d)[SCAN_L]) const {
+        const Window wg = at(rg, t), wv = at(rv, t), wd = at(rd, t);
+        const int left = te - t;
+        if (all && left >= SCAN_L) {
 #pragma unroll
-        for (int d = LC; d < 64; d *= 2) {
-            const bool has = REV ? lane + d < 64 : lane >= d;
+            for (int l = 0; l < SCAN_L; ++l) {
+                g[l] = wg.load(l);
+                if (VALUES) v[l] = wv.load(l);
+                if (DOUTS) d[l] = wd.load(l);
+            }
+        } else {
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float pa = REV ? __shfl_down(A[i], d, 64) : __shfl_up(A[i], d, 64);
-                const float pb = REV ? __shfl_down(B[i], d, 64) : __shfl_up(B[i], d, 64);
-                if (has) {
-                    B[i] += cut_mul(A[i], pb);
-                    A[i] *= pa;
+            for (int l = 0; l < SCAN_L; ++l) {
+                g[l] = vv((T)200.f), v[l] = vv((T)0.f), d[l] = vv((T)0.f);
+                if (l < left && live) {
+                    g[l] = wg.load(l);
+                    if (VALUES) v[l] = wv.load(l);
+                    if (DOUTS) d[l] = wd.load(l);
                 }
             }
         }
-        const bool edge = REV ? lane < LC : lane >= 64 - LC;             // holds the wave's whole composition
-        if (edge) {
+    }
+    // (not requested ahead: they would hold registers for a whole superchunk; they are on their way while the inputs are waited for)
+    __device__ __forceinline__ void masks(const ScanArgs& p, int t, int te, float (&m)[SCAN_L]) const {
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                sm[(wave * CT + chl + i) * 2] = A[i];
-                sm[(wave * CT + chl + i) * 2 + 1] = B[i];
+        for (int l = 0; l < SCAN_L; ++l) m[l] = 1.f;
+        if (p.masks) {
+            const float* q = p.masks + (long)t * p.N + n0;
+            if (te - t >= SCAN_L) {
+#pragma unroll
+                for (int l = 0; l < SCAN_L; ++l) m[l] = q[(long)l * p.N + dn];
+            } else {
+#pragma unroll
+                for (int l = 0; l < SCAN_L; ++l)
+                    if (l < te - t) m[l] = q[(long)l * p.N + dn];
             }
         }
-        float ea[V], eb[V];
+    }
+    __device__ __forceinline__ void put(const Rows& r, int t, int te, bool all, const vv (&o)[SCAN_L]) const {
+        const Window w = at(r, t);
+        const int left = te - t;
+        if (all && left >= SCAN_L) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            ea[i] = 1.f, eb[i] = 0.f;
-            if (LC < 64) {
-                const float pa = REV ? __shfl_down(A[i], LC, 64) : __shfl_up(A[i], LC, 64);
-                const float pb = REV ? __shfl_down(B[i], LC, 64) : __shfl_up(B[i], LC, 64);
-                const bool first = REV ? lane >= 64 - LC : lane < LC;
-                if (!first) ea[i] = pa, eb[i] = pb;
-            }
+            for (int l = 0; l < SCAN_L; ++l) w.store(l, o[l]);
+        } else if (live) {
+#pragma unroll
+            for (int l = 0; l < SCAN_L; ++l)
+                if (l < left) w.store(l, o[l]);
         }
+    }
+
+    // (A, B): this wave's composed steps (REV: in descending order).  Returns the state at their start in `in` and moves `carry`
+    // behind the last wave; PROD: `prod` collects the product of all A.  sm: NW * CT * 2 floats; the caller alternates two of them.
+    template <bool REV, bool PROD>
+    __device__ __forceinline__ void exchange(const float (&A)[V], const float (&B)[V], float (&carry)[V], float (&in)[V], float (&prod)[V],
+                                             pairs* sm) const {
+        pairs mine;
+#pragma unroll
+        for (int i = 0; i < V; ++i) mine[2 * i] = A[i], mine[2 * i + 1] = B[i];
+        sm[wave * 64 + lane] = mine;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            float h = carry[i], mine = h;
+        for (int k = 0; k < NW; ++k) {
+            const int w = REV ? NW - 1 - k : k;
+            if (w == wave) {
 #pragma unroll
-            for (int k = 0; k < NW; ++k) {
-                const int w = REV ? NW - 1 - k : k;
-                if (w == wave) mine = h;
-                const float a = sm[(w * CT + chl + i) * 2], b = sm[(w * CT + chl + i) * 2 + 1];
-                h = cut_mul(a, h) + b;
+                for (int i = 0; i < V; ++i) in[i] = carry[i];
             }
-            carry[i] = h;
-            in[i] = cut_mul(ea[i], mine) + eb[i];
+            const pairs q = sm[w * 64 + lane];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                carry[i] = cut_mul(q[2 * i], carry[i]) + q[2 * i + 1];
+                if (PROD) prod[i] = cut_mul(q[2 * i], prod[i]);
+            }
         }
+    }
+    // the blocks before this one (REV: behind it, last to first), composed: `carry` moves over them.  A contiguous range per wave.
+    template <bool REV>
+    __device__ __forceinline__ void skip_blocks(const ScanArgs& p, int blk, float (&carry)[V], pairs* sm) const {
+        const long C = (long)p.N * p.H;
+        const int cnt = REV ? p.blocks - 1 - blk : blk, per = (cnt + NW - 1) / NW;
+        const int r = REV ? NW - 1 - wave : wave, b0 = min(cnt, r * per), b1 = min(cnt, b0 + per);
+        float A[V], B[V], in[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) A[i] = 1.f, B[i] = 0.f;
+#pragma unroll 4
+        for (int b = b0; b < b1; ++b) {
+            const float* q = p.agg + 2L * (REV ? p.blocks - 1 - b : b) * C + c;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                B[i] = cut_mul(q[i], B[i]) + q[C + i];
+                A[i] = cut_mul(q[i], A[i]);
+            }
+        }
+        exchange<REV, false>(A, B, carry, in, in, sm);
     }
 };
 
 // --------------------------------------------------------------------------------------------------------- forward
 // AGG: only the block's composition is formed (first pass of a time split).
-template <class T, int V, int LC, int NW, bool AGG>
+template <class T, int V, int NW, int MODE, bool AGG>
 __global__ __launch_bounds__(NW * 64) void scan_fwd_kernel(const ScanArgs p) {
-    typedef Scan<T, V, LC, NW> S;
+    typedef Scan<T, V, NW, MODE> S;
     typedef typename S::vv vv;
-    __shared__ float sm[2][NW * S::CT * 2];
+    __shared__ typename S::pairs sm[2][NW * 64];
     S s;
     s.place(p);
     const long C = (long)p.N * p.H;
     const int blk = blockIdx.y, tb = blk * p.block_steps, te = min(p.T, tb + p.block_steps);
-    float carry[V];
+    const typename S::Rows rg = s.rows(p.gate, p.gt, p.gn), rv = s.rows(p.value, p.vt, p.vn), ro = s.rows(p.out, p.ot, p.on);
+    const bool all = (long)(blockIdx.x + 1) * S::CT <= C;    // every lane of the tile has channels
+    float carry[V], prod[V];
     int par = 0;
 #pragma unroll
-    for (int i = 0; i < V; ++i) carry[i] = !AGG && p.h0 && s.live ? p.h0[s.c + i] : 0.f;
-    if (!AGG && p.blocks > 1) {                              // the blocks before this one, composed: a contiguous range per group
-        const int G = NW * S::GW, per = (blk + G - 1) / G, b0 = min(blk, s.group * per), b1 = min(blk, b0 + per);
-        float A[V], B[V], in[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) A[i] = 1.f, B[i] = 0.f;
-        if (s.live)
-            for (int b = b0; b < b1; ++b)
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float a = p.agg[(2L * b) * C + s.c + i];
-                    B[i] = cut_mul(a, B[i]) + p.agg[(2L * b + 1) * C + s.c + i];
-                    A[i] *= a;
-                }
-        s.template exchange<false>(A, B, carry, in, sm[par]);
+    for (int i = 0; i < V; ++i) carry[i] = !AGG && p.h0 ? p.h0[s.c + i] : 0.f, prod[i] = 1.f;
+    if (!AGG && p.blocks > 1) {
+        s.template skip_blocks<false>(p, blk, carry, sm[par]);
         par ^= 1;
     }
-    float wa[V];                                             // AGG: the block's composition so far is (wa, carry)
-#pragma unroll
-    for (int i = 0; i < V; ++i) wa[i] = 1.f;
-
-    vv g[SCAN_L], v[SCAN_L];
-    float m[SCAN_L];
-    auto fetch = [&](int t0) {
-#pragma unroll
-        for (int l = 0; l < SCAN_L; ++l) {
-            const int t = t0 + l;
-            if (s.live && t < te) {
-                g[l] = S::load(p.gate, t * p.gt + s.n * p.gn + s.j);
-                v[l] = S::load(p.value, t * p.vt + s.n * p.vn + s.j);
-                m[l] = p.masks ? p.masks[(long)t * p.N + s.n] : 1.f;
-            }
-        }
-    };
-    fetch(tb + s.group * SCAN_L);
+    vv g[SCAN_L], v[SCAN_L], none[SCAN_L];
+    auto fetch = [&](int t) __attribute__((always_inline)) { s.template fetch<true, false>(p, rg, rv, rg, t, te, all, g, v, none); };
+    fetch(tb + s.wave * SCAN_L);
     for (int t0 = tb; t0 < te; t0 += S::SC) {
-        const int tg = t0 + s.group * SCAN_L;
-        float a[SCAN_L][V], b[SCAN_L][V], A[V], B[V], in[V];
+        const int tw = t0 + s.wave * SCAN_L;
+        float m[SCAN_L], a[SCAN_L][V], b[SCAN_L][V], A[V], B[V], in[V];
+        s.masks(p, tw, te, m);
 #pragma unroll
         for (int i = 0; i < V; ++i) A[i] = 1.f, B[i] = 0.f;
 #pragma unroll
         for (int l = 0; l < SCAN_L; ++l) {
-            const bool on = s.live && tg + l < te;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 float f, nf;
-                gate_of(on ? to_f32(g[l][i]) : 0.f, f, nf);
-                a[l][i] = on ? m[l] * f : 1.f;
-                b[l][i] = on ? nf * to_f32(v[l][i]) : 0.f;
+                gate_of<sizeof(T) == 4>(to_f32(g[l][i]), f, nf);
+                a[l][i] = m[l] * f;
+                b[l][i] = nf * to_f32(v[l][i]);
                 B[i] = cut_mul(a[l][i], B[i]) + b[l][i];
-                A[i] *= a[l][i];
+                A[i] = cut_mul(a[l][i], A[i]);
             }
         }
-        if (t0 + S::SC < te) fetch(tg + S::SC);
-        if (AGG) {
-            // the product of all a of the superchunk: composed with a state of 1 and no addend
-#pragma unroll
-            for (int i = 0; i < V; ++i) in[i] = 0.f;
-            float A2[V], Z[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) A2[i] = A[i], Z[i] = 0.f;
-            float dummy[V];
-            s.template exchange<false>(A2, Z, wa, dummy, sm[par]);
-            par ^= 1;
-        }
-        s.template exchange<false>(A, B, carry, in, sm[par]);
+        if (t0 + S::SC < te) fetch(tw + S::SC);
+        s.template exchange<false, AGG>(A, B, carry, in, prod, sm[par]);
         par ^= 1;
         if (!AGG) {
-            if (p.saved && s.live && tg % SCAN_SAVE == 0 && tg < te) {
+            if (p.saved && tw % SCAN_SAVE == 0 && tw < te && s.live) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) p.saved[(long)(tg / SCAN_SAVE) * C + s.c + i] = in[i];
+                for (int i = 0; i < V; ++i) p.saved[(long)(tw / SCAN_SAVE) * C + s.c + i] = in[i];
             }
+            vv o[SCAN_L];
 #pragma unroll
-            for (int l = 0; l < SCAN_L; ++l) {
-                vv o;
+            for (int l = 0; l < SCAN_L; ++l)
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     in[i] = cut_mul(a[l][i], in[i]) + b[l][i];
-                    o[i] = from_f32<T>(in[i]);
+                    o[l][i] = from_f32<T>(in[i]);
                 }
-                const int t = tg + l;
-                if (s.live && t < te) *reinterpret_cast<vv*>((T*)p.out + t * p.ot + s.n * p.on + s.j) = o;
-            }
+            s.put(ro, tw, te, all, o);
         }
     }
-    if (s.group == 0 && s.live) {
+    if (s.wave == 0 && s.live) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             if (AGG) {
-                p.agg[(2L * blk) * C + s.c + i] = wa[i];
+                p.agg[(2L * blk) * C + s.c + i] = prod[i];
                 p.agg[(2L * blk + 1) * C + s.c + i] = carry[i];
             } else if (te == p.T && p.last) {
                 p.last[s.c + i] = carry[i];
@@ -240,150 +312,107 @@ __global__ __launch_bounds__(NW * 64) void scan_fwd_kernel(const ScanArgs p) {
 }
 
 // --------------------------------------------------------------------------------------------------------- backward
-template <class T, int V, int LC, int NW, bool AGG>
+// The states are formed again from the saved ones, in fp32, rather than read from the rounded output.
+template <class T, int V, int NW, int MODE, bool AGG>
 __global__ __launch_bounds__(NW * 64) void scan_bwd_kernel(const ScanArgs p) {
-    typedef Scan<T, V, LC, NW> S;
+    typedef Scan<T, V, NW, MODE> S;
     typedef typename S::vv vv;
-    __shared__ float sm[2][2][NW * S::CT * 2];
+    __shared__ typename S::pairs sm[2][2][NW * 64];
     S s;
     s.place(p);
     const long C = (long)p.N * p.H;
     const int blk = blockIdx.y, tb = blk * p.block_steps, te = min(p.T, tb + p.block_steps);
-    float carry[V];                                          // E behind the steps that are done
+    const typename S::Rows rg = s.rows(p.gate, p.gt, p.gn), rv = s.rows(p.value, p.vt, p.vn), rd = s.rows(p.dout, p.dt, p.dn);
+    const typename S::Rows qg = s.rows(p.dgate, p.dgt, p.dgn), qv = s.rows(p.dvalue, p.dvt, p.dvn);
+    const bool all = (long)(blockIdx.x + 1) * S::CT <= C;
+    float carry[V], prod[V];                                 // carry: E behind the steps that are done
     int par = 0;
 #pragma unroll
-    for (int i = 0; i < V; ++i) carry[i] = !AGG && p.dlast && s.live ? p.dlast[s.c + i] : 0.f;
-    if (!AGG && p.blocks > 1) {                              // the blocks behind this one, last to first
-        const int G = NW * S::GW, cnt = p.blocks - 1 - blk, per = (cnt + G - 1) / G;
-        const int r = G - 1 - s.group, b0 = min(cnt, r * per), b1 = min(cnt, b0 + per);      // group G-1 has the last blocks
-        float A[V], B[V], in[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) A[i] = 1.f, B[i] = 0.f;
-        if (s.live)
-            for (int b = b0; b < b1; ++b)
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const long q = 2L * (p.blocks - 1 - b);
-                    const float a = p.agg[q * C + s.c + i];
-                    B[i] = cut_mul(a, B[i]) + p.agg[(q + 1) * C + s.c + i];
-                    A[i] *= a;
-                }
-        s.template exchange<true>(A, B, carry, in, sm[0][par]);
+    for (int i = 0; i < V; ++i) carry[i] = !AGG && p.dlast ? p.dlast[s.c + i] : 0.f, prod[i] = 1.f;
+    if (!AGG && p.blocks > 1) {
+        s.template skip_blocks<true>(p, blk, carry, sm[0][par]);
         par ^= 1;
     }
-    float wa[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) wa[i] = 1.f;
-
     vv g[SCAN_L], v[SCAN_L], d[SCAN_L];
-    float m[SCAN_L];
-    auto fetch = [&](int t0) {
-#pragma unroll
-        for (int l = 0; l < SCAN_L; ++l) {
-            const int t = t0 + l;
-            if (s.live && t < te) {
-                g[l] = S::load(p.gate, t * p.gt + s.n * p.gn + s.j);
-                if (!AGG) v[l] = S::load(p.value, t * p.vt + s.n * p.vn + s.j);
-                d[l] = S::load(p.dout, t * p.dt + s.n * p.dn + s.j);
-                m[l] = p.masks ? p.masks[(long)t * p.N + s.n] : 1.f;
-            }
-        }
-    };
+    auto fetch = [&](int t) __attribute__((always_inline)) { s.template fetch<!AGG, true>(p, rg, rv, rd, t, te, all, g, v, d); };
     const int chunks = (te - tb + S::SC - 1) / S::SC;
-    fetch(tb + (chunks - 1) * S::SC + s.group * SCAN_L);
+    fetch(tb + (chunks - 1) * S::SC + s.wave * SCAN_L);
     for (int q = chunks - 1; q >= 0; --q) {
-        const int t0 = tb + q * S::SC, tg = t0 + s.group * SCAN_L;
-        float f[SCAN_L][V], A[V], B[V], P[V], Q[V], in[V], ein[V], start[V];
+        const int t0 = tb + q * S::SC, tw = t0 + s.wave * SCAN_L;
+        float f[SCAN_L][V], nf[SCAN_L][V], A[V], B[V], P[V], Q[V], in[V], ein[V];
         vv vc[SCAN_L], dc[SCAN_L];
         float mc[SCAN_L];
+        s.masks(p, tw, te, mc);
 #pragma unroll
         for (int i = 0; i < V; ++i) A[i] = 1.f, B[i] = 0.f, P[i] = 1.f, Q[i] = 0.f;
 #pragma unroll
         for (int l = 0; l < SCAN_L; ++l) {
-            const bool on = s.live && tg + l < te;
-            mc[l] = on ? m[l] : 1.f;
-            if (!AGG) vc[l] = v[l];
             dc[l] = d[l];
+            if (!AGG) vc[l] = v[l];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                float ff, nf;
-                const float x = on ? to_f32(g[l][i]) : 0.f;
-                gate_of(x, ff, nf);
-                f[l][i] = gate_pack(x, ff, nf);
+                gate_of<sizeof(T) == 4>(to_f32(g[l][i]), f[l][i], nf[l][i]);
                 if (!AGG) {
-                    const float a = on ? mc[l] * ff : 1.f;
-                    B[i] = cut_mul(a, B[i]) + (on ? nf * to_f32(vc[l][i]) : 0.f);
-                    A[i] *= a;
+                    const float a = mc[l] * f[l][i];
+                    B[i] = cut_mul(a, B[i]) + nf[l][i] * to_f32(vc[l][i]);
+                    A[i] = cut_mul(a, A[i]);
                 }
             }
         }
 #pragma unroll
-        for (int l = SCAN_L - 1; l >= 0; --l) {
-            const bool on = s.live && tg + l < te;
+        for (int l = SCAN_L - 1; l >= 0; --l)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                if (on) {
-                    float ff, nf;
-                    gate_unpack(f[l][i], ff, nf);
-                    const float a = mc[l] * ff;
-                    Q[i] = cut_mul(a, to_f32(dc[l][i]) + Q[i]);
-                    P[i] *= a;
-                }
+                const float a = mc[l] * f[l][i];
+                Q[i] = cut_mul(a, to_f32(dc[l][i]) + Q[i]);
+                P[i] = cut_mul(a, P[i]);
             }
-        }
-        if (q > 0) fetch(tg - S::SC);
+        if (q > 0) fetch(tw - S::SC);
         if (!AGG) {
+            // fp32 copies of values and derivatives and the products m f would take 96 registers more
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                start[i] = !s.live ? 0.f : p.saved ? p.saved[(long)(t0 / SCAN_SAVE) * C + s.c + i] : p.h0 ? p.h0[s.c + i] : 0.f;
-            s.template exchange<false>(A, B, start, in, sm[1][par]);
-        } else {
-            float P2[V], Z[V], dummy[V];
+            for (int l = 0; l < SCAN_L; ++l) {
+                forget(vc[l]), forget(dc[l]);
 #pragma unroll
-            for (int i = 0; i < V; ++i) P2[i] = P[i], Z[i] = 0.f;
-            s.template exchange<true>(P2, Z, wa, dummy, sm[1][par]);
+                for (int i = 0; i < V; ++i) forget(f[l][i]);
+            }
+            float start[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) start[i] = p.saved ? p.saved[(long)(t0 / SCAN_SAVE) * C + s.c + i] : p.h0 ? p.h0[s.c + i] : 0.f;
+            s.template exchange<false, false>(A, B, start, in, prod, sm[1][par]);
         }
-        s.template exchange<true>(P, Q, carry, ein, sm[0][par]);
+        s.template exchange<true, AGG>(P, Q, carry, ein, prod, sm[0][par]);
         par ^= 1;
         if (!AGG) {
             float hp[SCAN_L][V];                             // m_t h_{t-1}
 #pragma unroll
-            for (int l = 0; l < SCAN_L; ++l) {
-                const bool on = s.live && tg + l < te;
+            for (int l = 0; l < SCAN_L; ++l)
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    float ff, nf;
-                    gate_unpack(f[l][i], ff, nf);
                     hp[l][i] = cut_mul(mc[l], in[i]);
-                    if (on) in[i] = cut_mul(ff, hp[l][i]) + nf * to_f32(vc[l][i]);
+                    in[i] = cut_mul(f[l][i], hp[l][i]) + nf[l][i] * to_f32(vc[l][i]);
                 }
-            }
 #pragma unroll
-            for (int l = SCAN_L - 1; l >= 0; --l) {
-                const int t = tg + l;
-                const bool on = s.live && t < te;
-                vv og, ov;
+            for (int l = 0; l < SCAN_L; ++l) forget(vc[l]);
+            vv og[SCAN_L], ov[SCAN_L];
+#pragma unroll
+            for (int l = SCAN_L - 1; l >= 0; --l)
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    float ff, nf;
-                    gate_unpack(f[l][i], ff, nf);
-                    const float D = to_f32(dc[l][i]) + ein[i];
-                    og[i] = from_f32<T>(D * (hp[l][i] - to_f32(vc[l][i])) * ff * nf);
-                    ov[i] = from_f32<T>(D * nf);
-                    if (on) ein[i] = cut_mul(mc[l] * ff, D);
+                    const float D = to_f32(dc[l][i]) + ein[i], y = D * nf[l][i];
+                    og[l][i] = from_f32<T>((hp[l][i] - to_f32(vc[l][i])) * f[l][i] * y);
+                    ov[l][i] = from_f32<T>(y);
+                    ein[i] = cut_mul(mc[l] * f[l][i], D);
                 }
-                if (on) {
-                    *reinterpret_cast<vv*>((T*)p.dgate + t * p.dgt + s.n * p.dgn + s.j) = og;
-                    *reinterpret_cast<vv*>((T*)p.dvalue + t * p.dvt + s.n * p.dvn + s.j) = ov;
-                }
-            }
+            s.put(qg, tw, te, all, og);
+            s.put(qv, tw, te, all, ov);
         }
     }
-    if (s.group == 0 && s.live) {
+    if (s.wave == 0 && s.live) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             if (AGG) {
-                p.agg[(2L * blk) * C + s.c + i] = wa[i];
+                p.agg[(2L * blk) * C + s.c + i] = prod[i];
                 p.agg[(2L * blk + 1) * C + s.c + i] = carry[i];
             } else if (tb == 0 && p.dh0) {
                 p.dh0[s.c + i] = carry[i];
@@ -408,7 +437,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(const void* gate, long g
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         float f, nf;
-        gate_of(to_f32(g[i]), f, nf);
+        gate_of<sizeof(T) == 4>(to_f32(g[i]), f, nf);
         h[i] = f * cut_mul(m, h[i]) + nf * to_f32(v[i]);
         o[i] = from_f32<T>(h[i]);
     }
@@ -422,18 +451,19 @@ __global__ __launch_bounds__(256) void scan_copy_kernel(const float* src, float*
 }
 
 // --------------------------------------------------------------------------------------------------------- host side
-struct ScanPlan { int v, lc, nw, sc, ct, blocks, block_steps; };
+struct ScanPlan { int v, nw, sc, ct, blocks, block_steps; };
 
-static ScanPlan scan_plan(long T, long N, long H, int e, bool wide) {
+// V = 2 (16-bit storage: 4 bytes a lane) where rows allow it and there are enough channels to give every CU a tile, or time to split.  Waves: as many as the steps fill, 8 at most.
+// Time is split over workgroups where the tiles alone would leave most CUs without work: the second read of the gates and values
+// that this costs is made by all CUs at once.
+static ScanPlan scan_plan(long T, long N, long H, int e, bool pair) {
     ScanPlan p;
-    p.v = wide ? 8 / e : 1;
-    p.lc = wide ? 16 : 64;
-    const int gw = 64 / p.lc;
-    p.nw = wide ? (T <= 32 ? 1 : T <= 128 ? 4 : 8) : (T <= 32 ? 4 : 8);
-    p.sc = p.nw * gw * SCAN_L;
-    p.ct = p.lc * p.v;
-    p.blocks = 1;
-    const long tiles = cdiv(N * H, p.ct), chunks = cdiv(T, p.sc);
+    const long C = N * H;
+    p.v = e == 2 && pair && (C >= 128 * 256 || T > 1024) ? 2 : 1;
+    p.nw = T <= 16 ? 1 : T <= 64 ? 4 : 8;
+    p.sc = p.nw * SCAN_L;
+    p.ct = 64 * p.v;
+    const long tiles = cdiv(C, p.ct), chunks = cdiv(T, p.sc);
     long per = chunks;
     if (tiles < 96 && chunks > 1) per = cdiv(chunks, min(chunks, (long)cdiv(512, tiles)));
     if (per < 1) per = 1;
@@ -441,7 +471,10 @@ static ScanPlan scan_plan(long T, long N, long H, int e, bool wide) {
     p.blocks = chunks ? cdiv(chunks, per) : 1;
     return p;
 }
-static bool vec8(const void* p, long st, long sn, int e) { return ((uintptr_t)p & 7) == 0 && st * e % 8 == 0 && sn * e % 8 == 0; }
+// two neighbouring channels can be taken at once
+static bool in_pairs(const void* p, long st, long sn, int e) { return ((uintptr_t)p & (2 * e - 1)) == 0 && st % 2 == 0 && sn % 2 == 0; }
+// offsets within a tile of 128 channels or 16 steps need more than 31 bits
+static bool is_far(long st, long sn, long N, long H, int e) { return (min(N, 128 / H + 2) * sn + H) * e >= (1L << 31) || SCAN_L * st * e >= (1L << 31); }
 
 static int scan_check(long T, long N, long H, int dtype) {
     ACKTR_ARG(dtype_ok(dtype), "gated_scan: unknown dtype code %d", dtype);
@@ -450,30 +483,38 @@ static int scan_check(long T, long N, long H, int dtype) {
     return 0;
 }
 
-template <class T, bool BWD, bool AGG, int V, int LC>
+template <class T, bool BWD, bool AGG, int V, int MODE>
 static void scan_launch_nw(const ScanArgs& a, const ScanPlan& p, hipStream_t s) {
     const dim3 grid(cdiv((long)a.N * a.H, p.ct), p.blocks);
     auto go = [&](auto nw) {
         constexpr int NW = decltype(nw)::value;
-        if constexpr (BWD) scan_bwd_kernel<T, V, LC, NW, AGG><<<grid, NW * 64, 0, s>>>(a);
-        else scan_fwd_kernel<T, V, LC, NW, AGG><<<grid, NW * 64, 0, s>>>(a);
+        if constexpr (BWD) scan_bwd_kernel<T, V, NW, MODE, AGG><<<grid, NW * 64, 0, s>>>(a);
+        else scan_fwd_kernel<T, V, NW, MODE, AGG><<<grid, NW * 64, 0, s>>>(a);
     };
     if (p.nw == 1) go(std::integral_constant<int, 1>{});
     else if (p.nw == 4) go(std::integral_constant<int, 4>{});
     else go(std::integral_constant<int, 8>{});
 }
+template <class T, bool BWD, bool AGG>
+static void scan_launch(const ScanArgs& a, const ScanPlan& p, bool far, hipStream_t s) {
+    const bool whole = a.N == 1 || a.H % p.ct == 0;
+    if (far) return scan_launch_nw<T, BWD, AGG, 1, SCAN_FAR>(a, p, s);
+    if constexpr (sizeof(T) == 2) {
+        if (p.v == 2 && whole) return scan_launch_nw<T, BWD, AGG, 2, SCAN_WHOLE>(a, p, s);
+        if (p.v == 2) return scan_launch_nw<T, BWD, AGG, 2, SCAN_MIXED>(a, p, s);
+    }
+    if (whole) scan_launch_nw<T, BWD, AGG, 1, SCAN_WHOLE>(a, p, s);
+    else scan_launch_nw<T, BWD, AGG, 1, SCAN_MIXED>(a, p, s);
+}
 template <class T, bool BWD>
-static int scan_run(ScanArgs a, const ScanPlan& p, hipStream_t s) {
+static int scan_run(ScanArgs a, const ScanPlan& p, bool far, hipStream_t s) {
     a.blocks = p.blocks;
     a.block_steps = p.block_steps;
-    constexpr int W = 8 / sizeof(T);
     if (p.blocks > 1) {
-        if (p.v > 1) scan_launch_nw<T, BWD, true, W, 16>(a, p, s);
-        else scan_launch_nw<T, BWD, true, 1, 64>(a, p, s);
+        scan_launch<T, BWD, true>(a, p, far, s);
         ACKTR_LAUNCH_CHECK();
     }
-    if (p.v > 1) scan_launch_nw<T, BWD, false, W, 16>(a, p, s);
-    else scan_launch_nw<T, BWD, false, 1, 64>(a, p, s);
+    scan_launch<T, BWD, false>(a, p, far, s);
     ACKTR_LAUNCH_CHECK();
     return 0;
 }
@@ -487,8 +528,8 @@ extern "C" int acktr_gated_scan_save_interval(void) { return SCAN_SAVE; }
 extern "C" long acktr_gated_scan_workspace_bytes(long T, long N, long H, int dtype) {
     if (scan_check(T, N, H, dtype)) return -1;
     long most = 0;
-    for (int wide = 0; wide < 2; ++wide) {
-        const ScanPlan p = scan_plan(T, N, H, (int)elem_bytes(dtype), wide != 0);
+    for (int pair = 0; pair < 2; ++pair) {
+        const ScanPlan p = scan_plan(T, N, H, (int)elem_bytes(dtype), pair != 0);
         if (p.blocks > 1) most = max(most, 8L * p.blocks * N * H);
     }
     return most;
@@ -509,15 +550,16 @@ extern "C" int acktr_gated_scan_fwd(const void* gate, long gt, long gn, const vo
     }
     const int e = (int)elem_bytes(dtype);
     ACKTR_ARG(gate && value && out, "gated_scan_fwd: gate, value and out are required");
-    const bool wide = H % (8 / e) == 0 && vec8(gate, gt, gn, e) && vec8(value, vt, vn, e) && vec8(out, ot, on, e);
+    const bool far = is_far(gt, gn, N, H, e) || is_far(vt, vn, N, H, e) || is_far(ot, on, N, H, e);
+    const bool pair = !far && H % 2 == 0 && in_pairs(gate, gt, gn, e) && in_pairs(value, vt, vn, e) && in_pairs(out, ot, on, e);
     ACKTR_ARG(workspace_bytes >= acktr_gated_scan_workspace_bytes(T, N, H, dtype), "gated_scan_fwd: workspace of %ld bytes is too small",
               workspace_bytes);
-    const ScanPlan p = scan_plan(T, N, H, e, wide);
+    const ScanPlan p = scan_plan(T, N, H, e, pair);
     ScanArgs a{};
     a.gate = gate, a.gt = gt, a.gn = gn, a.value = value, a.vt = vt, a.vn = vn, a.h0 = h0, a.masks = masks;
     a.out = out, a.ot = ot, a.on = on, a.last = last, a.saved = saved, a.agg = (float*)workspace;
     a.T = (int)T, a.N = (int)N, a.H = (int)H;
-    return with_dtype(dtype, [&](auto t) -> int { return scan_run<decltype(t), false>(a, p, s); });
+    return with_dtype(dtype, [&](auto t) -> int { return scan_run<decltype(t), false>(a, p, far, s); });
 }
 
 extern "C" int acktr_gated_scan_bwd(const void* dout, long dt, long dn, const void* gate, long gt, long gn, const void* value, long vt, long vn,
@@ -536,18 +578,19 @@ extern "C" int acktr_gated_scan_bwd(const void* dout, long dt, long dn, const vo
     }
     const int e = (int)elem_bytes(dtype);
     ACKTR_ARG(dout && gate && value && dgate && dvalue, "gated_scan_bwd: dout, gate, value, dgate and dvalue are required");
-    const bool wide = H % (8 / e) == 0 && vec8(dout, dt, dn, e) && vec8(gate, gt, gn, e) && vec8(value, vt, vn, e) &&
-                      vec8(dgate, dgt, dgn, e) && vec8(dvalue, dvt, dvn, e);
+    const bool far = is_far(gt, gn, N, H, e) || is_far(vt, vn, N, H, e) || is_far(dt, dn, N, H, e) || is_far(dgt, dgn, N, H, e) || is_far(dvt, dvn, N, H, e);
+    const bool pair = !far && H % 2 == 0 && in_pairs(dout, dt, dn, e) && in_pairs(gate, gt, gn, e) && in_pairs(value, vt, vn, e) &&
+                      in_pairs(dgate, dgt, dgn, e) && in_pairs(dvalue, dvt, dvn, e);
     ACKTR_ARG(workspace_bytes >= acktr_gated_scan_workspace_bytes(T, N, H, dtype), "gated_scan_bwd: workspace of %ld bytes is too small",
               workspace_bytes);
-    const ScanPlan p = scan_plan(T, N, H, e, wide);
+    const ScanPlan p = scan_plan(T, N, H, e, pair);
     ACKTR_ARG(saved || T <= SCAN_SAVE, "gated_scan_bwd: %ld steps need the states that the forward pass saves every %d steps", T, SCAN_SAVE);
     ScanArgs a{};
     a.dout = dout, a.dt = dt, a.dn = dn, a.gate = gate, a.gt = gt, a.gn = gn, a.value = value, a.vt = vt, a.vn = vn;
     a.h0 = h0, a.masks = masks, a.saved = const_cast<float*>(saved), a.dlast = dlast;
     a.dgate = dgate, a.dgt = dgt, a.dgn = dgn, a.dvalue = dvalue, a.dvt = dvt, a.dvn = dvn, a.dh0 = dh0, a.agg = (float*)workspace;
     a.T = (int)T, a.N = (int)N, a.H = (int)H;
-    return with_dtype(dtype, [&](auto t) -> int { return scan_run<decltype(t), true>(a, p, s); });
+    return with_dtype(dtype, [&](auto t) -> int { return scan_run<decltype(t), true>(a, p, far, s); });
 }
 
 extern "C" int acktr_gated_scan_step(const void* gate, long gn, const void* value, long vn, float* state, const float* masks, void* out, long on,
@@ -559,8 +602,8 @@ extern "C" int acktr_gated_scan_step(const void* gate, long gn, const void* valu
     return with_dtype(dtype, [&](auto t) -> int {
         typedef decltype(t) T;
         constexpr int W = 8 / sizeof(T);
-        const bool wide = H % W == 0 && vec8(gate, 0, gn, sizeof(T)) && vec8(value, 0, vn, sizeof(T)) && vec8(out, 0, on, sizeof(T)) &&
-                          ((uintptr_t)state & 15) == 0;
+        auto rows8 = [](const void* q, long sn) { return ((uintptr_t)q & 7) == 0 && sn * (long)sizeof(T) % 8 == 0; };
+        const bool wide = H % W == 0 && rows8(gate, gn) && rows8(value, vn) && rows8(out, on) && ((uintptr_t)state & 15) == 0;
         if (wide) scan_step_kernel<T, W><<<cdiv(N * H, 256 * W), 256, 0, s>>>(gate, gn, value, vn, state, masks, out, on, (int)N, (int)H);
         else scan_step_kernel<T, 1><<<cdiv(N * H, 256), 256, 0, s>>>(gate, gn, value, vn, state, masks, out, on, (int)N, (int)H);
         ACKTR_LAUNCH_CHECK();
