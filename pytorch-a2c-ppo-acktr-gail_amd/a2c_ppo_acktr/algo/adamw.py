@@ -35,6 +35,7 @@ class AdamW(object):
             raise ValueError('AdamW: as many gradients and copies as parameters are needed')
         self.param_groups = [{'params': params, 'lr': lr, 'betas': betas, 'eps': eps, 'weight_decay': weight_decay,
                               'max_grad_norm': max_grad_norm}]
+        self._copied = [c for c in self.copies if c is not None]
         self._check_hyper()
         self.state_bits, self.seed = state_bits, int(seed)
         self.step_count = 0
@@ -71,9 +72,10 @@ class AdamW(object):
         self._state = torch.zeros(words, dtype=torch.float64, device=dev)
         self._state[6:8].view(torch.int64).copy_(torch.tensor([self.step_count, self.seed]))
         chunk = L.acktr_adamw_chunk()
-        pairs = [torch.stack((torch.full((c,), i, dtype=torch.int32), torch.arange(c, dtype=torch.int32)), 1)
-                 for i, c in ((i, -(-n // chunk)) for i, n in enumerate(self._numel)) if c]
-        self._chunks = torch.cat(pairs).to(dev).contiguous() if pairs else torch.zeros(0, 2, dtype=torch.int32, device=dev)
+        count = torch.tensor([-(-n // chunk) for n in self._numel])
+        which = torch.repeat_interleave(count)                # {tensor, chunk number} pairs
+        first = torch.cumsum(count, 0) - count
+        self._chunks = torch.stack((which, torch.arange(which.numel()) - first[which]), 1).to(torch.int32).to(dev)
         self._seen = self._hyper = None
 
     def _gradients(self):
@@ -89,12 +91,14 @@ class AdamW(object):
 
     def _table(self, grads):
         """The device table of tensors, rebuilt only when one of them was replaced (checked by address, size and type)."""
-        seen = tuple((p.data_ptr(), p.numel(), p.dtype, g.data_ptr(), g.numel(), g.dtype, 0 if c is None else c.data_ptr())
-                     for p, g, c in zip(self.params, grads, self.copies))
+        ptr, num = torch.Tensor.data_ptr, torch.Tensor.numel
+        own = self.params + self._copied                      # (tensors that this object holds: their types stay)
+        seen = [list(map(ptr, own)), list(map(num, own)), list(map(ptr, grads)), list(map(num, grads)),
+                None if grads is self.grads else [g.dtype for g in grads]]
         if seen == self._seen:
             return
         dev = self._dev
-        rows = (_hip.AdamwTensor * len(seen))()
+        rows = (_hip.AdamwTensor * len(self.params))()
         for i, (p, g, c) in enumerate(zip(self.params, grads, self.copies)):
             for t, what in ((p, 'parameter'), (g, 'gradient'), (c, 'copy')):
                 if t is None:
@@ -113,8 +117,7 @@ class AdamW(object):
                                        ops.DTYPE_CODE[p.dtype], ops.DTYPE_CODE[g.dtype],
                                        ops.DTYPE_CODE[c.dtype] if c is not None else 0,
                                        (1 if quad(p) else 0) | (2 if quad(g) else 0) | (4 if quad(c) else 0))
-        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in list(self.params) +
-                       [c for c in self.copies if c is not None] if t.numel())
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.nbytes) for t in own if t.numel())
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise RuntimeError('AdamW: two of the tensors to be written overlap (the same parameter twice?)')
         if torch.cuda.is_current_stream_capturing():
@@ -126,7 +129,6 @@ class AdamW(object):
     def prepare(self):
         """Brings the device side up to date with the parameter list and the hyperparameters: outside a graph capture, and before a
         replay when a hyperparameter changed."""
-        self._check_hyper()
         dev = self.params[0].device
         if dev.type == 'cuda' and dev.index is None:
             dev = torch.device('cuda', torch.cuda.current_device())
@@ -141,6 +143,7 @@ class AdamW(object):
         hyper = (float(g['lr']), float(g['betas'][0]), float(g['betas'][1]), float(g['eps']), float(g['weight_decay']),
                  float(g['max_grad_norm'] or 0.0))
         if hyper != self._hyper:
+            self._check_hyper()
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError('AdamW: a hyperparameter changed; run prepare() before the capture')
             with torch.no_grad():
@@ -151,7 +154,7 @@ class AdamW(object):
 
     # ------------------------------------------------------------------ torch.optim surface
     def zero_grad(self, set_to_none=False):
-        for t in self.grads if self.grads is not None else self.params + [c for c in self.copies if c is not None]:
+        for t in self.grads if self.grads is not None else self.params + self._copied:
             if self.grads is not None:
                 t.zero_()
             elif t.grad is not None:

@@ -538,46 +538,48 @@ def _act_code(act):
     return LINEAR_ACT[act]
 
 
-def _span(t):
+def _reach(t):
+    """[first byte, last byte + 1) of a tensor"""
+    if t is None:
+        return 0, 0
+    p = t.data_ptr()
     if t.is_contiguous():
-        p = t.data_ptr()
         return p, p + t.nbytes
     reach = 1
     for n, s in zip(t.shape, t.stride()):
         if n == 0:
             return 0, 0
         reach += (n - 1) * s
-    p, e = t.data_ptr(), t.element_size()
-    return p, p + reach * e
+    return p, p + reach * t.element_size()
 
 
-def _no_overlap(a, b, what):
-    """a (to be written) and b (read) share no element."""
-    if a is None or b is None:
-        return
-    (a0, a1), (b0, b1) = _span(a), _span(b)
-    if a0 < b1 and b0 < a1:
-        # two column slices of the same rows do not meet although their spans do
-        if a.dim() == b.dim() > 1 and a.stride() == b.stride() and a.element_size() == b.element_size():
-            steps, e = [s for n, s in zip(a.shape[:-1], a.stride()[:-1]) if n > 1], a.element_size()
-            if steps and min(steps) > 0 and (b0 - a0) % e == 0:
-                step = min(steps)
-                d = ((b0 - a0) // e) % step
-                if all(s % step == 0 for s in steps) and d >= a.shape[-1] and d + b.shape[-1] <= step:
-                    return
-        raise RuntimeError('%s must not overlap' % what)
+def _apart(out, name, others, what):
+    """`out` (to be written; its elements must not share memory) has no element in common with any of `others`."""
+    if not out.is_contiguous():
+        reach = 1
+        for s, n in sorted((s, n) for n, s in zip(out.shape, out.stride()) if n > 1):
+            if s < reach:
+                raise RuntimeError('%s: %s has elements that share memory (strides %s)' % (what, name, tuple(out.stride())))
+            reach += s * (n - 1)
+    a0, a1 = _reach(out)
+    for t in others:
+        if t is None:
+            continue
+        b0, b1 = _reach(t)
+        if a0 < b1 and b0 < a1 and not _side_by_side(out, a0, t, b0):
+            raise RuntimeError('%s: %s overlaps another operand' % (what, name))
 
 
-def _writable(t, name):
-    """Every element of a tensor that is written has a place of its own (an expanded tensor has not)."""
-    if t.is_contiguous():
-        return
-    axes = sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1)
-    reach = 1
-    for s, n in axes:
-        if s < reach:
-            raise RuntimeError('%s: its elements share memory (strides %s)' % (name, tuple(t.stride())))
-        reach = s * (n - 1) + reach
+def _side_by_side(a, a0, b, b0):
+    """Column slices of the same rows: their spans cross, their elements do not."""
+    e = a.element_size()
+    if a.dim() != b.dim() or a.dim() < 2 or a.stride() != b.stride() or b.element_size() != e or (b0 - a0) % e:
+        return False
+    steps = [s for n, s in zip(a.shape[:-1], a.stride()[:-1]) if n > 1]
+    if not steps or min(steps) <= 0 or any(s % min(steps) for s in steps):
+        return False
+    d = (b0 - a0) // e % min(steps)
+    return d >= a.shape[-1] and d + b.shape[-1] <= min(steps)
 
 
 def _scratch(nbytes, like, what):
@@ -606,13 +608,9 @@ def linear_act_fwd(x, w, bias=None, act=None, residual=None, out=None, pre=None)
     pz, ldz = None, 0
     if pre is not None:
         pz, ldz = _rows(pre, 'pre', mn, dt, at)
-        _writable(pre, 'pre')
-        for b in (x, w, bias, residual, out if given else None):
-            _no_overlap(pre, b, 'linear_act_fwd: pre and another operand')
+        _apart(pre, 'pre', (x, w, bias, residual, out if given else None), 'linear_act_fwd')
     if given:
-        _writable(out, 'out')
-        for b in (x, w, bias, None if pr == py and ldr == ldy else residual):
-            _no_overlap(out, b, 'linear_act_fwd: out and an input')
+        _apart(out, 'out', (x, w, bias, None if pr == py and ldr == ldy else residual), 'linear_act_fwd')
     L = _hip.lib()
     nb = L.acktr_linear_act_fwd_workspace_bytes(px, ldx, pw, ldw, M, N, K, code)
     ws = _scratch(nb, x, 'acktr_linear_act_fwd') if nb else None
@@ -650,9 +648,7 @@ def linear_act_bwd(dy, x, w, pre=None, act=None, dx=None, dw=None, db=None, need
         db = dy.new_empty(N) if db is None else db
         qb = _vec(db, 'db', N, dt, at)
     for i, a in enumerate(given):
-        _writable(a, 'a gradient')
-        for b in (dy, x, w, pre) + tuple(given[:i]):
-            _no_overlap(a, b, 'linear_act_bwd: a gradient and another operand')
+        _apart(a, 'a gradient', (dy, x, w, pre) + tuple(given[:i]), 'linear_act_bwd')
     L = _hip.lib()
     nb = L.acktr_linear_act_bwd_workspace_bytes(pg, ldg, px, ldx, pw, ldw, pz, ldz, need_dx, need_dw, need_db, M, N, K, code, act)
     ws = _scratch(nb, dy, 'acktr_linear_act_bwd') if nb else None
@@ -681,6 +677,16 @@ def _masks(masks, shape, index):
     return _dense(masks, 'masks', shape, f32, index)
 
 
+_interval = None
+
+
+def _scan_interval():
+    global _interval
+    if _interval is None:
+        _interval = _hip.lib().acktr_gated_scan_save_interval()
+    return _interval
+
+
 def gated_scan_fwd(gate, value, h0=None, masks=None, out=None, save=False):
     """(out, last, saved) of the gated linear recurrence h_t = f_t (m_t h_{t-1}) + (1 - f_t) value_t, f = sigmoid(gate).
     gate, value, out [T, N, H] (one type; any strides over T and N: halves of one projection, batch-first views); h0 [N, H] fp32 or
@@ -698,12 +704,10 @@ def gated_scan_fwd(gate, value, h0=None, masks=None, out=None, save=False):
     ph = _dense(h0, 'h0', (N, H), f32, at) if h0 is not None else None
     pm = _masks(masks, (T, N), at)
     if given:
-        _writable(out, 'out')
-        for b in (gate, value, h0, masks):
-            _no_overlap(out, b, 'gated_scan_fwd: out and an input')
+        _apart(out, 'out', (gate, value, h0, masks), 'gated_scan_fwd')
     L = _hip.lib()
     last = gate.new_empty((N, H), dtype=f32)
-    saved = gate.new_empty((-(-T // L.acktr_gated_scan_save_interval()), N, H), dtype=f32) if save else None
+    saved = gate.new_empty((-(-T // _scan_interval()), N, H), dtype=f32) if save else None
     nb = L.acktr_gated_scan_workspace_bytes(T, N, H, code)
     ws = _scratch(nb, gate, 'acktr_gated_scan_fwd') if nb else None
     _launch(L.acktr_gated_scan_fwd, (*pg, *pv, ph, pm, *po, last.data_ptr(), saved.data_ptr() if save else None, T, N, H, code,
@@ -725,19 +729,15 @@ def gated_scan_bwd(dout, gate, value, h0=None, masks=None, saved=None, dlast=Non
     pd, pg, pv = _steps(dout, 'dout', shape, dt, at), _steps(gate, 'gate', shape, dt, at), _steps(value, 'value', shape, dt, at)
     qg, qv = _steps(dgate, 'dgate', shape, dt, at), _steps(dvalue, 'dvalue', shape, dt, at)
     L = _hip.lib()
-    every = L.acktr_gated_scan_save_interval()
+    every = _scan_interval()
     ph = _dense(h0, 'h0', (N, H), f32, at) if h0 is not None else None
     pm = _masks(masks, (T, N), at)
     ps = _dense(saved, 'saved', (-(-T // every), N, H), f32, at) if saved is not None and T else None
     pl = _dense(dlast, 'dlast', (N, H), f32, at) if dlast is not None else None
     if T > every and saved is None:
         raise RuntimeError('gated_scan_bwd: more than %d steps need what gated_scan_fwd(save=True) saved' % every)
-    for a in given:
-        _writable(a, 'a gradient')
-        for b in (dout, gate, value, h0, masks, saved, dlast):
-            _no_overlap(a, b, 'gated_scan_bwd: a gradient and an input')
-    if len(given) == 2:
-        _no_overlap(dgate, dvalue, 'gated_scan_bwd: dgate and dvalue')
+    for i, a in enumerate(given):
+        _apart(a, 'a gradient', (dout, gate, value, h0, masks, saved, dlast) + tuple(given[:i]), 'gated_scan_bwd')
     dh0 = gate.new_empty((N, H), dtype=f32) if need_dh0 else None
     nb = L.acktr_gated_scan_workspace_bytes(T, N, H, code)
     ws = _scratch(nb, gate, 'acktr_gated_scan_bwd') if nb else None
@@ -761,10 +761,7 @@ def gated_scan_step(gate, value, state, masks=None, out=None):
     ps = _dense(state, 'state', shape, f32, at)
     pm = _masks(masks, (N,), at)
     if given:
-        _writable(out, 'out')
-        for b in (gate, value, state, masks):
-            _no_overlap(out, b, 'gated_scan_step: out and an input')
-    for b in (gate, value, masks):
-        _no_overlap(state, b, 'gated_scan_step: state and an input')
+        _apart(out, 'out', (gate, value, state, masks), 'gated_scan_step')
+    _apart(state, 'state', (gate, value, masks), 'gated_scan_step')
     _launch(_hip.lib().acktr_gated_scan_step, (pg, gn, pv, vn, ps, pm, po, on, N, H, code), at, 'gated_scan_step', 10.0 * N * H)
     return out

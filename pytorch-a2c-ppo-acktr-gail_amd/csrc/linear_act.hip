@@ -2,6 +2,9 @@
 //   dz = dy act'(z),  dx = dz w,  dw = dz^T x,  db = sum over rows of dz
 // Three products over the same tile kernel (tile_gemm.hpp), which reads each operand as it lies: forward k | k contiguous, input
 // gradient k | rows, weight gradient rows | rows.
+#include <initializer_list>
+#include <type_traits>
+
 #include "act_terms.hpp"
 #include "linear_act.hpp"
 
@@ -9,20 +12,24 @@ namespace acktr {
 
 // dst[r][c] = src[r][c] for c < cols, 0 up to ldd: a copy whose rows start at 16-byte boundaries, for operands that do not
 // (an odd width, a slice of a wider row).  It costs one pass over the operand; reading such rows element by element in the
-// product would cost a fetch per element of every tile that uses it.
+// product would cost a fetch per element of every tile that uses it.  Up to two operands a launch.
+struct PackJob { const void* src; long lds; int rows, cols; void* dst; int ldd; };
+struct PackJobs { PackJob job[2]; };
 template <class T>
-__global__ __launch_bounds__(256) void pack_rows_kernel(const T* __restrict__ src, long lds, int rows, int cols, T* __restrict__ dst, int ldd) {
-    typedef vec_t<T, 16 / sizeof(T)> vv;
+__global__ __launch_bounds__(256) void pack_rows_kernel(const PackJobs jobs) {
+    const PackJob p = jobs.job[blockIdx.y];
     constexpr int V = 16 / sizeof(T);
-    const int groups = ldd / V;
-    const long total = (long)rows * groups;
+    typedef vec_t<T, V> vv;
+    const int groups = p.ldd / V;
+    const long total = (long)p.rows * groups;
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
         const long r = i / groups;
         const int c = (int)(i % groups) * V;
+        const T* src = (const T*)p.src + r * p.lds + c;
         vv o;
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = c + j < cols ? src[r * lds + c + j] : (T)0.f;
-        *reinterpret_cast<vv*>(dst + r * ldd + c) = o;
+        for (int j = 0; j < V; ++j) o[j] = c + j < p.cols ? src[j] : (T)0.f;
+        *reinterpret_cast<vv*>((T*)p.dst + r * p.ldd + c) = o;
     }
 }
 
@@ -72,25 +79,37 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(const T* __restrict__ dy, 
         sums[(long)blockIdx.y * N + col] = t;
     }
 }
-// db = sum of the row blocks' sums, 8 partial sums a column (each over every eighth block), in fixed order
+// db = sum of the row blocks' sums, 32 partial sums a column (each over every 32nd block), in fixed order
 template <class T>
-__global__ __launch_bounds__(256) void col_sums_kernel(const float* __restrict__ sums, int blocks, int N, T* __restrict__ db) {
-    __shared__ float part[8][32];
+__global__ __launch_bounds__(1024) void col_sums_kernel(const float* __restrict__ sums, int blocks, int N, T* __restrict__ db) {
+    __shared__ float part[32][33];
     const int c = threadIdx.x & 31, j = threadIdx.x >> 5, col = blockIdx.x * 32 + c;
     float t = 0.f;
-    if (col < N)
-        for (int b = j; b < blocks; b += 8) t += sums[(long)b * N + col];
+    if (col < N) {
+#pragma unroll 8
+        for (int b = j; b < blocks; b += 32) t += sums[(long)b * N + col];
+    }
     part[j][c] = t;
     __syncthreads();
-    if (j == 0 && col < N) {
-        for (int i = 1; i < 8; ++i) t += part[i][c];
-        db[col] = from_f32<T>(t);
-    }
+    // column j: the 32 partial sums of a half wave, added pairwise
+    t = part[c][j];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor(t, o, 32);
+    if (c == 0 && blockIdx.x * 32 + j < N) db[blockIdx.x * 32 + j] = from_f32<T>(t);
 }
-
+// packs the jobs that have rows
 template <class T>
-static int pack(const void* src, long lds, int rows, int cols, void* dst, int ldd, hipStream_t s) {
-    pack_rows_kernel<T><<<min(cdiv((long)rows * (ldd * sizeof(T) / 16), 256), 4096), 256, 0, s>>>((const T*)src, lds, rows, cols, (T*)dst, ldd);
+static int pack(std::initializer_list<PackJob> list, hipStream_t s) {
+    PackJobs jobs{};
+    int n = 0;
+    long most = 0;
+    for (const PackJob& j : list)
+        if (j.rows > 0) {
+            jobs.job[n++] = j;
+            most = max(most, (long)j.rows * (j.ldd * (long)sizeof(T) / 16));
+        }
+    if (n == 0) return 0;
+    pack_rows_kernel<T><<<dim3(min(cdiv(most, 256), 4096), n), 256, 0, s>>>(jobs);
     ACKTR_LAUNCH_CHECK();
     return 0;
 }
@@ -125,7 +144,7 @@ static FwdSpace fwd_space(const void* x, long ldx, const void* w, long ldw, long
     f.x = 0;
     f.w = f.px ? up(M * kp * e, 256) : 0;
     f.slabs = f.w + (f.pw ? up(N * kp * e, 256) : 0);
-    f.bytes = f.slabs + slab_bytes(M, N, kp, e);
+    f.bytes = f.slabs + slab_bytes(M, N, plan_of(M, N, kp, e).slices);
     return f;
 }
 struct BwdSpace { bool aligned, pdy, px, pw; long dz, x, w, sums, slabs, bytes; };
@@ -143,8 +162,13 @@ static BwdSpace bwd_space(const void* dy, long lddy, const void* x, long ldx, co
     f.w = f.x + (f.px ? up(M * kp * e, 256) : 0);
     f.sums = f.w + (f.pw ? up(N * kp * e, 256) : 0);
     f.slabs = f.sums + (db ? up(4L * SUM_BLOCKS * N, 256) : 0);
-    long most = dx ? slab_bytes(M, K, N, e) : 0;
-    if (dw) most = max(most, slab_bytes(N, K, M, e));
+    long most = dx ? slab_bytes(M, K, plan_of(M, K, N, e).slices) : 0;
+    if (dw) most = max(most, slab_bytes(N, K, plan_of(N, K, M, e).slices));
+    if (dx && dw) {
+        LinArgs pw{}, px{};
+        pw.M = (int)N, pw.N = (int)K, pw.K = (int)M, px.M = (int)M, px.N = (int)K, px.K = (int)N;
+        most = max(most, slab_bytes(N, K, pair_plan_of(pw, px, e).slices));
+    }
     f.bytes = f.slabs + most;
     return f;
 }
@@ -177,14 +201,9 @@ extern "C" int acktr_linear_act_fwd(const void* x, long ldx, const void* w, long
                 (!pre || rows16(pre, ldp, e));
         char* ws = (char*)workspace;
         const int kp = (int)up(K, V_OF(e));
-        if (sp.px) {
-            if (int rc = pack<T>(x, ldx, (int)M, (int)K, ws + sp.x, kp, s)) return rc;
-            p.a = ws + sp.x, p.lda = kp;
-        }
-        if (sp.pw) {
-            if (int rc = pack<T>(w, ldw, (int)N, (int)K, ws + sp.w, kp, s)) return rc;
-            p.b = ws + sp.w, p.ldb = kp;
-        }
+        if (int rc = pack<T>({{x, ldx, sp.px ? (int)M : 0, (int)K, ws + sp.x, kp}, {w, ldw, sp.pw ? (int)N : 0, (int)K, ws + sp.w, kp}}, s)) return rc;
+        if (sp.px) p.a = ws + sp.x, p.lda = kp;
+        if (sp.pw) p.b = ws + sp.w, p.ldb = kp;
         p.K = kp;
         return linear_product<T>(LIN_FORWARD, p, (float*)(ws + sp.slabs), s);
     });
@@ -242,39 +261,28 @@ extern "C" int acktr_linear_act_bwd(const void* dy, long lddy, const void* x, lo
             else launch(std::false_type{}, integral_constant<int, 1>{});
             ACKTR_LAUNCH_CHECK();
             if (db) {
-                col_sums_kernel<T><<<cdiv(N, 32), 256, 0, s>>>(sums, gy, (int)N, (T*)db);
+                col_sums_kernel<T><<<cdiv(N, 32), 1024, 0, s>>>(sums, gy, (int)N, (T*)db);
                 ACKTR_LAUNCH_CHECK();
             }
         } else if (db) {                                     // no rows: the gradient of the bias is zero
-            col_sums_kernel<T><<<cdiv(N, 32), 256, 0, s>>>(sums, 0, (int)N, (T*)db);
+            col_sums_kernel<T><<<cdiv(N, 32), 1024, 0, s>>>(sums, 0, (int)N, (T*)db);
             ACKTR_LAUNCH_CHECK();
         }
         if (M > 0 && sp.pdy) {                               // no activation: dy itself, in aligned rows
-            if (int rc = pack<T>(dy, lddy, (int)M, (int)N, dz_ws, np, s)) return rc;
+            if (int rc = pack<T>({{dy, lddy, (int)M, (int)N, dz_ws, np}}, s)) return rc;
             dz = dz_ws, lddz = np;
         }
-        if (dx && M > 0) {                                   // dx[M, K] = dz[M, N] w[N, K]: sum over N
-            LinArgs p{};
-            p.a = dz, p.lda = lddz, p.b = w, p.ldb = ldw;
-            if (sp.pw) {
-                if (int rc = pack<T>(w, ldw, (int)N, (int)K, w_ws, kp, s)) return rc;
-                p.b = w_ws, p.ldb = kp;
-            }
-            p.M = (int)M, p.N = (int)K, p.K = (int)N;
-            p.y = dx, p.ldy = lddx, p.vec = K % 8 == 0 && rows16(dx, lddx, e);
-            if (int rc = linear_product<T>(LIN_DX, p, slabs, s)) return rc;
-        }
-        if (dw) {                                            // dw[N, K] = dz^T x: sum over M
-            LinArgs p{};
-            p.a = dz, p.lda = lddz, p.b = x, p.ldb = ldx;
-            if (M > 0 && sp.px) {
-                if (int rc = pack<T>(x, ldx, (int)M, (int)K, x_ws, kp, s)) return rc;
-                p.b = x_ws, p.ldb = kp;
-            }
-            p.M = (int)N, p.N = (int)K, p.K = (int)M;
-            p.y = dw, p.ldy = K, p.vec = K % 8 == 0 && rows16(dw, K, e);
-            if (int rc = linear_product<T>(LIN_DW, p, slabs, s)) return rc;
-        }
+        if (int rc = pack<T>({{x, ldx, sp.px ? (int)M : 0, (int)K, x_ws, kp}, {w, ldw, sp.pw && M > 0 ? (int)N : 0, (int)K, w_ws, kp}}, s)) return rc;
+        LinArgs px{}, pw{};
+        px.a = dz, px.lda = lddz, px.b = sp.pw ? w_ws : w, px.ldb = sp.pw ? kp : ldw;      // dx[M, K] = dz[M, N] w[N, K]: sum over N
+        px.M = (int)M, px.N = (int)K, px.K = (int)N;
+        px.y = dx, px.ldy = lddx, px.vec = K % 8 == 0 && rows16(dx, lddx, e);
+        pw.a = dz, pw.lda = lddz, pw.b = sp.px ? x_ws : x, pw.ldb = sp.px ? kp : ldx;      // dw[N, K] = dz^T x: sum over M
+        pw.M = (int)N, pw.N = (int)K, pw.K = (int)M;
+        pw.y = dw, pw.ldy = K, pw.vec = K % 8 == 0 && rows16(dw, K, e);
+        if (dx && dw && M > 0) return linear_gradients<T>(pw, px, slabs, s);
+        if (dx && M > 0) return linear_product<T>(LIN_DX, px, slabs, s);
+        if (dw) return linear_product<T>(LIN_DW, pw, slabs, s);
         return 0;
     });
 }

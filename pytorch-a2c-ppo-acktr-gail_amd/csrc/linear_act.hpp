@@ -27,44 +27,68 @@ static inline bool rows16(const void* p, long ld, long e) { return ((uintptr_t)p
 
 // Tile and reduction split of an M x N x K product, by an estimate of its time.  A K step (128 bytes of k) of a 64 x 64 piece is the
 // unit.  `rate`: units per microsecond that a CU full of such workgroups gets through; `step`: microseconds a step takes a workgroup
-// that has a CU to itself (measured on 16384 x 2048 x 2048 and on 2048 x 2048 x 16384: 256 x 256 tiles 1.65 us a step full, 1.17 us
-// alone; 128 x 128 1.0 us for two, 0.61 alone; 128 x 64 0.30 for one of many, 0.5 alone; 64 x 64 0.19, 0.45 alone; fp32 is bound by its
-// matrix instructions, 0.47 us a unit, from 64 x 64 tiles on, so larger ones only lose parallelism).  Big tiles read the least, small
-// ones fill the chip; a long reduction with few tiles is cut into slices, whose fp32 partial products cost a second pass
-// (3 bytes per picosecond and a launch).  The estimates are within 15 % of the times measured at 4096 x 512 x 1568.
+// that has a CU to itself.  Measured (bf16; 16384 x 2048 x 2048 for the rates, the weight gradients of 2048 x 2048 x 16384 and
+// 512 x 1568 x 4096 for the steps): 256 x 256 1352 TFLOP/s, 1.13 us; 128 x 128 1137, 0.61; 128 x 64 886, 0.37; 64 x 64 718, 0.31.
+// fp32 is bound by its matrix instructions from 64 x 64 tiles on (143 TFLOP/s; 0.47 us a unit): larger ones only lose parallelism.
+// Big tiles read the least, small ones fill the chip; a long reduction with few tiles is cut into slices, whose fp32 partial products
+// cost a second pass (3 bytes per picosecond and a launch).
 struct Tile { int bm, bn; float rate, step; };
-struct Plan { int tile, slices; long kslice; };
-constexpr Tile TILES[] = {{64, 64, 5.3f, 0.45f}, {128, 64, 6.6f, 0.5f}, {128, 128, 8.0f, 0.62f}, {256, 256, 9.7f, 1.17f}};
-constexpr Tile TILES32[] = {{64, 64, 2.1f, 0.75f}, {128, 64, 2.15f, 1.2f}};
+struct Plan { int tile, slices; long kslice; float us; };
+constexpr Tile TILES[] = {{64, 64, 5.0f, 0.31f}, {128, 64, 6.6f, 0.37f}, {128, 128, 8.7f, 0.61f}, {256, 256, 10.2f, 1.13f}};
+constexpr Tile TILES32[] = {{64, 64, 2.1f, 0.75f}, {128, 64, 2.15f, 1.25f}};
+static inline const Tile& tile_of(int t, int e) { return e == 4 ? TILES32[t] : TILES[t]; }
+static inline long steps_of(long K, int e) { return (K * e + KSTEP_BYTES - 1) / KSTEP_BYTES; }
+static inline float slices_us(int slices, long M, long N) { return slices > 1 ? 3.f + (slices + 1) * 4.f * M * N / 3e6f : 0.f; }
+// f(slices, K steps in each) over the splits worth trying: at least 4 steps a slice
+template <class F>
+static inline void each_split(long steps, F&& f) {
+    for (int want = 1; want <= MAX_SLICES && (want == 1 || steps / want >= 4); want += want < 4 ? 1 : want / 2) {
+        const long per = (steps + want - 1) / want;
+        f(steps ? (int)((steps + per - 1) / per) : 1, per);
+    }
+}
 static Plan plan_of(long M, long N, long K, int e) {
-    const long kt = KSTEP_BYTES / e, steps = (K + kt - 1) / kt;
-    Plan best{0, 1, up(K, kt)};
-    float least = 0.f;
+    const long kt = KSTEP_BYTES / e, steps = steps_of(K, e);
+    Plan best{0, 1, up(K, kt), 0.f};
     for (int t = 0; t < (e == 4 ? 2 : 4); ++t) {
-        const Tile& ti = e == 4 ? TILES32[t] : TILES[t];
+        const Tile& ti = tile_of(t, e);
         const long tiles = (long)cdiv(M, ti.bm) * cdiv(N, ti.bn), units = (long)ti.bm * ti.bn / 4096;
-        for (int want = 1; want <= MAX_SLICES && (want == 1 || steps / want >= 4); want += want < 4 ? 1 : want / 2) {
-            const long per = (steps + want - 1) / want, slices = steps ? (steps + per - 1) / per : 1;
+        each_split(steps, [&](int slices, long per) {
             const float busy = (float)cdiv(tiles * slices, 256) * units / ti.rate;
-            float us = 3.f + per * (busy > ti.step ? busy : ti.step);
-            if (slices > 1) us += 3.f + (slices + 1) * 4.f * M * N / 3e6f;
-            if (least == 0.f || us < least) {
-                least = us;
-                best = Plan{t, (int)slices, slices > 1 ? per * kt : up(K, kt)};
-            }
-        }
+            const float us = 3.f + per * (busy > ti.step ? busy : ti.step) + slices_us(slices, M, N);
+            if (best.us == 0.f || us < best.us) best = Plan{t, slices, slices > 1 ? per * kt : up(K, kt), us};
+        });
     }
     return best;
 }
-
-static long slab_bytes(long M, long N, long K, int e) {
-    const Plan pl = plan_of(M, N, K, e);
-    return pl.slices > 1 ? up(4 * M * N * pl.slices, 256) : 0;
+// Both gradients of a layer in one launch (tile < 0: better apart): the units of both share the chip, the longer chain of steps bounds
+// them from below.
+struct PairPlan { int tile, slices; long kslice; };
+static PairPlan pair_plan_of(const LinArgs& dw, const LinArgs& dx, int e) {
+    const long kt = KSTEP_BYTES / e, steps = steps_of(dw.K, e), dx_steps = steps_of(dx.K, e);
+    PairPlan best{-1, 1, 0};
+    float least = plan_of(dw.M, dw.N, dw.K, e).us + plan_of(dx.M, dx.N, dx.K, e).us;
+    if (steps == 0 || dx_steps == 0) return best;
+    for (int t = 0; t < 2; ++t) {
+        const Tile& ti = tile_of(t, e);
+        const long tw = (long)cdiv(dw.M, ti.bm) * cdiv(dw.N, ti.bn), tx = (long)cdiv(dx.M, ti.bm) * cdiv(dx.N, ti.bn);
+        const float units = (float)(ti.bm * ti.bn / 4096);
+        each_split(steps, [&](int slices, long per) {
+            const float busy = ((float)tw * slices * per + (float)tx * dx_steps) * units / 256.f / ti.rate;
+            const float chain = (per > dx_steps ? per : dx_steps) * ti.step;
+            const float us = 4.f + (busy > chain ? busy : chain) + slices_us(slices, dw.M, dw.N);
+            if (us < least) least = us, best = PairPlan{t, slices, slices > 1 ? per * kt : up(dw.K, kt)};
+        });
+    }
+    return best;
 }
+static long slab_bytes(long M, long N, int slices) { return slices > 1 ? up(4 * M * N * slices, 256) : 0; }
 
 // One product with its epilogue; `slabs` holds the slices of a split reduction.  FORWARD: both operands k-contiguous, bias / activation /
 // residual; DX: A k-contiguous, B row-contiguous; DW: both row-contiguous.
 enum LinKind { LIN_FORWARD, LIN_DX, LIN_DW };
 template <class T> int linear_product(LinKind kind, const LinArgs& p, float* slabs, hipStream_t s);
+// DW and DX of one layer, in one launch where that is faster
+template <class T> int linear_gradients(LinArgs dw, LinArgs dx, float* slabs, hipStream_t s);
 
 }  // namespace acktr

@@ -3,4 +3,5 @@
 
 namespace acktr {
 template int linear_product<float>(LinKind, const LinArgs&, float*, hipStream_t);
+template int linear_gradients<float>(LinArgs, LinArgs, float*, hipStream_t);
 }

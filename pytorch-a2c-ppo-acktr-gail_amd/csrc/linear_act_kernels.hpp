@@ -89,15 +89,14 @@ __device__ __forceinline__ void spill_turn(const f32v4 (&acc)[G::MI][G::NI], int
     if constexpr (TURN + P < G::MI) spill_turn<G, P, PITCH, TURN + P>(acc, base, at);
 }
 
+// One tile of a product: workgroup `id` of the p.tiles_m * p.tiles_n ones of slice `slice`.
 // FULL: bias / activation / residual; otherwise the product is stored as it is.
-template <class T, bool AKC, bool BKC, int BM, int BN, int WM, int WN, bool FULL>
-__global__ __launch_bounds__(WM * WN * 64, (BM * BN > 128 * 128 ? WM * WN / 4 : 2)) void linear_tile_kernel(const LinArgs p) {
-    typedef TileGemm<T, AKC, BKC, BM, BN, WM, WN> G;
-    extern __shared__ char smem[];
-    ACKTR_LDS char* sm = (ACKTR_LDS char*)smem;
+template <class T, bool AKC, bool BKC, int BM, int BN, int WM, int WN, int STAGES, bool FULL>
+__device__ __forceinline__ void linear_tile(const LinArgs& p, int id, int slice, ACKTR_LDS char* sm) {
+    typedef TileGemm<T, AKC, BKC, BM, BN, WM, WN, STAGES> G;
     // Neighbouring tiles share operand rows, so each of the 8 L2 caches (workgroups go to them in turn) gets a contiguous piece
     // of the tile order, and the order walks blocks of 8 row tiles.
-    const int total = p.tiles_m * p.tiles_n, id = blockIdx.x;
+    const int total = p.tiles_m * p.tiles_n;
     const int per = (total + 7) / 8, full = total - 8 * (per - 1);            // XCDs 0 .. full-1 have `per` tiles, the others per-1
     const int x = id & 7, q = id >> 3;
     const int t = x < full ? x * per + q : full * per + (x - full) * (per - 1) + q;
@@ -105,7 +104,7 @@ __global__ __launch_bounds__(WM * WN * 64, (BM * BN > 128 * 128 ? WM * WN / 4 : 
     const int rows_in = min(8, p.tiles_m - band * 8);
     const int tm = band * 8 + inband % rows_in, tn = inband / rows_in;
     const int m0 = tm * BM, n0 = tn * BN;
-    const int k0 = blockIdx.y * p.kslice, k1 = min(p.K, k0 + p.kslice);
+    const int k0 = slice * p.kslice, k1 = min(p.K, k0 + p.kslice);
 
     G g;
     g.run(p.a, p.lda, m0, p.M, p.b, p.ldb, n0, p.N, k0, k1, sm);
@@ -144,7 +143,7 @@ __global__ __launch_bounds__(WM * WN * 64, (BM * BN > 128 * 128 ? WM * WN / 4 : 
                 fetch8(k, v);
                 if (m >= p.M || n >= p.N) continue;
                 if (p.slabs) {
-                    float* s = p.slabs + ((long)blockIdx.y * p.M + m) * p.N + n;
+                    float* s = p.slabs + ((long)slice * p.M + m) * p.N + n;
                     if (p.vec) {
                         *reinterpret_cast<f32v4*>(s) = f32v4{v[0], v[1], v[2], v[3]};
                         *reinterpret_cast<f32v4*>(s + 4) = f32v4{v[4], v[5], v[6], v[7]};
@@ -202,6 +201,24 @@ __global__ __launch_bounds__(WM * WN * 64, (BM * BN > 128 * 128 ? WM * WN / 4 : 
     else finish(std::integral_constant<int, ACKTR_ACT_NONE>{}, std::false_type{});
 }
 
+// waves a SIMD: the largest tile has it to itself with two, the others share it
+constexpr int waves_of(int bm, int bn, int waves) { return bm * bn > 128 * 128 ? waves / 4 : 2; }
+
+template <class T, bool AKC, bool BKC, int BM, int BN, int WM, int WN, int STAGES, bool FULL>
+__global__ __launch_bounds__(WM * WN * 64, waves_of(BM, BN, WM * WN)) void linear_tile_kernel(const LinArgs p) {
+    extern __shared__ char smem[];
+    linear_tile<T, AKC, BKC, BM, BN, WM, WN, STAGES, FULL>(p, blockIdx.x, blockIdx.y, (ACKTR_LDS char*)smem);
+}
+// Both gradients of a layer in one launch: the weight gradient's tiles (long reductions) first, the input gradient's fill up behind
+// them.  Apart, each leaves part of the chip idle at its end, and of a small layer most of it.
+template <class T, int BM, int BN, int STAGES>
+__global__ __launch_bounds__(256, 2) void linear_pair_kernel(const LinArgs dw, const LinArgs dx, int dw_groups) {
+    extern __shared__ char smem[];
+    const int id = blockIdx.x, per = dw.tiles_m * dw.tiles_n;
+    if (id < dw_groups) linear_tile<T, false, false, BM, BN, 2, 2, STAGES, false>(dw, id % per, id / per, (ACKTR_LDS char*)smem);
+    else linear_tile<T, true, false, BM, BN, 2, 2, STAGES, false>(dx, id - dw_groups, 0, (ACKTR_LDS char*)smem);
+}
+
 // Sum of the slices of a split reduction in slice order, then the epilogue.
 template <class T>
 __global__ __launch_bounds__(256) void linear_slabs_kernel(const LinArgs p, int slices) {
@@ -232,26 +249,36 @@ __global__ __launch_bounds__(256) void linear_slabs_kernel(const LinArgs p, int 
     }
 }
 
-template <class T, bool AKC, bool BKC, int BM, int BN, int WM, int WN, bool FULL>
-static int launch_tile(LinArgs& p, const Plan& pl, hipStream_t s) {
-    auto kern = linear_tile_kernel<T, AKC, BKC, BM, BN, WM, WN, FULL>;
-    constexpr int lds = TileGemm<T, AKC, BKC, BM, BN, WM, WN>::LDS;
-    if (lds > 65536) {                                       // once per kernel and device
-        static std::atomic<unsigned> allowed{0};
-        int dev = 0;
-        hipError_t e = hipGetDevice(&dev);
-        if (e == hipSuccess && !(allowed.load(std::memory_order_relaxed) >> (dev & 31) & 1u)) {
-            e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-            if (e == hipSuccess) allowed.fetch_or(1u << (dev & 31), std::memory_order_relaxed);
-        }
-        if (e != hipSuccess) {
-            set_error("linear_act: %d bytes of LDS refused: %s", lds, hipGetErrorString(e));
-            return (int)e;
-        }
+// more than 64 KiB of LDS are granted once per kernel and device
+static int allow_lds(const void* kern, int lds, std::atomic<unsigned>& allowed) {
+    if (lds <= 65536) return 0;
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e == hipSuccess && !(allowed.load(std::memory_order_relaxed) >> (dev & 31) & 1u)) {
+        e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e == hipSuccess) allowed.fetch_or(1u << (dev & 31), std::memory_order_relaxed);
     }
+    if (e == hipSuccess) return 0;
+    set_error("linear_act: %d bytes of LDS refused: %s", lds, hipGetErrorString(e));
+    return (int)e;
+}
+
+template <class T, bool AKC, bool BKC, int BM, int BN, int WM, int WN, int STAGES, bool FULL>
+static int launch_tile(LinArgs& p, const Plan& pl, hipStream_t s) {
+    auto kern = linear_tile_kernel<T, AKC, BKC, BM, BN, WM, WN, STAGES, FULL>;
+    constexpr int lds = TileGemm<T, AKC, BKC, BM, BN, WM, WN, STAGES>::LDS;
+    static std::atomic<unsigned> allowed{0};
+    if (int rc = allow_lds((const void*)kern, lds, allowed)) return rc;
     p.tiles_m = cdiv(p.M, BM);
     p.tiles_n = cdiv(p.N, BN);
     kern<<<dim3((unsigned)(p.tiles_m * p.tiles_n), pl.slices), dim3(WM * WN * 64), lds, s>>>(p);
+    ACKTR_LAUNCH_CHECK();
+    return 0;
+}
+
+template <class T>
+static int sum_slices(const LinArgs& p, int slices, hipStream_t s) {
+    linear_slabs_kernel<T><<<min(cdiv((long)p.M * ((p.N + 7) / 8), 256), 2048), 256, 0, s>>>(p, slices);
     ACKTR_LAUNCH_CHECK();
     return 0;
 }
@@ -263,20 +290,46 @@ static int product(LinArgs p, float* slabs, hipStream_t s) {
     p.slabs = pl.slices > 1 ? slabs : nullptr;
     int rc;
     if constexpr (sizeof(T) == 4) {
-        if (pl.tile == 0) rc = launch_tile<T, AKC, BKC, 64, 64, 2, 2, FULL>(p, pl, s);
-        else rc = launch_tile<T, AKC, BKC, 128, 64, 2, 2, FULL>(p, pl, s);
+        if (pl.tile == 0) rc = launch_tile<T, AKC, BKC, 64, 64, 2, 2, 2, FULL>(p, pl, s);
+        else rc = launch_tile<T, AKC, BKC, 128, 64, 2, 2, 3, FULL>(p, pl, s);
     } else {
         switch (pl.tile) {
-            case 0: rc = launch_tile<T, AKC, BKC, 64, 64, 2, 2, FULL>(p, pl, s); break;
-            case 1: rc = launch_tile<T, AKC, BKC, 128, 64, 2, 2, FULL>(p, pl, s); break;
-            case 2: rc = launch_tile<T, AKC, BKC, 128, 128, 2, 2, FULL>(p, pl, s); break;
-            default: rc = launch_tile<T, AKC, BKC, 256, 256, 2, 4, FULL>(p, pl, s);
+            case 0: rc = launch_tile<T, AKC, BKC, 64, 64, 2, 2, 3, FULL>(p, pl, s); break;
+            case 1: rc = launch_tile<T, AKC, BKC, 128, 64, 2, 2, 3, FULL>(p, pl, s); break;
+            case 2: rc = launch_tile<T, AKC, BKC, 128, 128, 2, 2, 2, FULL>(p, pl, s); break;
+            default: rc = launch_tile<T, AKC, BKC, 256, 256, 2, 4, 2, FULL>(p, pl, s);
         }
     }
     if (rc || pl.slices == 1) return rc;
-    linear_slabs_kernel<T><<<min(cdiv((long)p.M * ((p.N + 7) / 8), 256), 2048), 256, 0, s>>>(p, pl.slices);
+    return sum_slices<T>(p, pl.slices, s);
+}
+
+template <class T, int BM, int BN, int STAGES>
+static int launch_pair(LinArgs& dw, LinArgs& dx, int slices, hipStream_t s) {
+    auto kern = linear_pair_kernel<T, BM, BN, STAGES>;
+    constexpr int lds = TileGemm<T, true, false, BM, BN, 2, 2, STAGES>::LDS;
+    static std::atomic<unsigned> allowed{0};
+    if (int rc = allow_lds((const void*)kern, lds, allowed)) return rc;
+    dw.tiles_m = cdiv(dw.M, BM), dw.tiles_n = cdiv(dw.N, BN);
+    dx.tiles_m = cdiv(dx.M, BM), dx.tiles_n = cdiv(dx.N, BN);
+    const int first = dw.tiles_m * dw.tiles_n * slices;
+    kern<<<first + dx.tiles_m * dx.tiles_n, 256, lds, s>>>(dw, dx, first);
     ACKTR_LAUNCH_CHECK();
     return 0;
+}
+
+template <class T>
+int linear_gradients(LinArgs dw, LinArgs dx, float* slabs, hipStream_t s) {
+    const PairPlan pl = pair_plan_of(dw, dx, sizeof(T));
+    if (pl.tile < 0) {
+        if (int rc = product<T, true, false, false>(dx, slabs, s)) return rc;
+        return product<T, false, false, false>(dw, slabs, s);
+    }
+    dw.kslice = (int)pl.kslice, dw.slabs = pl.slices > 1 ? slabs : nullptr;
+    dx.kslice = dx.K, dx.slabs = nullptr;
+    const int rc = pl.tile == 0 ? launch_pair<T, 64, 64, sizeof(T) == 4 ? 2 : 3>(dw, dx, pl.slices, s) : launch_pair<T, 128, 64, 3>(dw, dx, pl.slices, s);
+    if (rc || pl.slices == 1) return rc;
+    return sum_slices<T>(dw, pl.slices, s);
 }
 
 template <class T>

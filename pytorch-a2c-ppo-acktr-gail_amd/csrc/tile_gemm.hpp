@@ -11,8 +11,9 @@
 //                      read with the transposing ds_read_b64_tr_b16 (a group of 16 lanes reads 4 lines x 16 rows and gets 4
 //                      consecutive k of its row each); fp32 fragments with one ds_read_b32 per k.
 // * A K step is 128 bytes of k (64 16-bit or 32 fp32 values), cut into two halves that alternate in registers: while the
-//   matrix cores work on one half, the other half is read from LDS; the next K step's memory loads are in flight for a
-//   whole K step.  One barrier per K step.
+//   matrix cores work on one half, the other half is read from LDS.  STAGES K steps have a place in LDS: memory loads are in
+//   flight for STAGES - 1 K steps (a large tile computes long enough on one step to cover the latency with 2 stages, 64 x 64
+//   needs 4).  One barrier per K step, which waits for the oldest loads only.
 // * The products are formed transposed (B's rows on the matrix instruction's row side), so that a lane ends up with four
 //   consecutive n of one m.  fp32 uses v_mfma_f32_16x16x4 on the same fragments: a lane group's four consecutive k are four
 //   instructions, each pairing the same k of A and B.
@@ -38,8 +39,12 @@ __device__ __forceinline__ void dma16(const void* base, unsigned off, unsigned l
 __device__ __forceinline__ void dma16_ptr(const void* p, unsigned lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory");
 }
-// every load and LDS access of this wave is done, then the workgroup's
-__device__ __forceinline__ void tile_sync() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// all but the newest LEFT loads and every LDS access of this wave are done, then the workgroup's
+template <int LEFT>
+__device__ __forceinline__ void tile_sync() {
+    static_assert(LEFT >= 0 && LEFT < 64, "the counter has 6 bits");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
+}
 
 __device__ __forceinline__ f32v4 mfma_half(const s16v8& a, const s16v8& b, const f32v4& c, __bf16) {
     typedef __bf16 v8 __attribute__((ext_vector_type(8)));
@@ -102,7 +107,7 @@ struct TileOperand {
     }
     // kleft: k that are left at this K step; lds: uniform address of the stage
     __device__ __forceinline__ void load(int kleft, unsigned lds, int wave) {
-        if (kleft >= KT) {
+        if (kleft >= KT) {                           // (uniform)
 #pragma unroll
             for (int i = 0; i < ITERS; ++i) dma16(base, off[i], lds + (i * NT + wave * 64) * 16);
         } else {
@@ -141,12 +146,13 @@ struct TileOperand {
 
 // A workgroup's BM x BN tile by WM x WN waves.  After run(): lane holds acc[mi][ni][i] = D(m, n) with
 // m = wave's first row + 16 mi + lane % 16, n = wave's first column + 16 ni + 4 (lane / 16) + i.
-template <class T, bool AKC, bool BKC, int BM, int BN, int WM, int WN>
+template <class T, bool AKC, bool BKC, int BM, int BN, int WM, int WN, int STAGES>
 struct TileGemm {
     static constexpr int NT = WM * WN * 64, MI = BM / WM / 16, NI = BN / WN / 16;
     typedef TileOperand<T, AKC, BM, NT> OpA;
     typedef TileOperand<T, BKC, BN, NT> OpB;
-    static constexpr int KT = OpA::KT, STAGE = OpA::BYTES + OpB::BYTES, LDS = 2 * STAGE;
+    static constexpr int KT = OpA::KT, STAGE = OpA::BYTES + OpB::BYTES, LDS = STAGES * STAGE;
+    static constexpr int LOADS = OpA::ITERS + OpB::ITERS;         // a wave's load instructions for a K step
 
     f32v4 acc[MI][NI];
 
@@ -189,26 +195,28 @@ struct TileGemm {
 #pragma unroll
             for (int j = 0; j < NI; ++j) acc[i][j] = f32v4{0.f, 0.f, 0.f, 0.f};
         int left = k1 - k0;                              // k not yet requested
-        auto request = [&](unsigned stage) {
+        const int steps = (k1 - k0 + KT - 1) / KT;
+        if (steps <= 0) return;
+        // the request for the K step that follows the last one requested; behind the end it fetches zeros, so that the number of
+        // loads in flight stays what the waits count on
+        auto request = [&](unsigned stage) __attribute__((always_inline)) {
             oa.load(left, lds + stage, wave);
             ob.load(left, lds + stage + OpA::BYTES, wave);
             left -= KT;
         };
-        const int steps = (k1 - k0 + KT - 1) / KT;
-        if (steps <= 0) return;
         s16v8 fa0[MI], fb0[NI], fa1[MI], fb1[NI];
-        request(0);
-        tile_sync();
-        if (steps > 1) request(STAGE);
+#pragma unroll
+        for (int i = 0; i < STAGES; ++i) request(i * STAGE);
+        tile_sync<(STAGES - 1) * LOADS>();
         frags(sm, 0, wm, wn, lane, fa0, fb0);
         unsigned cur = 0;
         for (int t = 0; t + 1 < steps; ++t) {
             frags(sm + cur, 1, wm, wn, lane, fa1, fb1);
             products(fa0, fb0);
             interleave();
-            tile_sync();                                 // this stage is read, the other one has arrived
-            if (t + 2 < steps) request(cur);
-            cur ^= STAGE;
+            tile_sync<(STAGES - 2) * LOADS>();           // this stage is read, the next one has arrived
+            request(cur);
+            cur = cur + STAGE == LDS ? 0 : cur + STAGE;
             frags(sm + cur, 0, wm, wn, lane, fa0, fb0);
             products(fa1, fb1);
             interleave();
@@ -216,6 +224,7 @@ struct TileGemm {
         frags(sm + cur, 1, wm, wn, lane, fa1, fb1);
         products(fa0, fb0);
         products(fa1, fb1);
+        tile_sync<0>();                                  // LDS is the caller's again
     }
 };
 
