@@ -566,14 +566,14 @@ long acktr_linear_act_fwd_workspace_bytes(const void* x, long ldx, const void* w
 int acktr_linear_act_fwd(const void* x, long ldx, const void* w, long ldw, const void* bias, const void* residual, long ldr, void* y,
                          long ldy, void* pre, long ldp, long M, long N, long K, int dtype, int act, void* workspace,
                          long workspace_bytes, void* stream);
-/* dz = dy act'(z) with the slopes in pre, dx[M, K] = dz w, dw[N, K] = dz^T x, db[N] = sum of dz over rows; dx, dw, db nullable (not computed then; w is
+/* dz = dy act'(z) with the slopes in pre, dx[M, K] = dz w + dx_add (nullable: what reaches x by other ways), dw[N, K] = dz^T x, db[N] = sum of dz over rows; dx, dw, db nullable (not computed then; w is
  * needed for dx only, x for dw only).  dw and db are dense.  dz is rounded to the storage type before the products.  The residual's
  * gradient is dy itself.  With M = 0, dw and db are zero.  Sums over rows are in a fixed order: results repeat bit for bit. */
 long acktr_linear_act_bwd_workspace_bytes(const void* dy, long lddy, const void* x, long ldx, const void* w, long ldw, const void* pre,
                                           long ldp, int dx, int dw, int db, long M, long N, long K, int dtype, int act);
 int acktr_linear_act_bwd(const void* dy, long lddy, const void* x, long ldx, const void* w, long ldw, const void* pre, long ldp,
-                         void* dx, long lddx, void* dw, void* db, long M, long N, long K, int dtype, int act, void* workspace,
-                         long workspace_bytes, void* stream);
+                         const void* dx_add, long ldxa, void* dx, long lddx, void* dw, void* db, long M, long N, long K, int dtype, int act,
+                         void* workspace, long workspace_bytes, void* stream);
 
 /* Gated linear recurrence over T steps of N sequences of H channels, f = sigmoid(gate):
  *   h_t = f_t (m_t h_{t-1}) + (1 - f_t) value_t,  h_{-1} = h0 (fp32 [N, H], nullable: zeros),  m = masks (fp32 [T, N], nullable: ones)

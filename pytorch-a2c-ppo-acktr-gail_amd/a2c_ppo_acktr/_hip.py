@@ -192,7 +192,7 @@ _PROTOS = {
     'acktr_linear_act_fwd_workspace_bytes': (c_l, [c_p, c_l, c_p, c_l, c_l, c_l, c_l, c_i]),
     'acktr_linear_act_fwd': (c_i, [c_p, c_l, c_p, c_l, c_p, c_p, c_l, c_p, c_l, c_p, c_l, c_l, c_l, c_l, c_i, c_i, c_p, c_l, c_p]),
     'acktr_linear_act_bwd_workspace_bytes': (c_l, [c_p, c_l] * 4 + [c_i] * 3 + [c_l] * 3 + [c_i] * 2),
-    'acktr_linear_act_bwd': (c_i, [c_p, c_l] * 5 + [c_p, c_p] + [c_l] * 3 + [c_i] * 2 + [c_p, c_l, c_p]),
+    'acktr_linear_act_bwd': (c_i, [c_p, c_l] * 6 + [c_p, c_p] + [c_l] * 3 + [c_i] * 2 + [c_p, c_l, c_p]),
     'acktr_gated_scan_save_interval': (c_i, []),
     'acktr_gated_scan_workspace_bytes': (c_l, [c_l, c_l, c_l, c_i]),
     'acktr_gated_scan_fwd': (c_i, [c_p, c_l, c_l] * 2 + [c_p, c_p] + [c_p, c_l, c_l] + [c_p, c_p] + [c_l] * 3 + [c_i, c_p, c_l, c_p]),

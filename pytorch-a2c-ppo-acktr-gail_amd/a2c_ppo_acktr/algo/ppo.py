@@ -12,6 +12,7 @@ import os
 import torch
 
 from .. import _hip, engine, ops
+from .adamw import AdamW
 from ..parallel import DataParallel, bounded_sync, quiesce_collectives
 
 # ACKTR_DEFER_HEAD=0: the head step finalizes in its own launch (comparison switch)
@@ -82,7 +83,29 @@ class _FlatAdam(object):
         _hip.check(rc, 'acktr_clip_adam_dev_f32')
 
 
+class _PolicyAdamW(AdamW):
+    """AdamW (decoupled weight decay) over a policy's parameters and its flat gradient buffer, with _FlatAdam's interface."""
+
+    def __init__(self, policy, lr, eps, weight_decay, state_bits, max_grad_norm):
+        super(_PolicyAdamW, self).__init__(list(policy.parameters()), lr=lr, eps=eps, weight_decay=weight_decay,
+                                           max_grad_norm=max_grad_norm or None, state_bits=state_bits)
+        self.policy = policy
+
+    def _gradients(self):
+        return [self.policy.grad_view(p) for p in self.params]
+
+    def zero_grad(self, set_to_none=False):
+        self.policy.flat_grads.zero_()
+
+    def step(self, max_grad_norm=None, capturing=False, **unused):
+        self.param_groups[0]['max_grad_norm'] = max_grad_norm if max_grad_norm else None
+        super(_PolicyAdamW, self).step()
+
+
 class PPO():
+    """weight_decay (not in the reference): a number switches the optimiser from Adam to AdamW, whose moments take state_bits (32 or
+    8) bits."""
+
     def __init__(self,
                  actor_critic,
                  clip_param,
@@ -93,7 +116,9 @@ class PPO():
                  lr=None,
                  eps=None,
                  max_grad_norm=None,
-                 use_clipped_value_loss=True):
+                 use_clipped_value_loss=True,
+                 weight_decay=None,
+                 state_bits=32):
 
         self.actor_critic = actor_critic
 
@@ -107,7 +132,12 @@ class PPO():
         self.max_grad_norm = max_grad_norm
         self.use_clipped_value_loss = use_clipped_value_loss
 
-        self.optimizer = _FlatAdam(actor_critic, lr=lr, eps=eps)
+        # only the flat Adam can ride in other launches (one-launch MLP step, deferred sums, conv weight images)
+        self._flat = weight_decay is None
+        if self._flat and state_bits != 32:
+            raise ValueError('state_bits belongs to weight_decay: Adam keeps 32-bit moments')
+        self.optimizer = _FlatAdam(actor_critic, lr=lr, eps=eps) if self._flat else \
+            _PolicyAdamW(actor_critic, lr, eps, weight_decay, state_bits, max_grad_norm)
         self.dp = DataParallel()
         # hipGraph replay of the minibatch step (launch-bound otherwise): captured at the second update() that
         # sees the same storage / shapes; ACKTR_HIP_GRAPH=0 disables it.
@@ -126,6 +156,7 @@ class PPO():
         all-reduce of the late gradient bucket (conv3, FC, head: 97 % of the bytes) overlaps with the rest of the
         backward: phase 1 = forward, loss, backward down to conv3's weights; phase 2 = the remaining backward."""
         ac = self.actor_critic
+        with_optimizer = with_optimizer and self._flat
         if phase == 2:
             engine.backward(ac, self._acts, ac.flat_grads, phase=2)
             return
@@ -200,7 +231,7 @@ class PPO():
         # the conv weight images are re-ordered ONCE per update (whatever happened to the parameters since the last one);
         # inside the update the Adam steps keep them current, so the minibatch steps have no pack launch
         with torch.no_grad():
-            self._image_map = engine.refresh_conv_images(ac, hi - lo) if self.max_grad_norm else None
+            self._image_map = engine.refresh_conv_images(ac, hi - lo) if self.max_grad_norm and self._flat else None
         key = (self._image_map.base if self._image_map is not None else None, rollouts.obs.data_ptr(), rollouts.actions.data_ptr(), rollouts.returns.data_ptr(),
                rollouts.value_preds.data_ptr(), rollouts.action_log_probs.data_ptr(), T, N, mbs, lo, hi,
                ac.flat_params.data_ptr(), self.clip_param, self.value_loss_coef, self.entropy_coef,

@@ -7,7 +7,7 @@ CNN  (reference model.py:189-195, distributions.py:71-73):
 MLP  (reference model.py:220-229, distributions.py:86-95):
     separate tanh towers for critic and actor, value head on the critic tower, mean head on the actor.
 
-Recurrent bases (model.py:111-166): a GRU between the trunk and the heads (CNN: on the FC features; MLP: on the raw
+Recurrent bases (model.py:111-166; `recurrent='gated'`: gated_forward / gated_backward in its place): a GRU between the trunk and the heads (CNN: on the FC features; MLP: on the raw
 inputs, the towers then read the GRU output).  `gru_forward` / `gru_backward` below run it over [T*N] rows (row
 t*N+n) as one input GEMM for all steps + per step one hidden GEMM and one gate kernel (csrc/gru.hip).
 
@@ -148,25 +148,84 @@ def gru_params(policy):
     return g.weight_ih_l0, g.weight_hh_l0, g.bias_ih_l0, g.bias_hh_l0
 
 
-def gru_forward(policy, a, x_seq, hxs, masks):
-    """model.py:111-166.  x_seq [T*N, I] (row t*N+n), hxs [N, H], masks [T*N(,1)].  The carried state is multiplied by
-    masks[t] at every step -- the same arithmetic as the reference's chunking, whose skipped multiplications are by
-    exactly 1.0.  Leaves on `a`: gru_out [T*N, H], hxs_out [N, H] (view of the last step) and what BPTT needs
-    (gru_rzn = r,z,n per row; gru_gh = W_hh products; gru_hm = masked previous states; gru_x, gru_masks)."""
+def rnn_rows(x_seq, hxs, masks, H):
+    """(hxs [N, H], masks [T*N], T, N) of a recurrent forward pass over x_seq [T*N, I]"""
     if hxs is None or masks is None:
         raise RuntimeError('a recurrent policy needs rnn_hxs and masks')
     dev = x_seq.device
-    w_ih, w_hh, b_ih, b_hh = gru_params(policy)
-    H = w_hh.shape[1]
     hxs = hxs.to(dev, f32).reshape(-1, H).contiguous()
-    N = hxs.shape[0]
-    B = x_seq.shape[0]
-    T = B // N
+    N, B = hxs.shape[0], x_seq.shape[0]
+    T = B // max(N, 1)
     if T * N != B or T < 1:
         raise RuntimeError('recurrent forward: %d input rows are not a multiple of the %d hidden-state rows' % (B, N))
     masks = masks.to(dev, f32).reshape(-1).contiguous()
     if masks.numel() != B:
         raise RuntimeError('recurrent forward: expected %d mask entries, got %d' % (B, masks.numel()))
+    return hxs, masks, T, N
+
+
+def gated_forward(policy, a, x_seq, hxs, masks, infer=False):
+    """The gated core (gated.GatedCore) in the place of the GRU: y = h + silu(W_out h + b_out) over the states
+    h_t = f_t (m_t h_{t-1}) + (1 - f_t) v_t, where (gate | value) = W_in x + b_in and f = sigmoid(gate).  The recurrence is linear in
+    the state, so all T steps are ONE scan instead of T dependent launches.  Leaves gru_out [T*N, H] and hxs_out [N, H] on `a` like
+    gru_forward, and what gated_backward needs.  infer: a single step that nobody differentiates (Policy.act / get_value)."""
+    core = policy.base.core
+    H = core.hidden_size
+    hxs, masks, T, N = rnn_rows(x_seq, hxs, masks, H)
+    (w_in, b_in), (w_out, b_out) = _wb(core.in_proj), _wb(core.out_proj)
+    proj = ops.linear_act_fwd(x_seq, w_in, b_in)                       # all steps at once: [T*N, 2H]
+    if infer and T == 1:
+        state = hxs.clone()
+        h = ops.gated_scan_step(proj[:, :H], proj[:, H:], state, masks)
+        a.gru_out, a.hxs_out = ops.linear_act_fwd(h, w_out, b_out, act='silu', residual=h), state
+        return a.gru_out
+    p3 = proj.view(T, N, 2 * H)
+    m2 = masks.view(T, N)
+    h3, last, saved = ops.gated_scan_fwd(p3[..., :H], p3[..., H:], hxs, m2, save=True)
+    h = h3.view(T * N, H)
+    pre = torch.empty_like(h)
+    a.gru_out = ops.linear_act_fwd(h, w_out, b_out, act='silu', residual=h, pre=pre)
+    a.hxs_out = last
+    a.core = (x_seq, p3, hxs, m2, saved, h, pre)
+    return a.gru_out
+
+
+def gated_backward(policy, a, dout, gflat, wgrad=True, dx_gate_src=None, dx_gate=None, need_dx=True):
+    """Backward pass of gated_forward, with gru_backward's arguments and result."""
+    core = policy.base.core
+    H = core.hidden_size
+    (w_in, b_in), (w_out, b_out) = _wb(core.in_proj), _wb(core.out_proj)
+    x, p3, hxs, m2, saved, h, pre = a.core
+    T, N = m2.shape
+    gv = (lambda p: policy.grad_view(p, gflat)) if wgrad else (lambda p: None)
+    dout = dout.contiguous()
+    dh, _, _ = ops.linear_act_bwd(dout, h, w_out, pre=pre, act='silu', dw=gv(w_out), db=gv(b_out), need_dw=wgrad, need_db=wgrad,
+                                  dx_add=dout)                         # h also reaches the output as the residual
+    dproj = torch.empty_like(p3)
+    ops.gated_scan_bwd(dh.view(T, N, H), p3[..., :H], p3[..., H:], hxs, m2, saved=saved, dgate=dproj[..., :H], dvalue=dproj[..., H:],
+                       need_dh0=False)
+    dproj = dproj.view(T * N, 2 * H)
+    gated = need_dx and dx_gate is not None
+    dx = None
+    if wgrad or (need_dx and not gated):
+        dx, _, _ = ops.linear_act_bwd(dproj, x, w_in, dw=gv(w_in), db=gv(b_in), need_dx=need_dx and not gated, need_dw=wgrad, need_db=wgrad)
+    if gated:
+        dx = ops.linear_dgrad(dproj, w_in, gate_src=dx_gate_src, gate=dx_gate)
+    return dx
+
+
+def gru_forward(policy, a, x_seq, hxs, masks, infer=False):
+    """model.py:111-166.  x_seq [T*N, I] (row t*N+n), hxs [N, H], masks [T*N(,1)].  The carried state is multiplied by
+    masks[t] at every step -- the same arithmetic as the reference's chunking, whose skipped multiplications are by
+    exactly 1.0.  Leaves on `a`: gru_out [T*N, H], hxs_out [N, H] (view of the last step) and what BPTT needs
+    (gru_rzn = r,z,n per row; gru_gh = W_hh products; gru_hm = masked previous states; gru_x, gru_masks)."""
+    if hasattr(policy.base, 'core'):
+        return gated_forward(policy, a, x_seq, hxs, masks, infer)
+    dev = x_seq.device
+    w_ih, w_hh, b_ih, b_hh = gru_params(policy)
+    H = w_hh.shape[1]
+    hxs, masks, T, N = rnn_rows(x_seq, hxs, masks, H)
+    B = x_seq.shape[0]
     L = _hip.lib()
     stream = _hip.cur_stream(dev)
     gi = ops.linear_fwd(x_seq, w_ih, b_ih, None)                       # all steps at once: [T*N, 3H]
@@ -207,6 +266,8 @@ def gru_backward(policy, a, dout, gflat, wgrad=True, dx_gate_src=None, dx_gate=N
     """BPTT through gru_forward.  dout [T*N, H] = d loss / d gru_out.  Overwrites the saved gates with d gi / d gh,
     writes the four GRU parameter gradients into `gflat` and returns d loss / d x_seq (gated by `dx_gate` on
     `dx_gate_src` when the GRU input was an activation output), or None."""
+    if hasattr(policy.base, 'core'):
+        return gated_backward(policy, a, dout, gflat, wgrad, dx_gate_src, dx_gate, need_dx)
     w_ih, w_hh, b_ih, b_hh = gru_params(policy)
     T, N = a.gru_T, a.gru_N
     H = w_hh.shape[1]
@@ -304,7 +365,7 @@ def forward(policy, inputs, gather_idx=None, rnn_hxs=None, masks=None, head=True
             a._feat_fn = lambda: ops.linear_fwd(a.flat3, L['fc'][0], L['fc'][1].view(-1), 'relu')
             return a
         a.feat = ops.linear_fwd(a.flat3, L['fc'][0], L['fc'][1].view(-1), 'relu')
-        a.head_in = gru_forward(policy, a, a.feat, rnn_hxs, masks) if rec else a.feat
+        a.head_in = gru_forward(policy, a, a.feat, rnn_hxs, masks, infer=not gate_bits) if rec else a.feat
         if head:
             wh, bh = head_views(policy, policy.flat_params)
             a.head = ops.linear_fwd(a.head_in, wh, bh, None)
@@ -316,7 +377,7 @@ def forward(policy, inputs, gather_idx=None, rnn_hxs=None, masks=None, head=True
         inputs = RolloutStorage._gather(inputs, gather_idx, inputs.shape[0])
     a.obs = inputs
     if rec:
-        inputs = gru_forward(policy, a, inputs, rnn_hxs, masks)
+        inputs = gru_forward(policy, a, inputs, rnn_hxs, masks, infer=not gate_bits)
     a.tower_in = inputs
     a.hc1 = ops.linear_fwd(inputs, L['c0'][0], L['c0'][1].view(-1), 'tanh')
     a.hc2 = ops.linear_fwd(a.hc1, L['c2'][0], L['c2'][1].view(-1), 'tanh')

@@ -12,6 +12,8 @@ be two launches and the data-parallel all-reduce a single bucket.
 
 Recurrent bases (`base_kwargs={'recurrent': True}`, model.py:89-95,111-166): `base.gru` is an nn.GRU used as a
 parameter container like the rest; the sequence runs in engine.gru_forward / gru_backward.
+`base_kwargs={'recurrent': 'gated'}` (not in the reference): `base.core`, a gated linear recurrence (gated.GatedCore), takes the
+GRU's place -- same interface, hidden state and masks; parallel over time steps.
 
 Not built: the broken Bernoulli head (reference distributions.py:49-50, F11).
 """
@@ -75,7 +77,7 @@ class Policy(nn.Module):
         """Groups of parameters that must be contiguous; each group starts 16-byte aligned."""
         if isinstance(self.base, CNNBase):
             w = engine.cnn_layer_params(self)
-            groups = [[p] for p in self.base.gru.parameters()] if self.base.is_recurrent else []
+            groups = [[p] for p in self.base.rnn.parameters()] if self.base.is_recurrent else []
             for name in ('conv1', 'conv2', 'conv3', 'fc'):
                 groups.append([w[name][0]])
                 groups.append([w[name][1]])
@@ -242,14 +244,23 @@ class NNBase(nn.Module):
     def __init__(self, recurrent, recurrent_input_size, hidden_size):
         super(NNBase, self).__init__()
         self._hidden_size = hidden_size
-        self._recurrent = recurrent
-        if recurrent:                                   # reference model.py:89-95 (same initialiser calls, same order)
+        if recurrent not in (True, False, 'gated'):
+            raise ValueError("recurrent must be True, False or 'gated' (got %r)" % (recurrent,))
+        self._recurrent = bool(recurrent)
+        if recurrent == 'gated':
+            from .gated import GatedCore
+            self.core = GatedCore(recurrent_input_size, hidden_size)
+        elif recurrent:                                 # reference model.py:89-95 (same initialiser calls, same order)
             self.gru = nn.GRU(recurrent_input_size, hidden_size)
             for name, param in self.gru.named_parameters():
                 if 'bias' in name:
                     nn.init.constant_(param, 0)
                 elif 'weight' in name:
                     nn.init.orthogonal_(param)
+
+    @property
+    def rnn(self):
+        return self.core if hasattr(self, 'core') else self.gru
 
     @property
     def is_recurrent(self):

@@ -619,9 +619,10 @@ def linear_act_fwd(x, w, bias=None, act=None, residual=None, out=None, pre=None)
     return out
 
 
-def linear_act_bwd(dy, x, w, pre=None, act=None, dx=None, dw=None, db=None, need_dx=True, need_dw=True, need_db=True):
+def linear_act_bwd(dy, x, w, pre=None, act=None, dx=None, dw=None, db=None, need_dx=True, need_dw=True, need_db=True, dx_add=None):
     """(dx, dw, db) of linear_act_fwd for dy [M, N] = the derivative by its output (the residual's gradient is dy itself).
-    pre: what the forward pass left there (not needed without an activation).  Gradients that are not needed are None."""
+    pre: what the forward pass left there (not needed without an activation).  dx_add [M, K]: added to dx
+    before it is rounded (what reaches x by another way, a residual's gradient).  Gradients that are not needed are None."""
     code, act = _dtype_code(dy, 'dy'), _act_code(act)
     if dy.dim() != 2 or x.dim() != 2 or w.dim() != 2 or x.shape[0] != dy.shape[0] or tuple(w.shape) != (dy.shape[1], x.shape[1]):
         raise RuntimeError('linear_act_bwd: dy [M, N], x [M, K] and w [N, K] expected, got %s, %s and %s'
@@ -636,8 +637,10 @@ def linear_act_bwd(dy, x, w, pre=None, act=None, dx=None, dw=None, db=None, need
     px, ldx = _rows(x, 'x', (M, K), dt, at)
     pw, ldw = _rows(w, 'w', (N, K), dt, at)
     pz, ldz = _rows(pre, 'pre', (M, N), dt, at) if pre is not None else (None, 0)
-    qx = qw = qb = None
-    ldq = 0
+    qx = qw = qb = pa = None
+    ldq = lda = 0
+    if dx_add is not None:
+        pa, lda = _rows(dx_add, 'dx_add', (M, K), dt, at)
     if need_dx:
         dx = dy.new_empty((M, K)) if dx is None else dx
         qx, ldq = _rows(dx, 'dx', (M, K), dt, at)
@@ -648,11 +651,11 @@ def linear_act_bwd(dy, x, w, pre=None, act=None, dx=None, dw=None, db=None, need
         db = dy.new_empty(N) if db is None else db
         qb = _vec(db, 'db', N, dt, at)
     for i, a in enumerate(given):
-        _apart(a, 'a gradient', (dy, x, w, pre) + tuple(given[:i]), 'linear_act_bwd')
+        _apart(a, 'a gradient', (dy, x, w, pre, None if a is dx and qx == pa and ldq == lda else dx_add) + tuple(given[:i]), 'linear_act_bwd')
     L = _hip.lib()
     nb = L.acktr_linear_act_bwd_workspace_bytes(pg, ldg, px, ldx, pw, ldw, pz, ldz, need_dx, need_dw, need_db, M, N, K, code, act)
     ws = _scratch(nb, dy, 'acktr_linear_act_bwd') if nb else None
-    _launch(L.acktr_linear_act_bwd, (pg, ldg, px, ldx, pw, ldw, pz, ldz, qx, ldq, qw, qb, M, N, K, code, act, ws.data_ptr() if nb else None, nb),
+    _launch(L.acktr_linear_act_bwd, (pg, ldg, px, ldx, pw, ldw, pz, ldz, pa, lda, qx, ldq, qw, qb, M, N, K, code, act, ws.data_ptr() if nb else None, nb),
             at, 'linear_act_bwd', 2.0 * M * N * K * (bool(need_dx) + bool(need_dw)))
     return dx if need_dx else None, dw if need_dw else None, db if need_db else None
 

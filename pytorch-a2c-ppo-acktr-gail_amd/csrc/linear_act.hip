@@ -217,13 +217,13 @@ extern "C" long acktr_linear_act_bwd_workspace_bytes(const void* dy, long lddy, 
 }
 
 extern "C" int acktr_linear_act_bwd(const void* dy, long lddy, const void* x, long ldx, const void* w, long ldw, const void* pre, long ldp,
-                                    void* dx, long lddx, void* dw, void* db, long M, long N, long K, int dtype, int act, void* workspace,
+                                    const void* dx_add, long ldxa, void* dx, long lddx, void* dw, void* db, long M, long N, long K, int dtype, int act, void* workspace,
                                     long workspace_bytes, void* stream) {
     if (int rc = check_dims(M, K, N, dtype, act)) return rc;
     if (check_ld("dy", lddy, N)) return -1;
     ACKTR_ARG(!dx || w, "linear_act_bwd: dx needs w");
     ACKTR_ARG(!dw || x || M == 0, "linear_act_bwd: dw needs x");
-    if ((dx && (check_ld("w", ldw, K) || check_ld("dx", lddx, K))) || (dw && check_ld("x", ldx, K))) return -1;
+    if ((dx && (check_ld("w", ldw, K) || check_ld("dx", lddx, K) || (dx_add && check_ld("dx_add", ldxa, K)))) || (dw && check_ld("x", ldx, K))) return -1;
     ACKTR_ARG(act == ACKTR_ACT_NONE || pre || M == 0, "linear_act_bwd: an activation's gradient needs what the forward pass left in `pre`");
     if (act != ACKTR_ACT_NONE && check_ld("pre", ldp, N)) return -1;
     ACKTR_ARG(M == 0 || dy, "linear_act_bwd: dy is required");
@@ -276,7 +276,8 @@ extern "C" int acktr_linear_act_bwd(const void* dy, long lddy, const void* x, lo
         LinArgs px{}, pw{};
         px.a = dz, px.lda = lddz, px.b = sp.pw ? w_ws : w, px.ldb = sp.pw ? kp : ldw;      // dx[M, K] = dz[M, N] w[N, K]: sum over N
         px.M = (int)M, px.N = (int)K, px.K = (int)N;
-        px.y = dx, px.ldy = lddx, px.vec = K % 8 == 0 && rows16(dx, lddx, e);
+        px.y = dx, px.ldy = lddx, px.res = dx_add, px.ldr = ldxa;
+        px.vec = K % 8 == 0 && rows16(dx, lddx, e) && (!dx_add || rows16(dx_add, ldxa, e));
         pw.a = dz, pw.lda = lddz, pw.b = sp.px ? x_ws : x, pw.ldb = sp.px ? kp : ldx;      // dw[N, K] = dz^T x: sum over M
         pw.M = (int)N, pw.N = (int)K, pw.K = (int)M;
         pw.y = dw, pw.ldy = K, pw.vec = K % 8 == 0 && rows16(dw, K, e);

@@ -169,7 +169,7 @@ __device__ __forceinline__ void linear_tile(const LinArgs& p, int id, int slice,
         if constexpr (FULL) load_bias8<T>(p, n, b);
         else
             for (int i = 0; i < 8; ++i) b[i] = 0.f;
-        const bool res = FULL && p.res;
+        const bool res = p.res;
         vec_t<T, 8> r[IT];
         // a turn's residual rows are requested a turn ahead: their latency passes under the turn before
         auto residual = [&](int base) __attribute__((always_inline)) {

@@ -34,9 +34,9 @@ def test_linear_entry_arguments():
         assert fwd(**kw) == -1 and err(), kw
     assert fwd(M=0) == 0
     assert L.acktr_linear_act_fwd_workspace_bytes(one, 8, one, 8, 4, 8, 8, 9) == -1
-    bwd = lambda act=0, pre=None, dy=one, x=one, w=one, dx=one, dw=one, ldp=8, lddx=8, dt=1, nb=1 << 20: L.acktr_linear_act_bwd(
-        dy, 8, x, 8, w, 8, pre, ldp, dx, lddx, dw, None, 4, 8, 8, dt, act, one, nb, None)
-    for kw in (dict(act=2), dict(act=2, pre=one, ldp=7), dict(dy=None), dict(x=None), dict(w=None), dict(lddx=3), dict(dt=-1), dict(act=2, pre=one, nb=0)):
+    bwd = lambda act=0, pre=None, add=None, dy=one, x=one, w=one, dx=one, dw=one, ldp=8, lddx=8, dt=1, nb=1 << 20: L.acktr_linear_act_bwd(
+        dy, 8, x, 8, w, 8, pre, ldp, add, 5, dx, lddx, dw, None, 4, 8, 8, dt, act, one, nb, None)
+    for kw in (dict(act=2), dict(act=2, pre=one, ldp=7), dict(dy=None), dict(x=None), dict(w=None), dict(lddx=3), dict(add=one), dict(dt=-1), dict(act=2, pre=one, nb=0)):
         assert bwd(**kw) == -1 and err(), kw
 
 

@@ -113,6 +113,24 @@ def test_residual_in_place():
         assert torch.equal(ops.linear_act_fwd(x, w, act='silu', residual=r, out=r), want)
 
 
+@pytest.mark.parametrize('dt', [BF, HF, F32])
+@pytest.mark.parametrize('M,N,K', [(70, 37, 51), (200, 136, 96), (4096, 64, 512)])
+def test_addend_of_the_input_gradient(dt, M, N, K):
+    """dx = dz w + dx_add is rounded once: an addend of the product's size costs one fp32 rounding more; in place too"""
+    from a2c_ppo_acktr import ops
+    from gated_refs import E32, EPS, TINY
+    x, w, dy, add = rnd(1, M, K, dtype=dt), rnd(2, N, K, scale=0.1, dtype=dt), rnd(3, M, N, dtype=dt), rnd(4, M, K, dtype=dt)
+    _, _, slope, ts = linear64(x, w)
+    (r, t), _, _ = linear_grads64(dy, x, w, slope, ts)
+    total = r + add.double()
+    t = t - EPS[dt] * r.abs() + (EPS[dt] + E32) * total.abs() + E32 * add.double().abs() + TINY[dt]
+    for need in (True, False):
+        dx, _, _ = ops.linear_act_bwd(dy, x, w, dx_add=add, need_dw=need, need_db=need)
+        check(dx, (total, t), 'dx')
+    again, _, _ = ops.linear_act_bwd(dy, x, w, dx_add=add, dx=add)
+    assert again.data_ptr() == add.data_ptr() and torch.equal(again, dx)
+
+
 def test_only_what_is_needed():
     from a2c_ppo_acktr import ops
     x, w, dy = rnd(1, 100, 72, dtype=BF), rnd(2, 40, 72, dtype=BF), rnd(3, 100, 40, dtype=BF)
