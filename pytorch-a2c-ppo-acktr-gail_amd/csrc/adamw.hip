@@ -18,16 +18,18 @@
 namespace acktr {
 
 constexpr int AW_THREADS = 256, AW_CHUNK = 2048, AW_BLOCK = 256, AW_PARTIALS = 1024;
+// up to this many chunks, the update's workgroups sum the norm's partial sums themselves
+constexpr int AW_SMALL = 1024;
+
+// what a step's update needs besides the elements
+struct AwScalars { float coef, keep, step_size, inv_bc2, b1, nb1, b2, nb2, eps; unsigned key; };
 
 // device copy of the optimiser's state that is not per element (acktr_adamw_state_bytes)
 struct AwState {
     double lr, b1, b2, eps, wd, max_norm;      // written by the host when they change
     long long step, seed;
-    // written by the first launch of a step for the second
-    float coef, keep, step_size, inv_bc2, b1f, nb1f, b2f, nb2f, epsf;
-    unsigned key;
+    AwScalars now;                             // of the present step
     unsigned done;                             // finished workgroups of the norm launch; back at 0 when it ends
-    float norm;
     double partial[AW_PARTIALS];
 };
 
@@ -37,41 +39,48 @@ __device__ __forceinline__ unsigned mix32(unsigned x) {
     return x ^ (x >> 16);
 }
 
-// scalars of the next step; one lane
-__device__ __forceinline__ void aw_begin(AwState* st, double sumsq, bool clip) {
+// min(1, c / (|g| + 1e-6)); a norm that is not a number stays one
+__device__ __forceinline__ float aw_coef(double sumsq, double max_norm) {
+    const double c = max_norm / (sqrt(sumsq) + 1e-6);
+    return (float)(c > 1.0 ? 1.0 : c);
+}
+// bc1 = 1 - b1^t, bc2 = 1 - b2^t
+__device__ __forceinline__ AwScalars aw_scalars(const AwState* st, long long t, float coef, double bc1, double bc2) {
+    AwScalars a;
+    a.coef = coef;
+    a.keep = (float)(1.0 - st->lr * st->wd);
+    a.step_size = (float)(st->lr / bc1);
+    a.inv_bc2 = (float)(1.0 / sqrt(bc2));
+    a.b1 = (float)st->b1;
+    a.nb1 = (float)(1.0 - st->b1);
+    a.b2 = (float)st->b2;
+    a.nb2 = (float)(1.0 - st->b2);
+    a.eps = (float)st->eps;
+    a.key = mix32((unsigned)st->seed + (unsigned)t * 0x9e3779b9u);
+    return a;
+}
+// counts the step and writes its scalars; one lane
+__device__ __forceinline__ void aw_begin(AwState* st, float coef) {
     const long long t = st->step + 1;
     st->step = t;
-    double c = 1.0;
-    if (clip) {
-        const double norm = sqrt(sumsq);
-        c = st->max_norm / (norm + 1e-6);
-        if (c > 1.0) c = 1.0;                  // (a norm that is not a number stays one)
-        st->norm = (float)norm;
-    }
-    st->coef = (float)c;
-    st->keep = (float)(1.0 - st->lr * st->wd);
-    st->step_size = (float)(st->lr / (1.0 - pow(st->b1, (double)t)));
-    st->inv_bc2 = (float)(1.0 / sqrt(1.0 - pow(st->b2, (double)t)));
-    st->b1f = (float)st->b1;
-    st->nb1f = (float)(1.0 - st->b1);
-    st->b2f = (float)st->b2;
-    st->nb2f = (float)(1.0 - st->b2);
-    st->epsf = (float)st->eps;
-    st->key = mix32((unsigned)st->seed + (unsigned)t * 0x9e3779b9u);
+    st->now = aw_scalars(st, t, coef, 1.0 - pow(st->b1, (double)t), 1.0 - pow(st->b2, (double)t));
 }
+
+// Pointers that come out of the table are to device memory; said so, they are not accessed through the slower generic path.
+#define ACKTR_GLB __attribute__((address_space(1)))
 
 // 4 consecutive values from element i of a tensor of n; nothing behind the end is touched
 template <class T>
 __device__ __forceinline__ f32v4 ld4_as(const void* p, long i, long n, bool vec) {
     f32v4 r = {0.f, 0.f, 0.f, 0.f};
     if (vec && i + 4 <= n) {
-        const vec_t<T, 4> v = *reinterpret_cast<const vec_t<T, 4>*>((const T*)p + i);
+        const vec_t<T, 4> v = *reinterpret_cast<const ACKTR_GLB vec_t<T, 4>*>((const ACKTR_GLB T*)p + i);
 #pragma unroll
         for (int k = 0; k < 4; ++k) r[k] = to_f32(v[k]);
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-            if (i + k < n) r[k] = to_f32(((const T*)p)[i + k]);
+            if (i + k < n) r[k] = to_f32(((const ACKTR_GLB T*)p)[i + k]);
     }
     return r;
 }
@@ -81,11 +90,11 @@ __device__ __forceinline__ void st4_as(void* p, long i, long n, bool vec, const 
         vec_t<T, 4> o;
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[k] = from_f32<T>(v[k]);
-        *reinterpret_cast<vec_t<T, 4>*>((T*)p + i) = o;
+        *reinterpret_cast<ACKTR_GLB vec_t<T, 4>*>((ACKTR_GLB T*)p + i) = o;
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-            if (i + k < n) ((T*)p)[i + k] = from_f32<T>(v[k]);
+            if (i + k < n) ((ACKTR_GLB T*)p)[i + k] = from_f32<T>(v[k]);
     }
 }
 __device__ __forceinline__ f32v4 ld4(const void* p, int dt, long i, long n, bool vec) {
@@ -97,40 +106,59 @@ __device__ __forceinline__ void st4(void* p, int dt, long i, long n, bool vec, c
     else st4_as<_Float16>(p, i, n, vec, v);
 }
 
+// Sum of squares of all gradients, in fp64.  SMALL: partial sums only (and the step is counted): the update's workgroups add them up.
+// Otherwise the last workgroup to finish adds them, in the same fixed order, and writes the step's scalars: thousands of workgroups
+// would read too much, while for a few hundred the chain of atomics costs more than the rest of the launch (13 us against 5 for the
+// 867 thousand parameters of the NatureCNN policy).
+template <bool SMALL>
 __global__ __launch_bounds__(AW_THREADS) void adamw_norm_kernel(AwState* st, const acktr_adamw_tensor* tensors, const int2* chunks, int nchunks) {
     __shared__ double sm[16];
     __shared__ bool last;
     double s = 0.0;
-    for (int q = blockIdx.x; q < nchunks; q += gridDim.x) {
-        const int2 ck = chunks[q];
-        const acktr_adamw_tensor t = tensors[ck.x];
-        const long base = (long)ck.y * AW_CHUNK;
+    constexpr int IT = AW_CHUNK / AW_THREADS / 4;
+    if (SMALL && blockIdx.x == 0 && threadIdx.x == 0) st->step = st->step + 1;
+    // two chunks at a time, and the table entries of the next two travel with their values
+    const int step = gridDim.x;
+    int q = blockIdx.x;
+    const int none = nchunks - 1;
+    int2 c0 = chunks[min(q, none)], c1 = chunks[min(q + step, none)];
+    acktr_adamw_tensor t0 = tensors[c0.x], t1 = tensors[c1.x];
+    while (q < nchunks) {
+        f32v4 g[2 * IT];
+        const bool two = q + step < nchunks;
 #pragma unroll
-        for (int k = 0; k < AW_CHUNK / AW_THREADS / 4; ++k) {
-            const long i = base + (k * AW_THREADS + threadIdx.x) * 4;
-            if (i >= t.n) break;
-            const f32v4 g = ld4(t.g, t.g_dtype, i, t.n, t.vec & 2);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s += (double)g[j] * (double)g[j];
+        for (int k = 0; k < IT; ++k) {
+            g[k] = ld4(t0.g, t0.g_dtype, (long)c0.y * AW_CHUNK + (k * AW_THREADS + threadIdx.x) * 4, t0.n, t0.vec & 2);
+            g[IT + k] = two ? ld4(t1.g, t1.g_dtype, (long)c1.y * AW_CHUNK + (k * AW_THREADS + threadIdx.x) * 4, t1.n, t1.vec & 2) : f32v4{0.f, 0.f, 0.f, 0.f};
         }
+        q += 2 * step;
+        c0 = chunks[min(q, none)], c1 = chunks[min(q + step, none)];
+        t0 = tensors[c0.x], t1 = tensors[c1.x];
+#pragma unroll
+        for (int k = 0; k < 2 * IT; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s += (double)g[k][j] * (double)g[k][j];
     }
     s = block_sum(s, sm);
+    if (SMALL) {
+        if (threadIdx.x == 0) st->partial[blockIdx.x] = s;
+        return;
+    }
     if (threadIdx.x == 0) {
         __hip_atomic_store(&st->partial[blockIdx.x], s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         last = __hip_atomic_fetch_add(&st->done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
     }
     __syncthreads();
     if (!last) return;
-    // the last workgroup to finish sums the partial sums, always in the same order
     double v = 0.0;
     for (int i = threadIdx.x; i < (int)gridDim.x; i += AW_THREADS) v += __hip_atomic_load(&st->partial[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     v = block_sum(v, sm);
     if (threadIdx.x == 0) {
-        aw_begin(st, v, true);
+        aw_begin(st, aw_coef(v, st->max_norm));
         st->done = 0;
     }
 }
-__global__ void adamw_begin_kernel(AwState* st) { aw_begin(st, 0.0, false); }
+__global__ void adamw_begin_kernel(AwState* st) { aw_begin(st, 1.f); }
 
 // magnitude of a code of `TOP` as largest exponent field, for a scale of 1
 template <int TOP>
@@ -160,15 +188,14 @@ __device__ __forceinline__ float wave_max(float v) {
     return v;
 }
 
-template <int BITS>
+// SMALL: the step's scalars are formed here from `parts` partial sums, beside the loads of the elements.
+template <int BITS, bool SMALL>
 __global__ __launch_bounds__(AW_THREADS) void adamw_update_kernel(const AwState* __restrict__ st, const acktr_adamw_tensor* __restrict__ tensors,
-                                                                  const int2* __restrict__ chunks, void* mom1, void* mom2, float* scales) {
+                                                                  const int2* __restrict__ chunks, void* mom1, void* mom2, float* scales,
+                                                                  int parts) {
     const int2 ck = chunks[blockIdx.x];
     const acktr_adamw_tensor t = tensors[ck.x];
     const long base = (long)ck.y * AW_CHUNK;
-    const float coef = st->coef, keep = st->keep, step_size = st->step_size, inv_bc2 = st->inv_bc2, epsf = st->epsf;
-    const float b1 = st->b1f, nb1 = st->nb1f, b2 = st->b2f, nb2 = st->nb2f;
-    const unsigned key = st->key;
     constexpr int IT = AW_CHUNK / AW_THREADS / 4;
     f32v4 pv[IT], gv[IT];
     f32v4 mv[IT], vv[IT];
@@ -191,6 +218,27 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_update_kernel(const AwState*
             vs[k] = scales[si / AW_BLOCK * 2 + 1];
         }
     }
+    AwScalars a;
+    if (SMALL) {
+        __shared__ double sh[3];
+        if (threadIdx.x < 64) {
+            double v[AW_SMALL / 64], total = 0.0;
+#pragma unroll
+            for (int j = 0; j < AW_SMALL / 64; ++j) v[j] = st->partial[threadIdx.x + 64 * j < parts ? threadIdx.x + 64 * j : 0];
+#pragma unroll
+            for (int j = 0; j < AW_SMALL / 64; ++j) total += (int)threadIdx.x + 64 * j < parts ? v[j] : 0.0;
+            total = wave_sum(total);
+            if (threadIdx.x == 0) sh[0] = total;
+        } else if (threadIdx.x == 64) {                      // (a wave each: a double pow takes as long as the sum)
+            sh[1] = 1.0 - pow(st->b1, (double)st->step);
+        } else if (threadIdx.x == 128) {
+            sh[2] = 1.0 - pow(st->b2, (double)st->step);
+        }
+        __syncthreads();
+        a = aw_scalars(st, st->step, aw_coef(sh[0], st->max_norm), sh[1], sh[2]);
+    } else {
+        a = st->now;
+    }
 #pragma unroll
     for (int k = 0; k < IT; ++k) {
         const long i = base + (k * AW_THREADS + threadIdx.x) * 4, si = t.state + i;
@@ -206,11 +254,11 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_update_kernel(const AwState*
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float g = gv[k][j] * coef;
-            const float m = mv[k][j] * b1 + g * nb1;
-            const float v = vv[k][j] * b2 + (g * g) * nb2;
-            const float denom = sqrtf(v) * inv_bc2 + epsf;
-            pv[k][j] = pv[k][j] * keep - (m / denom) * step_size;
+            const float g = gv[k][j] * a.coef;
+            const float m = mv[k][j] * a.b1 + g * a.nb1;
+            const float v = vv[k][j] * a.b2 + (g * g) * a.nb2;
+            const float denom = sqrtf(v) * a.inv_bc2 + a.eps;
+            pv[k][j] = pv[k][j] * a.keep - (m / denom) * a.step_size;
             mv[k][j] = m;
             vv[k][j] = v;
         }
@@ -238,13 +286,13 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_update_kernel(const AwState*
             unsigned ma = 0, va = 0;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const unsigned r = mix32((unsigned)(si + j) ^ key);
+                const unsigned r = mix32((unsigned)(si + j) ^ a.key);
                 const float y = mv[k][j] * im, z = vv[k][j] * iv;
-                unsigned a = code_of<15>(fabsf(y), r & 0xfffffu), b = code_of<31>(z, r >> 12);
-                if (y < 0.f) a += 128u;
-                if (b == 0 && z > 0.f) b = 1;
-                ma |= (bad ? 0u : a) << (8 * j);
-                va |= (bad ? 0u : b) << (8 * j);
+                unsigned cm = code_of<15>(fabsf(y), r & 0xfffffu), cv = code_of<31>(z, r >> 12);
+                if (y < 0.f) cm += 128u;
+                if (cv == 0 && z > 0.f) cv = 1;
+                ma |= (bad ? 0u : cm) << (8 * j);
+                va |= (bad ? 0u : cv) << (8 * j);
             }
             *reinterpret_cast<unsigned*>((uint8_t*)mom1 + si) = ma;
             *reinterpret_cast<unsigned*>((uint8_t*)mom2 + si) = va;
@@ -292,15 +340,21 @@ extern "C" int acktr_adamw_step(void* state, const acktr_adamw_tensor* tensors, 
               "adamw: buffers must be 16-byte aligned");
     hipStream_t s = (hipStream_t)stream;
     AwState* st = (AwState*)state;
-    if (clip && nchunks) {
-        adamw_norm_kernel<<<(int)min(nchunks, (long)AW_PARTIALS), AW_THREADS, 0, s>>>(st, tensors, (const int2*)chunks, (int)nchunks);
-    } else {
-        adamw_begin_kernel<<<1, 1, 0, s>>>(st);
-    }
+    const int2* table = (const int2*)chunks;
+    const int n = (int)nchunks;
+    const bool small = clip && n && n <= AW_SMALL;
+    if (small) adamw_norm_kernel<true><<<n, AW_THREADS, 0, s>>>(st, tensors, table, n);
+    else if (clip && n) adamw_norm_kernel<false><<<min(n, AW_PARTIALS), AW_THREADS, 0, s>>>(st, tensors, table, n);
+    else adamw_begin_kernel<<<1, 1, 0, s>>>(st);
     ACKTR_LAUNCH_CHECK();
-    if (!nchunks) return 0;
-    if (bits == 32) adamw_update_kernel<32><<<(int)nchunks, AW_THREADS, 0, s>>>(st, tensors, (const int2*)chunks, mom1, mom2, scales);
-    else adamw_update_kernel<8><<<(int)nchunks, AW_THREADS, 0, s>>>(st, tensors, (const int2*)chunks, mom1, mom2, scales);
+    if (!n) return 0;
+    if (bits == 32) {
+        if (small) adamw_update_kernel<32, true><<<n, AW_THREADS, 0, s>>>(st, tensors, table, mom1, mom2, scales, n);
+        else adamw_update_kernel<32, false><<<n, AW_THREADS, 0, s>>>(st, tensors, table, mom1, mom2, scales, 0);
+    } else {
+        if (small) adamw_update_kernel<8, true><<<n, AW_THREADS, 0, s>>>(st, tensors, table, mom1, mom2, scales, n);
+        else adamw_update_kernel<8, false><<<n, AW_THREADS, 0, s>>>(st, tensors, table, mom1, mom2, scales, 0);
+    }
     ACKTR_LAUNCH_CHECK();
     return 0;
 }
