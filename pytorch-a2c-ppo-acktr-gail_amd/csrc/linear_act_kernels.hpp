@@ -31,22 +31,15 @@ __device__ __forceinline__ void finish8(const LinArgs& p, int m, int n, float (&
     *reinterpret_cast<vec_t<T, 8>*>((T*)p.y + (long)m * p.ldy + n) = y;
     if (SLOPE) *reinterpret_cast<vec_t<ST, 8>*>((ST*)p.pre + (long)m * p.ldp + n) = z;
 }
-// the same value by value, for widths and rows of any alignment
+// one value, for widths and rows of any alignment; b, r: bias and residual as above
 template <class T, int ACT, bool SLOPE>
-__device__ __forceinline__ void finish8_any(const LinArgs& p, int m, int n, float (&v)[8]) {
+__device__ __forceinline__ void finish1(const LinArgs& p, int m, int n, float v, float b, T r, bool res) {
     typedef typename SlopeOf<T>::type ST;
-#pragma unroll 1
-    for (int i = 0; i < 8; ++i) {
-        if (n + i >= p.N) break;
-        float z = v[0], slope;
-        if (p.bias) z += to_f32(((const T*)p.bias)[n + i]);
-        float o = act_of<ACT, SLOPE>(z, slope);
-        if (p.res) o += to_f32(((const T*)p.res)[(long)m * p.ldr + n + i]);
-        ((T*)p.y)[(long)m * p.ldy + n + i] = from_f32<T>(o);
-        if (SLOPE) put_slope(((ST*)p.pre)[(long)m * p.ldp + n + i], slope);
-#pragma unroll
-        for (int j = 0; j < 7; ++j) v[j] = v[j + 1];         // (the registers rotate: they have no address)
-    }
+    float slope;
+    float o = act_of<ACT, SLOPE>(v + b, slope);
+    if (res) o += to_f32(r);
+    ((T*)p.y)[(long)m * p.ldy + n] = from_f32<T>(o);
+    if (SLOPE) put_slope(((ST*)p.pre)[(long)m * p.ldp + n], slope);
 }
 // f(activation code, whether slopes are wanted) as compile-time constants
 template <class F>
@@ -132,7 +125,43 @@ __device__ __forceinline__ void linear_tile(const LinArgs& p, int id, int slice,
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = lo[i], v[4 + i] = hi[i];
     };
-    if (p.slabs || !p.vec) {
+    // rows or widths that do not allow 8 columns at a time: a column a lane, so that a row's stores still lie side by side, eight rows
+    // in flight
+    constexpr int LA = WTN < 64 ? WTN : 64, RP1 = 64 / LA, CG = WTN / LA, U = 8;
+    static_assert(P * 16 / RP1 % U == 0, "whole groups of rows");
+    auto finish_any = [&](auto act, auto slope, auto slab) __attribute__((always_inline)) {
+        constexpr int ACT = decltype(act)::value;
+        constexpr bool SLOPE = decltype(slope)::value, SLAB = decltype(slab)::value;
+        const bool res = !SLAB && p.res;
+#pragma unroll 1
+        for (int base = 0; base < G::MI; base += P) {
+            spill(base);
+#pragma unroll 1
+            for (int k = 0; k < CG * (P * 16 / RP1 / U); ++k) {
+                const int c = (k % CG) * LA + lane % LA, r0 = (k / CG) * U * RP1 + lane / LA, nn = wn + c;
+                const bool in = nn < p.N;
+                const float b = !SLAB && FULL && p.bias && in ? to_f32(((const T*)p.bias)[nn]) : 0.f;
+                float v[U];
+                T rr[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int r = r0 + u * RP1, m = wm + base * 16 + r;
+                    v[u] = mine[r * PITCH + c];
+                    rr[u] = res && in && m < p.M ? ((const T*)p.res)[(long)m * p.ldr + nn] : (T)0.f;
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int m = wm + base * 16 + r0 + u * RP1;
+                    if (!in || m >= p.M) continue;
+                    if (SLAB) p.slabs[((long)slice * p.M + m) * p.N + nn] = v[u];
+                    else finish1<T, ACT, SLOPE>(p, m, nn, v[u], b, rr[u], res);
+                }
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+    };
+    using std::integral_constant;
+    if (p.slabs && p.vec) {
 #pragma unroll 1
         for (int base = 0; base < G::MI; base += P) {
             spill(base);
@@ -142,24 +171,19 @@ __device__ __forceinline__ void linear_tile(const LinArgs& p, int id, int slice,
                 float v[8];
                 fetch8(k, v);
                 if (m >= p.M || n >= p.N) continue;
-                if (p.slabs) {
-                    float* s = p.slabs + ((long)slice * p.M + m) * p.N + n;
-                    if (p.vec) {
-                        *reinterpret_cast<f32v4*>(s) = f32v4{v[0], v[1], v[2], v[3]};
-                        *reinterpret_cast<f32v4*>(s + 4) = f32v4{v[4], v[5], v[6], v[7]};
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (n + i < p.N) s[i] = v[i];
-                    }
-                } else if constexpr (FULL) {
-                    with_act(p, [&](auto act, auto slope) { finish8_any<T, decltype(act)::value, decltype(slope)::value>(p, m, n, v); });
-                } else {
-                    finish8_any<T, ACKTR_ACT_NONE, false>(p, m, n, v);
-                }
+                float* s = p.slabs + ((long)slice * p.M + m) * p.N + n;
+                *reinterpret_cast<f32v4*>(s) = f32v4{v[0], v[1], v[2], v[3]};
+                *reinterpret_cast<f32v4*>(s + 4) = f32v4{v[4], v[5], v[6], v[7]};
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
+        return;
+    }
+    if (p.slabs) return finish_any(integral_constant<int, ACKTR_ACT_NONE>{}, std::false_type{}, std::true_type{});
+    if (!p.vec) {
+        auto apart = [&](auto act, auto slope) __attribute__((always_inline)) { finish_any(act, slope, std::false_type{}); };
+        if constexpr (FULL) with_act(p, apart);
+        else apart(integral_constant<int, ACKTR_ACT_NONE>{}, std::false_type{});
         return;
     }
     auto finish = [&](auto act, auto slope) __attribute__((always_inline)) {
@@ -219,32 +243,37 @@ __global__ __launch_bounds__(256, 2) void linear_pair_kernel(const LinArgs dw, c
     else linear_tile<T, true, false, BM, BN, 2, 2, STAGES, false>(dx, id - dw_groups, 0, (ACKTR_LDS char*)smem);
 }
 
-// Sum of the slices of a split reduction in slice order, then the epilogue.
-template <class T>
+// Sum of the slices of a split reduction in slice order, then the epilogue.  V: columns a thread, 8 where rows allow it, else 1.
+template <class T, int V>
 __global__ __launch_bounds__(256) void linear_slabs_kernel(const LinArgs p, int slices) {
-    const int groups = (p.N + 7) / 8;
-    const long total = (long)p.M * groups;
+    const int groups = p.N / V;
+    const long total = (long)p.M * groups, plane = (long)p.M * p.N;
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
-        const int m = (int)(i / groups), n = (int)(i % groups) * 8;
+        const int m = (int)(i / groups), n = (int)(i % groups) * V;
         const float* s = p.slabs + (long)m * p.N + n;
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        for (int z = 0; z < slices; ++z, s += (long)p.M * p.N) {
-            if (p.vec) {
-                const f32v4 lo = *reinterpret_cast<const f32v4*>(s), hi = *reinterpret_cast<const f32v4*>(s + 4);
+        float v[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = 0.f;
+#pragma unroll 4
+        for (int z = 0; z < slices; ++z) {
+            if constexpr (V == 8) {
+                const f32v4 lo = *reinterpret_cast<const f32v4*>(s + z * plane), hi = *reinterpret_cast<const f32v4*>(s + z * plane + 4);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[j] += lo[j], v[4 + j] += hi[j];
             } else {
-                for (int j = 0; j < 8 && n + j < p.N; ++j) v[j] += s[j];
+                v[0] += s[z * plane];
             }
         }
-        if (p.vec) {
+        if constexpr (V == 8) {
             float b[8];
             load_bias8<T>(p, n, b);
             vec_t<T, 8> r;
             if (p.res) r = *reinterpret_cast<const vec_t<T, 8>*>((const T*)p.res + (long)m * p.ldr + n);
             with_act(p, [&](auto act, auto slope) { finish8<T, decltype(act)::value, decltype(slope)::value>(p, m, n, v, b, r, p.res); });
         } else {
-            with_act(p, [&](auto act, auto slope) { finish8_any<T, decltype(act)::value, decltype(slope)::value>(p, m, n, v); });
+            const float b = p.bias ? to_f32(((const T*)p.bias)[n]) : 0.f;
+            const T r = p.res ? ((const T*)p.res)[(long)m * p.ldr + n] : (T)0.f;
+            with_act(p, [&](auto act, auto slope) { finish1<T, decltype(act)::value, decltype(slope)::value>(p, m, n, v[0], b, r, p.res); });
         }
     }
 }
@@ -278,7 +307,8 @@ static int launch_tile(LinArgs& p, const Plan& pl, hipStream_t s) {
 
 template <class T>
 static int sum_slices(const LinArgs& p, int slices, hipStream_t s) {
-    linear_slabs_kernel<T><<<min(cdiv((long)p.M * ((p.N + 7) / 8), 256), 2048), 256, 0, s>>>(p, slices);
+    if (p.vec) linear_slabs_kernel<T, 8><<<min(cdiv((long)p.M * (p.N / 8), 256), 2048), 256, 0, s>>>(p, slices);
+    else linear_slabs_kernel<T, 1><<<min(cdiv((long)p.M * p.N, 256), 4096), 256, 0, s>>>(p, slices);
     ACKTR_LAUNCH_CHECK();
     return 0;
 }
