@@ -475,14 +475,17 @@ class _on(object):
         return False
 
 
-def _launch(fn, args, index, what, work):
+_current_device = getattr(torch._C, '_cuda_getDevice', torch.cuda.current_device)
+_current_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _launch(fn, index, what, work, *args):
     """fn(*args, stream) on device `index`, timed when the profiler is on."""
-    stream = _hip.cur_stream(index)
-    if profiler is None and index == torch.cuda.current_device():
-        rc = fn(*args, stream)
+    if profiler is None and index == _current_device():
+        rc = fn(*args, _current_stream(index))
     else:
         with _on(index), _Timed(what, work):
-            rc = fn(*args, stream)
+            rc = fn(*args, _current_stream(index))
     if rc:
         _hip.check(rc, 'acktr_' + what)
 
@@ -525,17 +528,19 @@ def _dense(t, name, shape, dtype, index):
 
 
 def _dtype_code(t, name):
-    if not isinstance(t, torch.Tensor) or t.dtype not in DTYPE_CODE:
+    code = DTYPE_CODE.get(getattr(t, 'dtype', None))
+    if code is None:
         raise RuntimeError('%s must be a bfloat16, float16 or float32 tensor (got %s)' % (name, getattr(t, 'dtype', type(t))))
     if not t.is_cuda:
         raise RuntimeError('%s must live on the MI355X device (got %s): this package has no CPU path' % (name, t.device))
-    return DTYPE_CODE[t.dtype]
+    return code
 
 
 def _act_code(act):
-    if act not in LINEAR_ACT:
+    code = LINEAR_ACT.get(act)
+    if code is None:
         raise RuntimeError('unknown activation %r (one of none, relu, tanh, silu, gelu)' % (act,))
-    return LINEAR_ACT[act]
+    return code
 
 
 def _reach(t):
@@ -545,12 +550,9 @@ def _reach(t):
     p = t.data_ptr()
     if t.is_contiguous():
         return p, p + t.nbytes
-    reach = 1
-    for n, s in zip(t.shape, t.stride()):
-        if n == 0:
-            return 0, 0
-        reach += (n - 1) * s
-    return p, p + reach * t.element_size()
+    if t.numel() == 0:
+        return 0, 0
+    return p, p + (1 + sum([(n - 1) * s for n, s in zip(t.shape, t.stride())])) * t.element_size()
 
 
 def _apart(out, name, others, what):
@@ -563,7 +565,7 @@ def _apart(out, name, others, what):
             reach += s * (n - 1)
     a0, a1 = _reach(out)
     for t in others:
-        if t is None:
+        if t is None or t.data_ptr() >= a1:
             continue
         b0, b1 = _reach(t)
         if a0 < b1 and b0 < a1 and not _side_by_side(out, a0, t, b0):
@@ -593,15 +595,16 @@ def linear_act_fwd(x, w, bias=None, act=None, residual=None, out=None, pre=None)
     fp32), sums in fp32, rounded once.  act: None, 'relu', 'tanh', 'silu' or 'gelu'.  pre [M, N]: receives
     what linear_act_bwd needs of the pre-activations (the activation's slopes, encoded).  out may be `residual` itself."""
     code, act = _dtype_code(x, 'x'), _act_code(act)
-    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1] or x.shape[1] < 1 or w.shape[0] < 1:
-        raise RuntimeError('linear_act_fwd: x [M, K] and w [N, K] expected, got %s and %s' % (tuple(x.shape), tuple(w.shape)))
-    (M, K), N, dt, at = x.shape, w.shape[0], x.dtype, x.get_device()
+    mk, nk = x.shape, w.shape
+    if len(mk) != 2 or len(nk) != 2 or mk[1] != nk[1] or mk[1] < 1 or nk[0] < 1:
+        raise RuntimeError('linear_act_fwd: x [M, K] and w [N, K] expected, got %s and %s' % (tuple(mk), tuple(nk)))
+    (M, K), N, dt, at = mk, nk[0], x.dtype, x.get_device()
     mn = (M, N)
     given = out is not None
     if not given:
         out = x.new_empty(mn)
-    px, ldx = _rows(x, 'x', (M, K), dt, at)
-    pw, ldw = _rows(w, 'w', (N, K), dt, at)
+    px, ldx = _rows(x, 'x', mk, dt, at)
+    pw, ldw = _rows(w, 'w', nk, dt, at)
     py, ldy = _rows(out, 'out', mn, dt, at)
     pb = _vec(bias, 'bias', N, dt, at) if bias is not None else None
     pr, ldr = _rows(residual, 'residual', mn, dt, at) if residual is not None else (None, 0)
@@ -614,8 +617,8 @@ def linear_act_fwd(x, w, bias=None, act=None, residual=None, out=None, pre=None)
     L = _hip.lib()
     nb = L.acktr_linear_act_fwd_workspace_bytes(px, ldx, pw, ldw, M, N, K, code)
     ws = _scratch(nb, x, 'acktr_linear_act_fwd') if nb else None
-    _launch(L.acktr_linear_act_fwd, (px, ldx, pw, ldw, pb, pr, ldr, py, ldy, pz, ldz, M, N, K, code, act, ws.data_ptr() if nb else None, nb),
-            at, 'linear_act_fwd', 2.0 * M * N * K)
+    _launch(L.acktr_linear_act_fwd, at, 'linear_act_fwd', 2.0 * M * N * K, px, ldx, pw, ldw, pb, pr, ldr, py, ldy, pz, ldz, M, N, K, code,
+            act, ws.data_ptr() if nb else None, nb)
     return out
 
 
@@ -655,8 +658,8 @@ def linear_act_bwd(dy, x, w, pre=None, act=None, dx=None, dw=None, db=None, need
     L = _hip.lib()
     nb = L.acktr_linear_act_bwd_workspace_bytes(pg, ldg, px, ldx, pw, ldw, pz, ldz, need_dx, need_dw, need_db, M, N, K, code, act)
     ws = _scratch(nb, dy, 'acktr_linear_act_bwd') if nb else None
-    _launch(L.acktr_linear_act_bwd, (pg, ldg, px, ldx, pw, ldw, pz, ldz, pa, lda, qx, ldq, qw, qb, M, N, K, code, act, ws.data_ptr() if nb else None, nb),
-            at, 'linear_act_bwd', 2.0 * M * N * K * (bool(need_dx) + bool(need_dw)))
+    _launch(L.acktr_linear_act_bwd, at, 'linear_act_bwd', 2.0 * M * N * K * (bool(need_dx) + bool(need_dw)), pg, ldg, px, ldx, pw, ldw, pz, ldz,
+            pa, lda, qx, ldq, qw, qb, M, N, K, code, act, ws.data_ptr() if nb else None, nb)
     return dx if need_dx else None, dw if need_dw else None, db if need_db else None
 
 
@@ -669,6 +672,27 @@ def _steps(t, name, shape, dtype, index):
     if inner != 1 and H > 1:
         _refuse(t, name, shape, dtype, index)
     return t.data_ptr(), (st if T > 1 else N * H), (sn if N > 1 else H)
+
+
+def _span3(q, shape, e):
+    """[first byte, last byte + 1) of a [T, N, H] operand (pointer, strides) of e-byte elements"""
+    p, st, sn = q
+    T, N, H = shape
+    return p, (p + ((T - 1) * st + (N - 1) * sn + H) * e if T and N else p)
+
+
+def _steps_apart(t, name, q, shape, e, spans, others, what):
+    """_apart for a [T, N, H] operand that is written: by its strides and the others' spans where those settle it"""
+    _, st, sn = q
+    T, N, H = shape
+    lo, hi = _span3(q, shape, e)
+    if (sn >= H and st >= (N - 1) * sn + H) or (st >= H and sn >= (T - 1) * st + H):
+        for a, b in spans:
+            if a < hi and lo < b:
+                break
+        else:
+            return
+    _apart(t, name, others, what)
 
 
 def _masks(masks, shape, index):
@@ -707,14 +731,16 @@ def gated_scan_fwd(gate, value, h0=None, masks=None, out=None, save=False):
     ph = _dense(h0, 'h0', (N, H), f32, at) if h0 is not None else None
     pm = _masks(masks, (T, N), at)
     if given:
-        _apart(out, 'out', (gate, value, h0, masks), 'gated_scan_fwd')
+        e, c = out.element_size(), 4 * N * H
+        spans = (_span3(pg, shape, e), _span3(pv, shape, e), (ph or 0, ph + c if ph else 0), (pm or 0, pm + 4 * T * N if pm else 0))
+        _steps_apart(out, 'out', po, shape, e, spans, (gate, value, h0, masks), 'gated_scan_fwd')
     L = _hip.lib()
     last = gate.new_empty((N, H), dtype=f32)
     saved = gate.new_empty((-(-T // _scan_interval()), N, H), dtype=f32) if save else None
     nb = L.acktr_gated_scan_workspace_bytes(T, N, H, code)
     ws = _scratch(nb, gate, 'acktr_gated_scan_fwd') if nb else None
-    _launch(L.acktr_gated_scan_fwd, (*pg, *pv, ph, pm, *po, last.data_ptr(), saved.data_ptr() if save else None, T, N, H, code,
-                                     ws.data_ptr() if nb else None, nb), at, 'gated_scan_fwd', 10.0 * T * N * H)
+    _launch(L.acktr_gated_scan_fwd, at, 'gated_scan_fwd', 10.0 * T * N * H, *pg, *pv, ph, pm, *po, last.data_ptr(),
+            saved.data_ptr() if save else None, T, N, H, code, ws.data_ptr() if nb else None, nb)
     return out, last, saved
 
 
@@ -739,13 +765,20 @@ def gated_scan_bwd(dout, gate, value, h0=None, masks=None, saved=None, dlast=Non
     pl = _dense(dlast, 'dlast', (N, H), f32, at) if dlast is not None else None
     if T > every and saved is None:
         raise RuntimeError('gated_scan_bwd: more than %d steps need what gated_scan_fwd(save=True) saved' % every)
-    for i, a in enumerate(given):
-        _apart(a, 'a gradient', (dout, gate, value, h0, masks, saved, dlast) + tuple(given[:i]), 'gated_scan_bwd')
+    if given:
+        e, c = gate.element_size(), 4 * N * H
+        spans = [_span3(pd, shape, e), _span3(pg, shape, e), _span3(pv, shape, e), (ph or 0, ph + c if ph else 0), (pm or 0, pm + 4 * T * N if pm else 0),
+                 (ps or 0, ps + -(-T // every) * c if ps else 0), (pl or 0, pl + c if pl else 0)]
+        reads = (dout, gate, value, h0, masks, saved, dlast)
+        for a in given:
+            _steps_apart(a, 'a gradient', qg if a is dgate else qv, shape, e, spans, reads, 'gated_scan_bwd')
+        if len(given) == 2:
+            _apart(dgate, 'dgate', (dvalue,), 'gated_scan_bwd')
     dh0 = gate.new_empty((N, H), dtype=f32) if need_dh0 else None
     nb = L.acktr_gated_scan_workspace_bytes(T, N, H, code)
     ws = _scratch(nb, gate, 'acktr_gated_scan_bwd') if nb else None
-    _launch(L.acktr_gated_scan_bwd, (*pd, *pg, *pv, ph, pm, ps, pl, *qg, *qv, dh0.data_ptr() if need_dh0 else None, T, N, H, code,
-                                     ws.data_ptr() if nb else None, nb), at, 'gated_scan_bwd', 20.0 * T * N * H)
+    _launch(L.acktr_gated_scan_bwd, at, 'gated_scan_bwd', 20.0 * T * N * H, *pd, *pg, *pv, ph, pm, ps, pl, *qg, *qv,
+            dh0.data_ptr() if need_dh0 else None, T, N, H, code, ws.data_ptr() if nb else None, nb)
     return dgate, dvalue, dh0
 
 
@@ -765,6 +798,8 @@ def gated_scan_step(gate, value, state, masks=None, out=None):
     pm = _masks(masks, (N,), at)
     if given:
         _apart(out, 'out', (gate, value, state, masks), 'gated_scan_step')
-    _apart(state, 'state', (gate, value, masks), 'gated_scan_step')
-    _launch(_hip.lib().acktr_gated_scan_step, (pg, gn, pv, vn, ps, pm, po, on, N, H, code), at, 'gated_scan_step', 10.0 * N * H)
+    lo, hi = ps, ps + 4 * N * H
+    if lo <= pg < hi or lo <= pv < hi or pg <= lo < pg + gn * N * 4 or pv <= lo < pv + vn * N * 4 or (pm and lo - 4 * N < pm < hi):
+        _apart(state, 'state', (gate, value, masks), 'gated_scan_step')
+    _launch(_hip.lib().acktr_gated_scan_step, at, 'gated_scan_step', 10.0 * N * H, pg, gn, pv, vn, ps, pm, po, on, N, H, code)
     return out
