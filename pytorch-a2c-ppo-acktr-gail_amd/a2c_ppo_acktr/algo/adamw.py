@@ -68,6 +68,7 @@ class AdamW(object):
         self.mom1 = torch.zeros(off, dtype=dt, device=dev)
         self.mom2 = torch.zeros(off, dtype=dt, device=dev)
         self.scales = torch.zeros(2 * off // block, dtype=f32, device=dev) if self.state_bits == 8 else None
+        self._tensors = torch.zeros(len(self.params) * ctypes.sizeof(_hip.AdamwTensor), dtype=torch.uint8, device=dev)
         words = -(-L.acktr_adamw_state_bytes() // 8)
         self._state = torch.zeros(words, dtype=torch.float64, device=dev)
         self._state[6:8].view(torch.int64).copy_(torch.tensor([self.step_count, self.seed]))
@@ -122,8 +123,8 @@ class AdamW(object):
             raise RuntimeError('AdamW: two of the tensors to be written overlap (the same parameter twice?)')
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError('AdamW: the tensors changed since the last step; run prepare() before the capture')
-        host = torch.frombuffer(bytearray(bytes(rows)), dtype=torch.uint8)
-        self._tensors = host.to(dev)
+        # (into the same memory: a captured step reads the table there)
+        self._tensors.copy_(torch.frombuffer(bytearray(bytes(rows)), dtype=torch.uint8))
         self._seen = seen
 
     def prepare(self):

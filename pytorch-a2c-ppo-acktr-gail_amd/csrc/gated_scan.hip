@@ -550,6 +550,7 @@ extern "C" int acktr_gated_scan_fwd(const void* gate, long gt, long gn, const vo
     }
     const int e = (int)elem_bytes(dtype);
     ACKTR_ARG(gate && value && out, "gated_scan_fwd: gate, value and out are required");
+    ACKTR_ARG(gt >= 0 && gn >= 0 && vt >= 0 && vn >= 0 && ot >= 0 && on >= 0, "gated_scan_fwd: negative stride");
     const bool far = is_far(gt, gn, N, H, e) || is_far(vt, vn, N, H, e) || is_far(ot, on, N, H, e);
     const bool pair = !far && H % 2 == 0 && in_pairs(gate, gt, gn, e) && in_pairs(value, vt, vn, e) && in_pairs(out, ot, on, e);
     ACKTR_ARG(workspace_bytes >= acktr_gated_scan_workspace_bytes(T, N, H, dtype), "gated_scan_fwd: workspace of %ld bytes is too small",
@@ -578,6 +579,8 @@ extern "C" int acktr_gated_scan_bwd(const void* dout, long dt, long dn, const vo
     }
     const int e = (int)elem_bytes(dtype);
     ACKTR_ARG(dout && gate && value && dgate && dvalue, "gated_scan_bwd: dout, gate, value, dgate and dvalue are required");
+    ACKTR_ARG(dt >= 0 && dn >= 0 && gt >= 0 && gn >= 0 && vt >= 0 && vn >= 0 && dgt >= 0 && dgn >= 0 && dvt >= 0 && dvn >= 0,
+              "gated_scan_bwd: negative stride");
     const bool far = is_far(gt, gn, N, H, e) || is_far(vt, vn, N, H, e) || is_far(dt, dn, N, H, e) || is_far(dgt, dgn, N, H, e) || is_far(dvt, dvn, N, H, e);
     const bool pair = !far && H % 2 == 0 && in_pairs(dout, dt, dn, e) && in_pairs(gate, gt, gn, e) && in_pairs(value, vt, vn, e) &&
                       in_pairs(dgate, dgt, dgn, e) && in_pairs(dvalue, dvt, dvn, e);
@@ -598,6 +601,7 @@ extern "C" int acktr_gated_scan_step(const void* gate, long gn, const void* valu
     if (int rc = scan_check(1, N, H, dtype)) return rc;
     if (N * H == 0) return 0;
     ACKTR_ARG(gate && value && state && out, "gated_scan_step: gate, value, state and out are required");
+    ACKTR_ARG(gn >= 0 && vn >= 0 && on >= 0, "gated_scan_step: negative stride");
     hipStream_t s = (hipStream_t)stream;
     return with_dtype(dtype, [&](auto t) -> int {
         typedef decltype(t) T;

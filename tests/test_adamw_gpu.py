@@ -308,6 +308,27 @@ def test_captured_and_replayed(bits, clip):
     assert all(torch.equal(a, b) for a, b in zip(*runs))
 
 
+def test_a_captured_step_follows_the_table():
+    """gradients that were replaced by an eager step are what a step captured before reads afterwards; nothing points to freed memory"""
+    from a2c_ppo_acktr import algo, ops
+    p = rnd(1, 500).requires_grad_()
+    p.grad = rnd(2, 500)
+    opt = algo.AdamW([p.detach()], grads=None, copies=[None], **HP)
+    opt.params[0].grad = p.grad
+    opt.step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with ops.graph_capture(g):
+        opt.step()
+    opt.params[0].grad = rnd(3, 500)                         # another tensor
+    opt.step()
+    want = algo.AdamW([p.detach().clone()], grads=[opt.params[0].grad.clone()], **HP)
+    want.load_state_dict(opt.state_dict())
+    g.replay()
+    want.step()
+    assert torch.equal(want.params[0], opt.params[0]) and opt.steps_done() == 3
+
+
 def test_refusals():
     from a2c_ppo_acktr import algo
     p, g = rnd(1, 100), rnd(2, 100)

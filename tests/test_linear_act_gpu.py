@@ -68,6 +68,13 @@ def test_larger(dt, M, N, K):
     run(M, N, K, dt, 'gelu')
 
 
+@pytest.mark.parametrize('dt', [BF, HF])
+@pytest.mark.parametrize('M,N,K', [(8190, 4090, 264), (8190, 136, 4088), (300, 4088, 4090), (8192, 4096, 128)])
+def test_largest_tiles_with_ragged_edges(dt, M, N, K):
+    """forward, input gradient and weight gradient, in turn, fill two or one rounds of 256 x 256 tiles, with cut edges"""
+    run(M, N, K, dt, 'silu')
+
+
 def test_large_pre_activations():
     """tails of every activation: values far from zero"""
     for act in ACTS:
