@@ -79,24 +79,6 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(const T* __restrict__ dy, 
         sums[(long)blockIdx.y * N + col] = t;
     }
 }
-// db = sum of the row blocks' sums, 32 partial sums a column (each over every 32nd block), in fixed order
-template <class T>
-__global__ __launch_bounds__(1024) void col_sums_kernel(const float* __restrict__ sums, int blocks, int N, T* __restrict__ db) {
-    __shared__ float part[32][33];
-    const int c = threadIdx.x & 31, j = threadIdx.x >> 5, col = blockIdx.x * 32 + c;
-    float t = 0.f;
-    if (col < N) {
-#pragma unroll 8
-        for (int b = j; b < blocks; b += 32) t += sums[(long)b * N + col];
-    }
-    part[j][c] = t;
-    __syncthreads();
-    // column j: the 32 partial sums of a half wave, added pairwise
-    t = part[c][j];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor(t, o, 32);
-    if (c == 0 && blockIdx.x * 32 + j < N) db[blockIdx.x * 32 + j] = from_f32<T>(t);
-}
 // packs the jobs that have rows
 template <class T>
 static int pack(std::initializer_list<PackJob> list, hipStream_t s) {
@@ -127,7 +109,7 @@ static int check_ld(const char* what, long ld, long cols) {
     return 0;
 }
 
-static constexpr int V_OF(int e) { return 16 / e; }
+static constexpr int per16(int e) { return 16 / e; }
 
 }  // namespace acktr
 
@@ -137,8 +119,8 @@ using namespace acktr;
 struct FwdSpace { bool px, pw; long x, w, slabs, bytes; };
 static FwdSpace fwd_space(const void* x, long ldx, const void* w, long ldw, long M, long N, long K, int e) {
     FwdSpace f;
-    const bool whole = K % V_OF(e) == 0;
-    const long kp = up(K, V_OF(e));
+    const bool whole = K % per16(e) == 0;
+    const long kp = up(K, per16(e));
     f.px = !whole || !rows16(x, ldx, e);
     f.pw = !whole || !rows16(w, ldw, e);
     f.x = 0;
@@ -151,7 +133,7 @@ struct BwdSpace { bool aligned, pdy, px, pw; long dz, x, w, sums, slabs, bytes; 
 static BwdSpace bwd_space(const void* dy, long lddy, const void* x, long ldx, const void* w, long ldw, const void* pre, long ldp, bool dx, bool dw,
                           bool db, long M, long N, long K, int e, int act) {
     BwdSpace f;
-    const int V = V_OF(e);
+    const int V = per16(e);
     const long np = up(N, V), kp = up(K, V);
     f.aligned = N % V == 0 && rows16(dy, lddy, e) && (act == ACKTR_ACT_NONE || rows16(pre, ldp, e));
     f.pdy = act == ACKTR_ACT_NONE && (dx || dw) && (N % V != 0 || !rows16(dy, lddy, e));
@@ -200,7 +182,7 @@ extern "C" int acktr_linear_act_fwd(const void* x, long ldx, const void* w, long
         p.vec = N % 8 == 0 && rows16(y, ldy, e) && (!bias || ((uintptr_t)bias & 15) == 0) && (!residual || rows16(residual, ldr, e)) &&
                 (!pre || rows16(pre, ldp, e));
         char* ws = (char*)workspace;
-        const int kp = (int)up(K, V_OF(e));
+        const int kp = (int)up(K, per16(e));
         if (int rc = pack<T>({{x, ldx, sp.px ? (int)M : 0, (int)K, ws + sp.x, kp}, {w, ldw, sp.pw ? (int)N : 0, (int)K, ws + sp.w, kp}}, s)) return rc;
         if (sp.px) p.a = ws + sp.x, p.lda = kp;
         if (sp.pw) p.b = ws + sp.w, p.ldb = kp;
@@ -233,12 +215,14 @@ extern "C" int acktr_linear_act_bwd(const void* dy, long lddy, const void* x, lo
     hipStream_t s = (hipStream_t)stream;
     return with_dtype(dtype, [&](auto t) -> int {
         typedef decltype(t) T;
-        constexpr int e = sizeof(T), V = V_OF(e);
+        constexpr int e = sizeof(T), V = per16(e);
         const int np = (int)up(N, V), kp = (int)up(K, V);
         char* ws = (char*)workspace;
         T *dz_ws = (T*)(ws + sp.dz), *x_ws = (T*)(ws + sp.x), *w_ws = (T*)(ws + sp.w);
         float *sums = (float*)(ws + sp.sums), *slabs = (float*)(ws + sp.slabs);
 
+        LinArgs px{}, pw{};
+        int blocks = 0;
         // dz and the column sums.  Rows of dy (or pre) that do not start at 16 bytes, or end inside 16, are taken value by value;
         // dz itself is written into aligned rows, which the two products read.
         const void* dz = dy;
@@ -260,26 +244,22 @@ extern "C" int acktr_linear_act_bwd(const void* dy, long lddy, const void* x, lo
             else if (sp.aligned) launch(std::false_type{}, integral_constant<int, V>{});
             else launch(std::false_type{}, integral_constant<int, 1>{});
             ACKTR_LAUNCH_CHECK();
-            if (db) {
-                col_sums_kernel<T><<<cdiv(N, 32), 1024, 0, s>>>(sums, gy, (int)N, (T*)db);
-                ACKTR_LAUNCH_CHECK();
-            }
-        } else if (db) {                                     // no rows: the gradient of the bias is zero
-            col_sums_kernel<T><<<cdiv(N, 32), 1024, 0, s>>>(sums, 0, (int)N, (T*)db);
-            ACKTR_LAUNCH_CHECK();
+            blocks = gy;
         }
+        pw.M = (int)N, pw.N = (int)K, pw.K = (int)M;
+        pw.sums = sums, pw.blocks = blocks, pw.db = db;
+        if (db && !dw)                                       // no weight gradient's launch for it to ride in
+            if (int rc = linear_bias<T>(pw, s)) return rc;
         if (M > 0 && sp.pdy) {                               // no activation: dy itself, in aligned rows
             if (int rc = pack<T>({{dy, lddy, (int)M, (int)N, dz_ws, np}}, s)) return rc;
             dz = dz_ws, lddz = np;
         }
         if (int rc = pack<T>({{x, ldx, sp.px ? (int)M : 0, (int)K, x_ws, kp}, {w, ldw, sp.pw && M > 0 ? (int)N : 0, (int)K, w_ws, kp}}, s)) return rc;
-        LinArgs px{}, pw{};
         px.a = dz, px.lda = lddz, px.b = sp.pw ? w_ws : w, px.ldb = sp.pw ? kp : ldw;      // dx[M, K] = dz[M, N] w[N, K]: sum over N
         px.M = (int)M, px.N = (int)K, px.K = (int)N;
         px.y = dx, px.ldy = lddx, px.res = dx_add, px.ldr = ldxa;
         px.vec = K % 8 == 0 && rows16(dx, lddx, e) && (!dx_add || rows16(dx_add, ldxa, e));
         pw.a = dz, pw.lda = lddz, pw.b = sp.px ? x_ws : x, pw.ldb = sp.px ? kp : ldx;      // dw[N, K] = dz^T x: sum over M
-        pw.M = (int)N, pw.N = (int)K, pw.K = (int)M;
         pw.y = dw, pw.ldy = K, pw.vec = K % 8 == 0 && rows16(dw, K, e);
         if (dx && dw && M > 0) return linear_gradients<T>(pw, px, slabs, s);
         if (dx && M > 0) return linear_product<T>(LIN_DX, px, slabs, s);

@@ -18,9 +18,13 @@ struct LinArgs {
     float* slabs;                       // split reduction: fp32 partial products [slices][M][N] instead of y
     int kslice;                         // k per slice (a multiple of the K step), K without a split
     int tiles_m, tiles_n;
+    // the weight gradient's launch also forms the bias gradient db[M] from `blocks` rows of column sums [blocks][M]; nullable
+    const float* sums;
+    void* db;
+    int blocks;
 };
 
-constexpr int KSTEP_BYTES = 128, MAX_SLICES = 32, SUM_BLOCKS = 256;
+constexpr int KSTEP_BYTES = 128, MAX_SLICES = 32, SUM_BLOCKS = 256, SUM_COLS = 32, SUM_GROUPS = 8;
 
 static inline long up(long v, long a) { return (v + a - 1) / a * a; }
 static inline bool rows16(const void* p, long ld, long e) { return ((uintptr_t)p & 15) == 0 && ld * e % 16 == 0; }
@@ -90,5 +94,7 @@ enum LinKind { LIN_FORWARD, LIN_DX, LIN_DW };
 template <class T> int linear_product(LinKind kind, const LinArgs& p, float* slabs, hipStream_t s);
 // DW and DX of one layer, in one launch where that is faster
 template <class T> int linear_gradients(LinArgs dw, LinArgs dx, float* slabs, hipStream_t s);
+// the bias's gradient alone: M, sums, blocks and db of its arguments
+template <class T> int linear_bias(const LinArgs& dw, hipStream_t s);
 
 }  // namespace acktr

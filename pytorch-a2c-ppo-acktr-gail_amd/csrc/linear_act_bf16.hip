@@ -4,4 +4,5 @@
 namespace acktr {
 template int linear_product<__bf16>(LinKind, const LinArgs&, float*, hipStream_t);
 template int linear_gradients<__bf16>(LinArgs, LinArgs, float*, hipStream_t);
+template int linear_bias<__bf16>(const LinArgs&, hipStream_t);
 }
