@@ -264,13 +264,13 @@ __global__ __launch_bounds__(WM * WN * 64, waves_of(BM, BN, WM * WN)) void linea
 }
 // All gradients of a layer in one launch: the weight gradient's tiles (long reductions) first, the input gradient's fill up behind
 // them, then the bias's.  Apart, each leaves part of the chip idle at its end, and of a small layer most of it.
-template <class T, int BM, int BN, int STAGES>
+template <class T, int XM, int STAGES, int XSTAGES>
 __global__ __launch_bounds__(256, 2) void linear_pair_kernel(const LinArgs dw, const LinArgs dx, int dw_groups, int tile_groups) {
     extern __shared__ char smem[];
     const int id = blockIdx.x, per = dw.tiles_m * dw.tiles_n;
-    if (id < dw_groups) linear_tile<T, false, false, BM, BN, 2, 2, STAGES, false>(dw, id % per, id / per, (ACKTR_LDS char*)smem);
+    if (id < dw_groups) linear_tile<T, false, false, 64, 64, 2, 2, STAGES, false>(dw, id % per, id / per, (ACKTR_LDS char*)smem);
     else if (id >= tile_groups) bias_sums<T>(dw, id - tile_groups, (ACKTR_LDS char*)smem);
-    else linear_tile<T, true, false, BM, BN, 2, 2, STAGES, false>(dx, id - dw_groups, 0, (ACKTR_LDS char*)smem);
+    else linear_tile<T, true, false, XM, 64, 2, 2, XSTAGES, false>(dx, id - dw_groups, 0, (ACKTR_LDS char*)smem);
 }
 
 template <class T>
@@ -371,14 +371,15 @@ static int product(LinArgs p, float* slabs, hipStream_t s) {
     return sum_slices<T>(p, pl.slices, s);
 }
 
-template <class T, int BM, int BN, int STAGES>
+template <class T, int XM, int STAGES, int XSTAGES>
 static int launch_pair(LinArgs& dw, LinArgs& dx, int slices, hipStream_t s) {
-    auto kern = linear_pair_kernel<T, BM, BN, STAGES>;
-    constexpr int lds = TileGemm<T, true, false, BM, BN, 2, 2, STAGES>::LDS;
+    auto kern = linear_pair_kernel<T, XM, STAGES, XSTAGES>;
+    constexpr int lw = TileGemm<T, false, false, 64, 64, 2, 2, STAGES>::LDS, lx = TileGemm<T, true, false, XM, 64, 2, 2, XSTAGES>::LDS;
+    constexpr int lds = lw > lx ? lw : lx;
     static std::atomic<unsigned> allowed{0};
     if (int rc = allow_lds((const void*)kern, lds, allowed)) return rc;
-    dw.tiles_m = cdiv(dw.M, BM), dw.tiles_n = cdiv(dw.N, BN);
-    dx.tiles_m = cdiv(dx.M, BM), dx.tiles_n = cdiv(dx.N, BN);
+    dw.tiles_m = cdiv(dw.M, 64), dw.tiles_n = cdiv(dw.N, 64);
+    dx.tiles_m = cdiv(dx.M, XM), dx.tiles_n = cdiv(dx.N, 64);
     const int first = dw.tiles_m * dw.tiles_n * slices, tiles = first + dx.tiles_m * dx.tiles_n;
     kern<<<tiles + bias_groups(dw), 256, lds, s>>>(dw, dx, first, tiles);
     ACKTR_LAUNCH_CHECK();
@@ -394,7 +395,8 @@ int linear_gradients(LinArgs dw, LinArgs dx, float* slabs, hipStream_t s) {
     }
     dw.kslice = (int)pl.kslice, dw.slabs = pl.slices > 1 ? slabs : nullptr;
     dx.kslice = dx.K, dx.slabs = nullptr;
-    const int rc = pl.tile == 0 ? launch_pair<T, 64, 64, sizeof(T) == 4 ? 2 : 3>(dw, dx, pl.slices, s) : launch_pair<T, 128, 64, 3>(dw, dx, pl.slices, s);
+    constexpr int ST = sizeof(T) == 4 ? 2 : 3;
+    const int rc = pl.tile == 0 ? launch_pair<T, 64, ST, ST>(dw, dx, pl.slices, s) : launch_pair<T, 128, ST, 3>(dw, dx, pl.slices, s);
     if (rc || pl.slices == 1) return rc;
     return sum_slices<T>(dw, pl.slices, s);
 }
