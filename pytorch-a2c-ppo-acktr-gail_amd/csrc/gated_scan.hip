@@ -224,7 +224,6 @@ struct Scan {
         float A[V], B[V], in[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) A[i] = 1.f, B[i] = 0.f;
-#pragma unroll 4
         for (int b = b0; b < b1; ++b) {
             const float* q = p.agg + 2L * (REV ? p.blocks - 1 - b : b) * C + c;
 #pragma unroll
@@ -453,22 +452,25 @@ __global__ __launch_bounds__(256) void scan_copy_kernel(const float* src, float*
 // --------------------------------------------------------------------------------------------------------- host side
 struct ScanPlan { int v, nw, sc, ct, blocks, block_steps; };
 
-// V = 2 (16-bit storage: 4 bytes a lane) where rows allow it and there are enough channels to give every CU a tile, or time to split.  Waves: as many as the steps fill, 8 at most.
-// Time is split over workgroups where the tiles alone would leave most CUs without work: the second read of the gates and values
-// that this costs is made by all CUs at once.
+// Time is split over workgroups (about 512 of them) where tiles of 64 channels alone would leave most of the chip without work: it costs
+// a second read of gates and values, by all CUs at once.  V = 2 (16-bit storage, rows that allow it: 4 bytes a lane, half the loads)
+// pays where there are tiles of 128 channels for every CU, or a split with enough steps to share.  Waves: as many as the steps fill.
+// Measured, forward + backward, us (bf16 unless said; H = 512):
+//   split: T x N 2048 x 8 54 against 120 whole, 2048 x 16 94 / 121, 512 x 16 30 / 37, 2048 x 20 121 / 125, 1024 x 24 85 / 67,
+//     2048 x 32 169 / 155; 256 x 4 21 / 20; fp32 2048 x 12 112 / 126, 512 x 16 46 / 41
+//   V = 2: whole 1024 x 64 118 against 154, 2048 x 32 188 / 155; split 512 x 16 30 / 34, 1024 x 8 31 / 34, 512 x 8 26 / 23
 static ScanPlan scan_plan(long T, long N, long H, int e, bool pair) {
     ScanPlan p;
     const long C = N * H;
-    p.v = e == 2 && pair && (C >= 128 * 256 || T > 1024) ? 2 : 1;
     p.nw = T <= 16 ? 1 : T <= 64 ? 4 : 8;
     p.sc = p.nw * SCAN_L;
+    const long chunks = cdiv(T, p.sc);
+    const bool split = chunks > 2 && C <= 64 * (e == 2 ? 128 : 96);
+    p.v = e == 2 && pair && (split ? T * C >= 1 << 22 : C >= 128 * 256) ? 2 : 1;
     p.ct = 64 * p.v;
-    const long tiles = cdiv(C, p.ct), chunks = cdiv(T, p.sc);
-    long per = chunks;
-    if (tiles < 96 && chunks > 1) per = cdiv(chunks, min(chunks, (long)cdiv(512, tiles)));
-    if (per < 1) per = 1;
+    const long per = split ? cdiv(chunks, min(chunks, (long)cdiv(512, cdiv(C, p.ct)))) : max(chunks, 1L);
     p.block_steps = (int)(per * p.sc);
-    p.blocks = chunks ? cdiv(chunks, per) : 1;
+    p.blocks = (int)max(cdiv(chunks, per), 1);
     return p;
 }
 // two neighbouring channels can be taken at once
