@@ -109,7 +109,7 @@ __device__ __forceinline__ void st4(void* p, int dt, long i, long n, bool vec, c
 // Sum of squares of all gradients, in fp64.  SMALL: partial sums only (and the step is counted): the update's workgroups add them up.
 // Otherwise the last workgroup to finish adds them, in the same fixed order, and writes the step's scalars: thousands of workgroups
 // would read too much, while for a few hundred the chain of atomics costs more than the rest of the launch (13 us against 5 for the
-// 867 thousand parameters of the NatureCNN policy).
+// 867 thousand parameters of the NatureCNN policy).  Bound by reading: 201 million fp32 gradients in 232 us (3.5 TB/s).
 template <bool SMALL>
 __global__ __launch_bounds__(AW_THREADS) void adamw_norm_kernel(AwState* st, const acktr_adamw_tensor* tensors, const int2* chunks, int nchunks) {
     __shared__ double sm[16];
@@ -188,7 +188,9 @@ __device__ __forceinline__ float wave_max(float v) {
     return v;
 }
 
-// SMALL: the step's scalars are formed here from `parts` partial sums, beside the loads of the elements.
+// SMALL: the step's scalars are formed here from `parts` partial sums, beside the loads of the elements.  Bound by memory, 201 million
+// parameters: 32 bits with bf16 parameters' gradients and copies 1066 us (5.3 TB/s), 8 bits 590 us (5.5 TB/s).  A thread takes 8 elements
+// of a chunk of 2048, all loads before the first use.
 template <int BITS, bool SMALL>
 __global__ __launch_bounds__(AW_THREADS) void adamw_update_kernel(const AwState* __restrict__ st, const acktr_adamw_tensor* __restrict__ tensors,
                                                                   const int2* __restrict__ chunks, void* mom1, void* mom2, float* scales,
@@ -304,7 +306,7 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_update_kernel(const AwState*
     }
 }
 
-// the values that 8-bit moments stand for
+// the values that 8-bit moments stand for: 2 bytes read, 8 written an element, 201 million in 415 us (4.9 TB/s)
 __global__ __launch_bounds__(256) void adamw_read_kernel(const uint8_t* __restrict__ mom1, const uint8_t* __restrict__ mom2,
                                                          const float* __restrict__ scales, float* __restrict__ m, float* __restrict__ v, long n) {
     for (long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (long)gridDim.x * 1024) {

@@ -247,6 +247,9 @@ __device__ __forceinline__ void bias_sums(const LinArgs& p, int id, ACKTR_LDS ch
 }
 static inline int bias_groups(const LinArgs& p) { return p.db ? cdiv(p.M, SUM_COLS) : 0; }
 
+// A product in tiles (bf16, 16384 x 2048 x 2048, each in a loop of its own; the clock moves them by 10 %): forward 103 us (1335 TFLOP/s),
+// with bias, silu, residual and slopes 154 us; input gradient 102 (1352); weight gradient in 4 slices 121 (1133).  Small ones are bound by launch, first loads and epilogue: 512 x 512 x 512
+// takes 5.4 us.
 // waves a SIMD: the largest tile has it to itself with two, the others share it
 constexpr int waves_of(int bm, int bn, int waves) { return bm * bn > 128 * 128 ? waves / 4 : 2; }
 
@@ -279,7 +282,8 @@ __global__ __launch_bounds__(SUM_COLS * SUM_GROUPS) void bias_kernel(const LinAr
     bias_sums<T>(p, blockIdx.x, (ACKTR_LDS char*)part);
 }
 
-// Sum of the slices of a split reduction in slice order, then the epilogue.  V: columns a thread, 8 where rows allow it, else 1.
+// Sum of the slices of a split reduction in slice order, then the epilogue: bound by reading them (4 slices of
+// 2048 x 2048 13 us, 6.5 TB/s out of the caches that the tiles left them in).  V: columns a thread, 8 where rows allow it, else 1.
 template <class T, int V>
 __global__ __launch_bounds__(256) void linear_slabs_kernel(const LinArgs p, int slices) {
     const int groups = p.N / V;

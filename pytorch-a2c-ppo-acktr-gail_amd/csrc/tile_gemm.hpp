@@ -12,11 +12,15 @@
 //                      consecutive k of its row each); fp32 fragments with one ds_read_b32 per k.
 // * A K step is 128 bytes of k (64 16-bit or 32 fp32 values), cut into two halves that alternate in registers: while the
 //   matrix cores work on one half, the other half is read from LDS.  STAGES K steps have a place in LDS: memory loads are in
-//   flight for STAGES - 1 K steps (a large tile computes long enough on one step to cover the latency with 2 stages, 64 x 64
-//   needs 4).  One barrier per K step, which waits for the oldest loads only.
+//   flight for STAGES - 1 K steps (a large tile computes long enough on one step to cover the latency with 2 stages, the small
+//   ones take 3; 5 to 8 were no faster).  One barrier per K step, which waits for the oldest loads only.
 // * The products are formed transposed (B's rows on the matrix instruction's row side), so that a lane ends up with four
 //   consecutive n of one m.  fp32 uses v_mfma_f32_16x16x4 on the same fragments: a lane group's four consecutive k are four
 //   instructions, each pairing the same k of A and B.
+// * What bounds it (16384 x 2048 x 2048, bf16, one part of the loop at a time): 64 x 64 tiles 183 us, of which the copies into LDS
+//   alone take 162 (4.3 GB at 26 TB/s, whether or not the L2 caches hit), products 67, LDS reads 80; 128 x 128 tiles 125: 105, 66, 52;
+//   256 x 256 tiles 107: 79, 79, 46.  So small tiles are bound by the copies, and the largest one by how far copies, products and
+//   reads overlap.  Two wave groups half a step apart were slower there (127 us): their extra barriers cost more than the overlap.
 // * Memory loads are written as inline assembly because the compiler, which cannot tell the LDS stages apart, would wait for
 //   all of them in front of every LDS read.  They write no register; tile_sync() waits for them.
 #pragma once
