@@ -7,12 +7,14 @@ same pass.  The step counter and the hyperparameters live in device memory, so a
 with the right bias corrections.
 """
 import ctypes
+import operator
 
 import torch
 
 from .. import _hip, ops
 
 f32 = torch.float32
+_POINTER, _COUNT, _DENSE, _TYPE = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous, operator.attrgetter('dtype')
 
 
 class AdamW(object):
@@ -91,11 +93,11 @@ class AdamW(object):
         return out
 
     def _table(self, grads):
-        """The device table of tensors, rebuilt only when one of them was replaced (checked by address, size and type)."""
-        ptr, num = torch.Tensor.data_ptr, torch.Tensor.numel
-        own = self.params + self._copied                      # (tensors that this object holds: their types stay)
-        seen = [list(map(ptr, own)), list(map(num, own)), list(map(ptr, grads)), list(map(num, grads)),
-                None if grads is self.grads else [g.dtype for g in grads]]
+        """The device table of tensors, rebuilt (and its entries checked) only when one of them changed: another address, size, type
+        or layout."""
+        own = self.params + self._copied
+        every = own + grads
+        seen = [list(map(_POINTER, every)), list(map(_COUNT, every)), list(map(_TYPE, every)), all(map(_DENSE, every))]
         if seen == self._seen:
             return
         dev = self._dev

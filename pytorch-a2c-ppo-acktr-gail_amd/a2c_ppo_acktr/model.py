@@ -244,7 +244,7 @@ class NNBase(nn.Module):
     def __init__(self, recurrent, recurrent_input_size, hidden_size):
         super(NNBase, self).__init__()
         self._hidden_size = hidden_size
-        if recurrent not in (True, False, 'gated'):
+        if isinstance(recurrent, str) and recurrent != 'gated':
             raise ValueError("recurrent must be True, False or 'gated' (got %r)" % (recurrent,))
         self._recurrent = bool(recurrent)
         if recurrent == 'gated':

@@ -329,6 +329,36 @@ def test_a_captured_step_follows_the_table():
     assert torch.equal(want.params[0], opt.params[0]) and opt.steps_done() == 3
 
 
+def test_another_layout_at_the_same_address_is_refused():
+    from a2c_ppo_acktr import algo
+    p, g = rnd(1, 40, 40), rnd(2, 40, 40)
+    opt = algo.AdamW([p], **HP)
+    p.grad = g
+    opt.step()
+    before = p.clone()
+    p.grad = g.t()                                           # same memory, size and type
+    with pytest.raises(RuntimeError, match='contiguous'):
+        opt.step()
+    p.grad = g
+    opt.step()
+    assert opt.steps_done() == 2 and not torch.equal(p, before)
+
+
+def test_a_tensor_of_more_than_2_31_elements():
+    """the last elements of a long tensor take the step that they would take in a short one"""
+    from a2c_ppo_acktr import algo
+    n, tail = (1 << 31) + 4099, 5000
+    p, g = torch.zeros(n, dtype=torch.bfloat16, device=DEV), torch.zeros(n, dtype=torch.bfloat16, device=DEV)
+    p[-tail:] = rnd(1, tail).bfloat16()
+    g[-tail:] = rnd(2, tail).bfloat16()
+    q, h = p[-tail:].clone(), g[-tail:].clone()
+    long, short = algo.AdamW([p], grads=[g], **HP), algo.AdamW([q], grads=[h], **HP)
+    for _ in range(2):
+        long.step()
+        short.step()
+    assert torch.equal(p[-tail:], q) and not p[:4096].any()
+
+
 def test_refusals():
     from a2c_ppo_acktr import algo
     p, g = rnd(1, 100), rnd(2, 100)

@@ -84,6 +84,39 @@ def test_steps_are_the_sequence():
     assert float((state - last).abs().max()) < 64 * 2.0 ** -24 * 8
 
 
+def test_forward_and_backward_captured():
+    """both passes recorded into a graph by autograd; replays follow new inputs and stay right beside eager work"""
+    from a2c_ppo_acktr import gated, ops
+    T, N, I, H = 70, 3, 24, 40
+    core = gated.GatedCore(I, H).to(DEV)
+    x, st = torch.zeros(T, N, I, device=DEV).requires_grad_(), torch.zeros(N, H, device=DEV)
+    m, dy = torch.ones(T, N, device=DEV), torch.zeros(T, N, H, device=DEV)
+    leaves = [x] + list(core.parameters())
+
+    def both():
+        y, last = core(x, st, m)
+        return (y.detach(), last.detach()) + torch.autograd.grad(y, leaves, dy)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with ops.graph_capture(g):
+        out = both()
+    for k in range(3):
+        with torch.no_grad():
+            x.copy_(torch.randn(T, N, I, device=DEV))
+            st.copy_(torch.randn(N, H, device=DEV))
+            dy.copy_(torch.randn(T, N, H, device=DEV))
+            m.copy_((torch.rand(T, N, device=DEV) > 0.1).float())
+        want = [t.clone() for t in both()]
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, want)), k
+
+
 def test_autograd_corners():
     from a2c_ppo_acktr.gated import gated_scan, linear_act
     # a residual that is broadcast, an input used twice, a gradient that is expanded, no gradient for a part

@@ -43,6 +43,13 @@ def test_other_values_are_refused():
         algo.PPO(pol, 0.2, 1, 1, 0.5, 0.0, lr=1e-3, eps=1e-5, weight_decay=-1.0)
 
 
+def test_what_was_falsy_or_truthy_still_is():
+    from a2c_ppo_acktr.model import Policy
+    assert not Policy((11,), Box(), base_kwargs={'recurrent': None}).is_recurrent
+    assert not Policy((11,), Box(), base_kwargs={'recurrent': 0}).is_recurrent
+    assert hasattr(Policy((11,), Box(), base_kwargs={'recurrent': 1}).base, 'gru')
+
+
 def test_the_gru_is_what_it_was():
     """same initialiser calls in the same order: a seed gives the same GRU policy with and without the new core in the package"""
     from a2c_ppo_acktr.model import Policy

@@ -200,6 +200,45 @@ def test_gradient_against_differences():
         assert abs(num - ana) <= 2e-5 * float(grads[i].double().norm() * d.norm()), (i, num, ana)
 
 
+@pytest.mark.parametrize('dt', [BF, F32])
+@pytest.mark.parametrize('far', ['steps', 'sequences'])
+def test_strides_that_need_64_bits(far, dt):
+    """a few short rows, gigabytes apart"""
+    from a2c_ppo_acktr import ops
+    T, N, H = 20, 3, 40
+    e = torch.empty(0, dtype=dt).element_size()
+
+    def spread(t):
+        if far == 'steps':                                   # 16 steps reach over 2^31 bytes
+            return torch.empty(T, (1 << 27) // e + 8, dtype=dt, device=DEV)[:, :N * H].view(T, N, H).copy_(t)
+        return torch.empty(N, (1 << 30) // e + 8, dtype=dt, device=DEV)[:, :T * H].view(N, T, H).transpose(0, 1).copy_(t)
+    g, v, m, h0, dout, dl = inputs(T, N, H, dt)
+    out, dg, dv = spread(torch.zeros_like(dout)), spread(torch.zeros_like(dout)), spread(torch.zeros_like(dout))
+    gs, vs, ds = spread(g), spread(v), spread(dout)
+    _, fin, saved = ops.gated_scan_fwd(gs, vs, h0, m, out=out, save=True)
+    _, _, dh0 = ops.gated_scan_bwd(ds, gs, vs, h0, m, saved=saved, dlast=dl, dgate=dg, dvalue=dv)
+    ref = scan64(g, v, h0, m, dout, dl)
+    for name, t in (('out', out), ('last', fin), ('dgate', dg), ('dvalue', dv), ('dh0', dh0)):
+        check(t, ref[name], name)
+
+
+def test_more_than_2_31_elements():
+    """a sequence whose last steps lie past 2^31 elements: a restart cuts off what would need a reference of a million steps"""
+    from a2c_ppo_acktr import ops
+    T, N, H, tail = (1 << 20) + 300, 1, 2048, 200
+    g, v = torch.zeros(T, N, H, dtype=BF, device=DEV), torch.zeros(T, N, H, dtype=BF, device=DEV)
+    dout, m = torch.zeros(T, N, H, dtype=BF, device=DEV), torch.ones(T, N, device=DEV)
+    m[T - tail] = 0
+    for i, t in enumerate((g, v, dout)):
+        t[-tail:] = rnd(i, tail, N, H, dtype=BF)
+    out, fin, saved = ops.gated_scan_fwd(g, v, None, m, save=True)
+    dg, dv, dh0 = ops.gated_scan_bwd(dout, g, v, None, m, saved=saved)
+    ref = scan64(g[-tail:], v[-tail:], None, m[-tail:], dout[-tail:], None)
+    for name, t in (('out', out), ('last', fin), ('dgate', dg), ('dvalue', dv)):
+        check(t if name == 'last' else t[-tail:], ref[name], name)
+    assert not out[:-tail].any() and not dg[:-tail].any() and not dh0.any()
+
+
 def test_captured_and_replayed():
     from a2c_ppo_acktr import ops
     for T, N, H in ((150, 4, 64), (4000, 1, 16)):

@@ -212,6 +212,25 @@ def test_captured_and_replayed():
             assert all(torch.equal(p, q) for p, q in zip(out, want)), k
 
 
+def test_more_than_2_31_elements():
+    """the last rows of a product whose rows reach past 2^31 elements; gradients that only those rows have"""
+    from a2c_ppo_acktr import ops
+    M, N, K, tail = (1 << 20) + 700, 2048, 24, 300
+    x, w, b = rnd(1, M, K, dtype=BF), rnd(2, N, K, scale=0.3, dtype=BF), rnd(3, N, dtype=BF)
+    pre = torch.empty(M, N, dtype=BF, device=DEV)
+    y = ops.linear_act_fwd(x, w, b, act='silu', pre=pre)
+    dy = torch.zeros(M, N, dtype=BF, device=DEV)
+    dy[-tail:] = rnd(4, tail, N, scale=0.1, dtype=BF)
+    dx, dw, db = ops.linear_act_bwd(dy, x, w, pre=pre, act='silu')
+    ry, ty, slope, ts = linear64(x[-tail:], w, b, 'silu', None)
+    gx, gw, gb = linear_grads64(dy[-tail:], x[-tail:], w, slope, ts)
+    check(y[-tail:], (ry, ty), 'y')
+    check(dx[-tail:], gx, 'dx')
+    check(dw, gw, 'dw')
+    check(db, gb, 'db')
+    assert not dx[:-tail].any()
+
+
 def test_two_streams():
     from a2c_ppo_acktr import ops
     a, b = torch.cuda.Stream(), torch.cuda.Stream()
