@@ -79,6 +79,8 @@ class AdamW(object):
         which = torch.repeat_interleave(count)                # {tensor, chunk number} pairs
         first = torch.cumsum(count, 0) - count
         self._chunks = torch.stack((which, torch.arange(which.numel()) - first[which]), 1).to(torch.int32).to(dev)
+        # (pointers to what never moves)
+        self._fixed = self._state.data_ptr(), self._tensors.data_ptr(), self._chunks.data_ptr(), self._chunks.shape[0]
         self._seen = self._hyper = None
 
     def _gradients(self):
@@ -95,8 +97,7 @@ class AdamW(object):
     def _table(self, grads):
         """The device table of tensors, rebuilt (and its entries checked) only when one of them changed: another address, size, type
         or layout."""
-        own = self.params + self._copied
-        every = own + grads
+        every = self.params + self._copied + grads
         seen = [list(map(_POINTER, every)), list(map(_COUNT, every)), list(map(_TYPE, every)), all(map(_DENSE, every))]
         if seen == self._seen:
             return
@@ -120,7 +121,7 @@ class AdamW(object):
                                        ops.DTYPE_CODE[p.dtype], ops.DTYPE_CODE[g.dtype],
                                        ops.DTYPE_CODE[c.dtype] if c is not None else 0,
                                        (1 if quad(p) else 0) | (2 if quad(g) else 0) | (4 if quad(c) else 0))
-        spans = sorted((t.data_ptr(), t.data_ptr() + t.nbytes) for t in own if t.numel())
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.nbytes) for t in self.params + self._copied if t.numel())
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise RuntimeError('AdamW: two of the tensors to be written overlap (the same parameter twice?)')
         if torch.cuda.is_current_stream_capturing():
@@ -132,19 +133,17 @@ class AdamW(object):
     def prepare(self):
         """Brings the device side up to date with the parameter list and the hyperparameters: outside a graph capture, and before a
         replay when a hyperparameter changed."""
-        dev = self.params[0].device
-        if dev.type == 'cuda' and dev.index is None:
-            dev = torch.device('cuda', torch.cuda.current_device())
-        if self._dev is None or self._dev != dev:
+        g = self.param_groups[0]
+        dev = g['params'][0].device
+        if self._dev != dev:
             if dev.type != 'cuda':
                 raise RuntimeError('AdamW: parameters must live on the MI355X device (got %s): this package has no CPU path' % dev)
             if self._dev is not None:
                 raise RuntimeError('AdamW: the parameters moved to %s; build a new optimiser' % dev)
             with torch.no_grad():
                 self._allocate(dev)
-        g = self.param_groups[0]
-        hyper = (float(g['lr']), float(g['betas'][0]), float(g['betas'][1]), float(g['eps']), float(g['weight_decay']),
-                 float(g['max_grad_norm'] or 0.0))
+        b1, b2 = g['betas']
+        hyper = (float(g['lr']), float(b1), float(b2), float(g['eps']), float(g['weight_decay']), float(g['max_grad_norm'] or 0.0))
         if hyper != self._hyper:
             self._check_hyper()
             if torch.cuda.is_current_stream_capturing():
@@ -169,12 +168,9 @@ class AdamW(object):
     def step(self):
         """One step on all tensors: two launches."""
         self.prepare()
-        L = _hip.lib()
-        with ops._on(self._dev.index):
-            rc = L.acktr_adamw_step(self._state.data_ptr(), self._tensors.data_ptr(), self._chunks.data_ptr(), self._chunks.shape[0],
-                                    self.mom1.data_ptr(), self.mom2.data_ptr(), self.scales.data_ptr() if self.scales is not None else None,
-                                    self.state_bits, 1 if self._hyper[5] > 0 else 0, _hip.cur_stream(self._dev))
-        _hip.check(rc, 'acktr_adamw_step')
+        ops._launch(_hip.lib().acktr_adamw_step, self._dev.index, 'adamw_step', 20.0 * self._total, *self._fixed, self.mom1.data_ptr(),
+                    self.mom2.data_ptr(), self.scales.data_ptr() if self.scales is not None else None, self.state_bits,
+                    1 if self._hyper[5] > 0 else 0)
         self.step_count += 1
 
     def moments(self):
@@ -185,10 +181,8 @@ class AdamW(object):
         if self.state_bits == 32:
             return self.mom1, self.mom2
         m, v = torch.empty(self._total, dtype=f32, device=self._dev), torch.empty(self._total, dtype=f32, device=self._dev)
-        with ops._on(self._dev.index):
-            rc = _hip.lib().acktr_adamw_read_moments(self.mom1.data_ptr(), self.mom2.data_ptr(), self.scales.data_ptr(), m.data_ptr(),
-                                                     v.data_ptr(), self._total, _hip.cur_stream(self._dev))
-        _hip.check(rc, 'acktr_adamw_read_moments')
+        ops._launch(_hip.lib().acktr_adamw_read_moments, self._dev.index, 'adamw_read_moments', 0.0, self.mom1.data_ptr(),
+                    self.mom2.data_ptr(), self.scales.data_ptr(), m.data_ptr(), v.data_ptr(), self._total)
         return m, v
 
     def offsets(self):
