@@ -2,7 +2,8 @@
 
 Thin plumbing only: shape checks on the host (a wrong shape must never reach a
 kernel), device pointers + the current stream handed to the library.  Every
-function requires fp32 contiguous GPU tensors and raises otherwise.
+function requires fp32 contiguous GPU tensors and raises otherwise; the gated
+core's operators at the end take bf16, fp16 or fp32 and rows of wider tensors.
 """
 import contextlib
 import ctypes
