@@ -75,13 +75,17 @@ struct Scan {
     typedef vec_t<T, V> vv;
     typedef vec_t<float, 2 * V> pairs;
 
-    int lane, wave, c, dn, j, n0;                    // n0: the tile's first sequence, dn: this lane's, counted from there
+    int lane, wave, tile, c, dn, j, n0;                    // n0: the tile's first sequence, dn: this lane's, counted from there
     bool live;
 
     __device__ __forceinline__ void place(const ScanArgs& p) {
         lane = threadIdx.x & 63;
         wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        const long first = (long)blockIdx.x * CT, C = (long)p.N * p.H;
+        // Workgroups go to the 8 L2 caches in turn: each cache gets a contiguous piece of the tiles, whose neighbours share lines where
+        // rows do not start at a line's boundary (594 x 116 x 973, forward + backward: bf16 390 -> 314 us, fp32 633 -> 488).
+        const int tiles = gridDim.x, per = (tiles + 7) / 8, whole = tiles - 8 * (per - 1), x = blockIdx.x & 7, q = blockIdx.x >> 3;
+        tile = x < whole ? x * per + q : whole * per + (x - whole) * (per - 1) + q;
+        const long first = (long)tile * CT, C = (long)p.N * p.H;
         live = first + lane * V < C;
         c = (int)(live ? first + lane * V : first);
         n0 = (int)(first / p.H);
@@ -249,7 +253,7 @@ __global__ __launch_bounds__(NW * 64) void scan_fwd_kernel(const ScanArgs p) {
     const long C = (long)p.N * p.H;
     const int blk = blockIdx.y, tb = blk * p.block_steps, te = min(p.T, tb + p.block_steps);
     const typename S::Rows rg = s.rows(p.gate, p.gt, p.gn), rv = s.rows(p.value, p.vt, p.vn), ro = s.rows(p.out, p.ot, p.on);
-    const bool all = (long)(blockIdx.x + 1) * S::CT <= C;    // every lane of the tile has channels
+    const bool all = (long)(s.tile + 1) * S::CT <= C;    // every lane of the tile has channels
     float carry[V], prod[V];
     int par = 0;
 #pragma unroll
@@ -325,7 +329,7 @@ __global__ __launch_bounds__(NW * 64) void scan_bwd_kernel(const ScanArgs p) {
     const int blk = blockIdx.y, tb = blk * p.block_steps, te = min(p.T, tb + p.block_steps);
     const typename S::Rows rg = s.rows(p.gate, p.gt, p.gn), rv = s.rows(p.value, p.vt, p.vn), rd = s.rows(p.dout, p.dt, p.dn);
     const typename S::Rows qg = s.rows(p.dgate, p.dgt, p.dgn), qv = s.rows(p.dvalue, p.dvt, p.dvn);
-    const bool all = (long)(blockIdx.x + 1) * S::CT <= C;
+    const bool all = (long)(s.tile + 1) * S::CT <= C;
     float carry[V], prod[V];                                 // carry: E behind the steps that are done
     int par = 0;
 #pragma unroll
