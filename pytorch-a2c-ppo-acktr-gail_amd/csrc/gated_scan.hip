@@ -461,21 +461,23 @@ struct ScanPlan { int v, nw, sc, ct, blocks, block_steps; };
 
 // Time is split over workgroups (about 512 of them) where tiles of 64 channels alone would leave most of the chip without work: it costs
 // a second read of gates and values, by all CUs at once.  V = 2 (16-bit storage, rows that allow it: 4 bytes a lane, half the loads)
-// pays where there are tiles of 128 channels for every CU, or a split with enough steps to share.  Waves: as many as the steps fill.
+// pays where there are tiles of 128 channels for every CU, or a split with enough steps to share.  Waves: as many as the steps fill, up
+// to 8, or 4 where two workgroups and more share a CU anyway.
 // Measured, forward + backward, us (bf16 unless said; H = 512):
 //   split: T x N 2048 x 8 54 against 120 whole, 2048 x 16 94 / 121, 512 x 16 30 / 37, 2048 x 20 121 / 125, 1024 x 24 85 / 67,
 //     2048 x 32 169 / 155; 256 x 4 21 / 20; fp32 2048 x 12 112 / 126, 512 x 16 46 / 41
+//   4 waves instead of 8 (H = 1024): 300 x 64 67 against 76, 594 x 116 267 / 275, 128 x 256 120 / 131; 2048 x 32, a tile a CU, 279 / 236
 //   V = 2: whole 1024 x 64 118 against 154, 2048 x 32 188 / 155; split 512 x 16 30 / 34, 1024 x 8 31 / 34, 512 x 8 26 / 23
 static ScanPlan scan_plan(long T, long N, long H, int e, bool pair) {
     ScanPlan p;
     const long C = N * H;
-    p.nw = T <= 16 ? 1 : T <= 64 ? 4 : 8;
-    p.sc = p.nw * SCAN_L;
-    const long chunks = cdiv(T, p.sc);
-    const bool split = chunks > 2 && C <= 64 * (e == 2 ? 128 : 96);
+    const bool split = T > 2 * 8 * SCAN_L && C <= 64 * (e == 2 ? 128 : 96);
     p.v = e == 2 && pair && (split ? T * C >= 1 << 22 : C >= 128 * 256) ? 2 : 1;
     p.ct = 64 * p.v;
-    const long per = split ? cdiv(chunks, min(chunks, (long)cdiv(512, cdiv(C, p.ct)))) : max(chunks, 1L);
+    const long tiles = cdiv(C, p.ct);
+    p.nw = T <= 16 ? 1 : T <= 64 || tiles >= 512 ? 4 : 8;
+    p.sc = p.nw * SCAN_L;
+    const long chunks = cdiv(T, p.sc), per = split ? cdiv(chunks, min(chunks, (long)cdiv(512, tiles))) : max(chunks, 1L);
     p.block_steps = (int)(per * p.sc);
     p.blocks = (int)max(cdiv(chunks, per), 1);
     return p;
