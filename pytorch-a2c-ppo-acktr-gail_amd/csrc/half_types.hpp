@@ -13,6 +13,11 @@ template <class T, int N>
 struct VecOf { typedef T type __attribute__((ext_vector_type(N))); };
 template <class T, int N>
 using vec_t = typename VecOf<T, N>::type;
+// the same in memory at any element's address: one wide access, which the hardware splits where it has to
+template <class T, int N>
+struct UnalignedVecOf { typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T)))); };
+template <class T, int N>
+using uvec_t = typename UnalignedVecOf<T, N>::type;
 
 template <class T> __device__ __forceinline__ float to_f32(T v) { return (float)v; }
 template <class T> __device__ __forceinline__ T from_f32(float v) { return (T)v; }

@@ -10,12 +10,23 @@
 
 namespace acktr {
 
+// V values of a row, `left` of which it still has; 0 behind them
+template <class T, int V>
+__device__ __forceinline__ vec_t<T, V> row_piece(const T* p, int left) {
+    if (left >= V) return *reinterpret_cast<const uvec_t<T, V>*>(p);
+    vec_t<T, V> v;
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = j < left ? p[j] : (T)0.f;
+    return v;
+}
+
 // dst[r][c] = src[r][c] for c < cols, 0 up to ldd: a copy whose rows start at 16-byte boundaries, for operands that do not
 // (an odd width, a slice of a wider row).  It costs one pass over the operand; reading such rows element by element in the
-// product would cost a fetch per element of every tile that uses it.  Up to two operands a launch (4.3 us for 1011 x 777 and 390 x 777
+// product would cost a fetch per element of every tile that uses it.  Up to three operands a launch (4.2 us for 1011 x 777 and 390 x 777
 // fp16 values together).
 struct PackJob { const void* src; long lds; int rows, cols; void* dst; int ldd; };
-struct PackJobs { PackJob job[2]; };
+struct PackJobs { PackJob job[3]; };
+constexpr int PACK_U = 4;                    // 16-byte pieces a thread has in flight
 template <class T>
 __global__ __launch_bounds__(256) void pack_rows_kernel(const PackJobs jobs) {
     const PackJob p = jobs.job[blockIdx.y];
@@ -23,39 +34,46 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(const PackJobs jobs) {
     typedef vec_t<T, V> vv;
     const int groups = p.ldd / V;
     const long total = (long)p.rows * groups;
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
-        const long r = i / groups;
-        const int c = (int)(i % groups) * V;
-        const T* src = (const T*)p.src + r * p.lds + c;
-        vv o;
+    for (long i0 = (long)blockIdx.x * (256 * PACK_U) + threadIdx.x; i0 < total; i0 += (long)gridDim.x * (256 * PACK_U)) {
+        vv o[PACK_U];
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = c + j < p.cols ? src[j] : (T)0.f;
-        *reinterpret_cast<vv*>((T*)p.dst + r * p.ldd + c) = o;
+        for (int u = 0; u < PACK_U; ++u) {
+            const long i = min(i0 + u * 256, total - 1);
+            const long r = total < (1L << 31) ? (long)((unsigned)i / (unsigned)groups) : i / groups;
+            const int c = (int)(i - r * groups) * V;
+            o[u] = row_piece<T, V>((const T*)p.src + r * p.lds + c, p.cols - c);
+        }
+#pragma unroll
+        for (int u = 0; u < PACK_U; ++u) {
+            const long i = i0 + u * 256;               // (rows of ldd values lie one behind the other)
+            if (i < total) *reinterpret_cast<vv*>((T*)p.dst + i * V) = o[u];
+        }
     }
 }
 
 // dz = dy slope (ACT; dz null: not wanted; without ACT dz is dy itself) and, per block of rows, the column sums of dz.
 // A thread holds one group of V columns and walks the block's rows in steps of 8; sums[block][N] (nullable).  Bound by memory: bf16,
 // 16384 x 2048 in 40 us (5.0 TB/s).  dz is written once, in rows that both products read, rather than formed in each of them.
+// Zeros are written up to the end of dz's aligned row, which the products read.  V: 16 bytes, or 1 where a small matrix has rows that
+// do not fill or start at 16 bytes (fp16, with 8 and 1: 1011 x 390 4.7 and 3.8 us, 4011 x 390 8.2 and 6.2, 8011 x 390 8.2 and 10.6,
+// 8011 x 1390 15.4 and 24.9).
 template <class T, bool ACT, int V>
 __global__ __launch_bounds__(256) void act_bwd_kernel(const T* __restrict__ dy, long lddy, const void* __restrict__ pre, long ldp,
                                                       T* __restrict__ dz, long lddz, int M, int N, int rows_per, float* __restrict__ sums) {
-    typedef vec_t<T, V> vv;
     typedef typename SlopeOf<T>::type ST;
-    typedef vec_t<ST, V> sv;
     const int cg = threadIdx.x & 31, rg = threadIdx.x >> 5;
-    const int n = (blockIdx.x * 32 + cg) * V;
+    const int n = (blockIdx.x * 32 + cg) * V, left = N - n;
     const int r0 = blockIdx.y * rows_per, r1 = min(M, r0 + rows_per);
     float s[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) s[i] = 0.f;
-    if (n < N) {
+    if (n < (ACT && dz ? (int)lddz : N)) {
 #pragma unroll 4
         for (int r = r0 + rg; r < r1; r += 8) {
-            const vv g = *reinterpret_cast<const vv*>(dy + r * lddy + n);
-            sv z;
-            vv o;
-            if (ACT) z = *reinterpret_cast<const sv*>((const ST*)pre + r * ldp + n);
+            const vec_t<T, V> g = row_piece<T, V>(dy + r * lddy + n, left);
+            vec_t<ST, V> z;
+            vec_t<T, V> o;
+            if (ACT) z = row_piece<ST, V>((const ST*)pre + r * ldp + n, left);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 float d = to_f32(g[i]);
@@ -63,10 +81,8 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(const T* __restrict__ dy, 
                 s[i] += d;
                 o[i] = from_f32<T>(d);
             }
-            if (ACT && dz) *reinterpret_cast<vv*>(dz + r * lddz + n) = o;
+            if (ACT && dz) *reinterpret_cast<vec_t<T, V>*>(dz + r * lddz + n) = o;
         }
-    } else if (ACT && V == 1 && dz && n < lddz) {            // the padding columns of aligned dz rows, which the products read
-        for (int r = r0 + rg; r < r1; r += 8) dz[r * lddz + n] = from_f32<T>(0.f);
     }
     if (!sums) return;
     __shared__ float part[8][32 * V];
@@ -93,7 +109,7 @@ static int pack(std::initializer_list<PackJob> list, hipStream_t s) {
             most = max(most, (long)j.rows * (j.ldd * (long)sizeof(T) / 16));
         }
     if (n == 0) return 0;
-    pack_rows_kernel<T><<<dim3(min(cdiv(most, 256), 4096), n), 256, 0, s>>>(jobs);
+    pack_rows_kernel<T><<<dim3(min(cdiv(most, 256 * PACK_U), 4096), n), 256, 0, s>>>(jobs);
     ACKTR_LAUNCH_CHECK();
     return 0;
 }
@@ -111,6 +127,7 @@ static int check_ld(const char* what, long ld, long cols) {
     return 0;
 }
 
+static constexpr long ROWS_WIDE = 1 << 21;    // values from which unaligned rows are taken 16 bytes at a time
 static constexpr int per16(int e) { return 16 / e; }
 
 }  // namespace acktr
@@ -131,13 +148,12 @@ static FwdSpace fwd_space(const void* x, long ldx, const void* w, long ldw, long
     f.bytes = f.slabs + slab_bytes(M, N, plan_of(M, N, kp, e).slices);
     return f;
 }
-struct BwdSpace { bool aligned, pdy, px, pw; long dz, x, w, sums, slabs, bytes; };
+struct BwdSpace { bool pdy, px, pw; long dz, x, w, sums, slabs, bytes; };
 static BwdSpace bwd_space(const void* dy, long lddy, const void* x, long ldx, const void* w, long ldw, const void* pre, long ldp, bool dx, bool dw,
                           bool db, long M, long N, long K, int e, int act) {
     BwdSpace f;
     const int V = per16(e);
     const long np = up(N, V), kp = up(K, V);
-    f.aligned = N % V == 0 && rows16(dy, lddy, e) && (act == ACKTR_ACT_NONE || rows16(pre, ldp, e));
     f.pdy = act == ACKTR_ACT_NONE && (dx || dw) && (N % V != 0 || !rows16(dy, lddy, e));
     f.px = dw && (K % V != 0 || !rows16(x, ldx, e));
     f.pw = dx && (K % V != 0 || !rows16(w, ldw, e));
@@ -181,8 +197,6 @@ extern "C" int acktr_linear_act_fwd(const void* x, long ldx, const void* w, long
         p.a = x, p.lda = ldx, p.b = w, p.ldb = ldw;
         p.M = (int)M, p.N = (int)N, p.K = (int)K;
         p.y = y, p.ldy = ldy, p.bias = bias, p.res = residual, p.ldr = ldr, p.pre = pre, p.ldp = ldp, p.act = act;
-        p.vec = N % 8 == 0 && rows16(y, ldy, e) && (!bias || ((uintptr_t)bias & 15) == 0) && (!residual || rows16(residual, ldr, e)) &&
-                (!pre || rows16(pre, ldp, e));
         char* ws = (char*)workspace;
         const int kp = (int)up(K, per16(e));
         if (int rc = pack<T>({{x, ldx, sp.px ? (int)M : 0, (int)K, ws + sp.x, kp}, {w, ldw, sp.pw ? (int)N : 0, (int)K, ws + sp.w, kp}}, s)) return rc;
@@ -225,26 +239,19 @@ extern "C" int acktr_linear_act_bwd(const void* dy, long lddy, const void* x, lo
 
         LinArgs px{}, pw{};
         int blocks = 0;
-        // dz and the column sums.  Rows of dy (or pre) that do not start at 16 bytes, or end inside 16, are taken value by value;
-        // dz itself is written into aligned rows, which the two products read.
+        // dz, in aligned rows, which the two products read, and the column sums
         const void* dz = dy;
         long lddz = lddy;
         const bool write = act != ACKTR_ACT_NONE && M > 0;
         if (write) dz = dz_ws, lddz = np;
         if (M > 0 && (write || db)) {
-            const int cols = sp.aligned ? 32 * V : 32;
-            const int gx = cdiv(N, cols);
+            const bool wide = (long)M * N >= ROWS_WIDE || (N % V == 0 && rows16(dy, lddy, e) && (!write || rows16(pre, ldp, e)));
+            const int gx = cdiv(write ? np : N, wide ? 32 * V : 32);
             const int want = max(1, min(SUM_BLOCKS, 2048 / gx));
             const int rows_per = (int)up(max(16, cdiv(M, want)), 8), gy = cdiv(M, rows_per);
-            auto launch = [&](auto act_c, auto v_c) {
-                act_bwd_kernel<T, decltype(act_c)::value, decltype(v_c)::value><<<dim3(gx, gy), 256, 0, s>>>(
-                    (const T*)dy, lddy, pre, ldp, dz_ws, np, (int)M, (int)N, rows_per, db ? sums : nullptr);
-            };
-            using std::integral_constant;
-            if (write && sp.aligned) launch(std::true_type{}, integral_constant<int, V>{});
-            else if (write) launch(std::true_type{}, integral_constant<int, 1>{});
-            else if (sp.aligned) launch(std::false_type{}, integral_constant<int, V>{});
-            else launch(std::false_type{}, integral_constant<int, 1>{});
+            const auto kern = write ? (wide ? act_bwd_kernel<T, true, V> : act_bwd_kernel<T, true, 1>)
+                                    : (wide ? act_bwd_kernel<T, false, V> : act_bwd_kernel<T, false, 1>);
+            kern<<<dim3(gx, gy), 256, 0, s>>>((const T*)dy, lddy, pre, ldp, dz_ws, np, (int)M, (int)N, rows_per, db ? sums : nullptr);
             ACKTR_LAUNCH_CHECK();
             blocks = gy;
         }
@@ -252,17 +259,13 @@ extern "C" int acktr_linear_act_bwd(const void* dy, long lddy, const void* x, lo
         pw.sums = sums, pw.blocks = blocks, pw.db = db;
         if (db && !dw)                                       // no weight gradient's launch for it to ride in
             if (int rc = linear_bias<T>(pw, s)) return rc;
-        if (M > 0 && sp.pdy) {                               // no activation: dy itself, in aligned rows
-            if (int rc = pack<T>({{dy, lddy, (int)M, (int)N, dz_ws, np}}, s)) return rc;
-            dz = dz_ws, lddz = np;
-        }
-        if (int rc = pack<T>({{x, ldx, sp.px ? (int)M : 0, (int)K, x_ws, kp}, {w, ldw, sp.pw && M > 0 ? (int)N : 0, (int)K, w_ws, kp}}, s)) return rc;
+        if (sp.pdy) dz = dz_ws, lddz = np;                   // no activation: dy itself, in aligned rows
+        if (int rc = pack<T>({{dy, lddy, sp.pdy ? (int)M : 0, (int)N, dz_ws, np}, {x, ldx, sp.px ? (int)M : 0, (int)K, x_ws, kp}, {w, ldw, sp.pw && M > 0 ? (int)N : 0, (int)K, w_ws, kp}}, s)) return rc;
         px.a = dz, px.lda = lddz, px.b = sp.pw ? w_ws : w, px.ldb = sp.pw ? kp : ldw;      // dx[M, K] = dz[M, N] w[N, K]: sum over N
         px.M = (int)M, px.N = (int)K, px.K = (int)N;
         px.y = dx, px.ldy = lddx, px.res = dx_add, px.ldr = ldxa;
-        px.vec = K % 8 == 0 && rows16(dx, lddx, e) && (!dx_add || rows16(dx_add, ldxa, e));
         pw.a = dz, pw.lda = lddz, pw.b = sp.px ? x_ws : x, pw.ldb = sp.px ? kp : ldx;      // dw[N, K] = dz^T x: sum over M
-        pw.y = dw, pw.ldy = K, pw.vec = K % 8 == 0 && rows16(dw, K, e);
+        pw.y = dw, pw.ldy = K;
         if (dx && dw && M > 0) return linear_gradients<T>(pw, px, slabs, s);
         if (dx && M > 0) return linear_product<T>(LIN_DX, px, slabs, s);
         if (dw) return linear_product<T>(LIN_DW, pw, slabs, s);

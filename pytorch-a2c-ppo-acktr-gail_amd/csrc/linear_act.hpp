@@ -14,7 +14,7 @@ struct LinArgs {
     const void *bias, *res;             // nullable
     void* pre;                          // slopes for the backward pass; nullable
     long ldr, ldp;
-    int act, vec;                       // vec: 16-byte stores of 8 columns are possible everywhere
+    int act;
     float* slabs;                       // split reduction: fp32 partial products [slices][M][N] instead of y
     int kslice;                         // k per slice (a multiple of the K step), K without a split
     int tiles_m, tiles_n;
@@ -25,6 +25,7 @@ struct LinArgs {
 };
 
 constexpr int KSTEP_BYTES = 128, MAX_SLICES = 32, SUM_BLOCKS = 256, SUM_COLS = 32, SUM_GROUPS = 8;
+constexpr long SUM_WIDE = 1 << 18;        // results from which the sum of slices takes 8 columns a thread
 
 static inline long up(long v, long a) { return (v + a - 1) / a * a; }
 static inline bool rows16(const void* p, long ld, long e) { return ((uintptr_t)p & 15) == 0 && ld * e % 16 == 0; }

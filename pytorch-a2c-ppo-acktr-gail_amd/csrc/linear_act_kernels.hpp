@@ -9,8 +9,8 @@
 
 namespace acktr {
 
-// act(v + bias) + res for 8 columns n.. of row m, and their stores.  v: the product.  Vector form: N is a multiple of 8 and all rows
-// start at 16 bytes; bias and residual are already in registers (b, r; zero where there is none).
+// act(v + bias) + res for 8 columns n.. of row m, and their stores (rows may start anywhere).  v: the product; bias and residual are
+// already in registers (b, r; zero where there is none).
 template <class T, int ACT, bool SLOPE>
 __device__ __forceinline__ void finish8(const LinArgs& p, int m, int n, float (&v)[8], const float (&b)[8], const vec_t<T, 8>& r, bool res) {
     typedef typename SlopeOf<T>::type ST;
@@ -28,10 +28,10 @@ __device__ __forceinline__ void finish8(const LinArgs& p, int m, int n, float (&
             z[i] = c;
         }
     }
-    *reinterpret_cast<vec_t<T, 8>*>((T*)p.y + (long)m * p.ldy + n) = y;
-    if (SLOPE) *reinterpret_cast<vec_t<ST, 8>*>((ST*)p.pre + (long)m * p.ldp + n) = z;
+    *reinterpret_cast<uvec_t<T, 8>*>((T*)p.y + (long)m * p.ldy + n) = y;
+    if (SLOPE) *reinterpret_cast<uvec_t<ST, 8>*>((ST*)p.pre + (long)m * p.ldp + n) = z;
 }
-// one value, for widths and rows of any alignment; b, r: bias and residual as above
+// one value, for the columns behind the last 8; b, r: bias and residual as above
 template <class T, int ACT, bool SLOPE>
 __device__ __forceinline__ void finish1(const LinArgs& p, int m, int n, float v, float b, T r, bool res) {
     typedef typename SlopeOf<T>::type ST;
@@ -61,8 +61,8 @@ template <class T>
 __device__ __forceinline__ void load_bias8(const LinArgs& p, int n, float (&b)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) b[i] = 0.f;
-    if (p.bias && n < p.N) {
-        const vec_t<T, 8> x = *reinterpret_cast<const vec_t<T, 8>*>((const T*)p.bias + n);
+    if (p.bias && n + 8 <= p.N) {
+        const vec_t<T, 8> x = *reinterpret_cast<const uvec_t<T, 8>*>((const T*)p.bias + n);
 #pragma unroll
         for (int i = 0; i < 8; ++i) b[i] = to_f32(x[i]);
     }
@@ -125,11 +125,13 @@ __device__ __forceinline__ void linear_tile(const LinArgs& p, int id, int slice,
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = lo[i], v[4 + i] = hi[i];
     };
-    // rows or widths that do not allow 8 columns at a time: a column a lane, so that a row's stores still lie side by side, eight rows
+    // the columns behind the last whole 8 (from `whole` on): a column a lane, so that a row's stores still lie side by side, eight rows
     // in flight
+    const int whole = p.N & ~7;
     constexpr int LA = WTN < 64 ? WTN : 64, RP1 = 64 / LA, CG = WTN / LA, U = 8;
     static_assert(P * 16 / RP1 % U == 0, "whole groups of rows");
-    auto finish_any = [&](auto act, auto slope, auto slab) __attribute__((always_inline)) {
+    auto finish_rest = [&](auto act, auto slope, auto slab) __attribute__((always_inline)) {
+        if (whole == p.N || wn + WTN <= whole || wn >= p.N) return;           // (uniform)
         constexpr int ACT = decltype(act)::value;
         constexpr bool SLOPE = decltype(slope)::value, SLAB = decltype(slab)::value;
         const bool res = !SLAB && p.res;
@@ -139,7 +141,7 @@ __device__ __forceinline__ void linear_tile(const LinArgs& p, int id, int slice,
 #pragma unroll 1
             for (int k = 0; k < CG * (P * 16 / RP1 / U); ++k) {
                 const int c = (k % CG) * LA + lane % LA, r0 = (k / CG) * U * RP1 + lane / LA, nn = wn + c;
-                const bool in = nn < p.N;
+                const bool in = nn >= whole && nn < p.N;
                 const float b = !SLAB && FULL && p.bias && in ? to_f32(((const T*)p.bias)[nn]) : 0.f;
                 float v[U];
                 T rr[U];
@@ -161,7 +163,7 @@ __device__ __forceinline__ void linear_tile(const LinArgs& p, int id, int slice,
         }
     };
     using std::integral_constant;
-    if (p.slabs && p.vec) {
+    if (p.slabs) {
 #pragma unroll 1
         for (int base = 0; base < G::MI; base += P) {
             spill(base);
@@ -170,21 +172,14 @@ __device__ __forceinline__ void linear_tile(const LinArgs& p, int id, int slice,
                 const int m = wm + base * 16 + k * RPI + lr;
                 float v[8];
                 fetch8(k, v);
-                if (m >= p.M || n >= p.N) continue;
+                if (m >= p.M || n + 8 > p.N) continue;
                 float* s = p.slabs + ((long)slice * p.M + m) * p.N + n;
-                *reinterpret_cast<f32v4*>(s) = f32v4{v[0], v[1], v[2], v[3]};
-                *reinterpret_cast<f32v4*>(s + 4) = f32v4{v[4], v[5], v[6], v[7]};
+                *reinterpret_cast<uvec_t<float, 4>*>(s) = f32v4{v[0], v[1], v[2], v[3]};
+                *reinterpret_cast<uvec_t<float, 4>*>(s + 4) = f32v4{v[4], v[5], v[6], v[7]};
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
-        return;
-    }
-    if (p.slabs) return finish_any(integral_constant<int, ACKTR_ACT_NONE>{}, std::false_type{}, std::true_type{});
-    if (!p.vec) {
-        auto apart = [&](auto act, auto slope) __attribute__((always_inline)) { finish_any(act, slope, std::false_type{}); };
-        if constexpr (FULL) with_act(p, apart);
-        else apart(integral_constant<int, ACKTR_ACT_NONE>{}, std::false_type{});
-        return;
+        return finish_rest(integral_constant<int, ACKTR_ACT_NONE>{}, std::false_type{}, std::true_type{});
     }
     auto finish = [&](auto act, auto slope) __attribute__((always_inline)) {
         constexpr int ACT = decltype(act)::value;
@@ -200,7 +195,7 @@ __device__ __forceinline__ void linear_tile(const LinArgs& p, int id, int slice,
 #pragma unroll
             for (int k = 0; k < IT; ++k) {
                 const int m = wm + base * 16 + k * RPI + lr;
-                if (res && m < p.M && n < p.N) r[k] = *reinterpret_cast<const vec_t<T, 8>*>((const T*)p.res + (long)m * p.ldr + n);
+                if (res && m < p.M && n + 8 <= p.N) r[k] = *reinterpret_cast<const uvec_t<T, 8>*>((const T*)p.res + (long)m * p.ldr + n);
             }
         };
         residual(0);
@@ -216,10 +211,11 @@ __device__ __forceinline__ void linear_tile(const LinArgs& p, int id, int slice,
                 const int m = wm + base * 16 + k * RPI + lr;
                 float v[8];
                 fetch8(k, v);
-                if (m < p.M && n < p.N) finish8<T, ACT, SLOPE>(p, m, n, v, b, now[k], res);
+                if (m < p.M && n + 8 <= p.N) finish8<T, ACT, SLOPE>(p, m, n, v, b, now[k], res);
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
+        finish_rest(act, slope, std::false_type{});
     };
     if constexpr (FULL) with_act(p, finish);
     else finish(std::integral_constant<int, ACKTR_ACT_NONE>{}, std::false_type{});
@@ -283,7 +279,9 @@ __global__ __launch_bounds__(SUM_COLS * SUM_GROUPS) void bias_kernel(const LinAr
 }
 
 // Sum of the slices of a split reduction in slice order, then the epilogue: bound by reading them (4 slices of
-// 2048 x 2048 13 us, 6.5 TB/s out of the caches that the tiles left them in).  V: columns a thread, 8 where rows allow it, else 1.
+// 2048 x 2048 13 us, 6.5 TB/s out of the caches that the tiles left them in).  V: columns a thread; 8
+// halve the accesses of a large matrix, one a thread gives a small one more loads in flight (with 8 and 1: 2048 x 2048 13.9 and 16.5 us,
+// 512 x 512 4.0 and 4.0, 256 x 256 5.3 and 4.4, 17 x 847 of 32 slices 22 and 4.6).
 template <class T, int V>
 __global__ __launch_bounds__(256) void linear_slabs_kernel(const LinArgs p, int slices) {
     const int groups = p.N / V;
@@ -308,7 +306,7 @@ __global__ __launch_bounds__(256) void linear_slabs_kernel(const LinArgs p, int 
             float b[8];
             load_bias8<T>(p, n, b);
             vec_t<T, 8> r;
-            if (p.res) r = *reinterpret_cast<const vec_t<T, 8>*>((const T*)p.res + (long)m * p.ldr + n);
+            if (p.res) r = *reinterpret_cast<const uvec_t<T, 8>*>((const T*)p.res + (long)m * p.ldr + n);
             with_act(p, [&](auto act, auto slope) { finish8<T, decltype(act)::value, decltype(slope)::value>(p, m, n, v, b, r, p.res); });
         } else {
             const float b = p.bias ? to_f32(((const T*)p.bias)[n]) : 0.f;
@@ -348,8 +346,9 @@ static int launch_tile(LinArgs& p, const Plan& pl, hipStream_t s) {
 
 template <class T>
 static int sum_slices(const LinArgs& p, int slices, hipStream_t s) {
-    if (p.vec) linear_slabs_kernel<T, 8><<<min(cdiv((long)p.M * (p.N / 8), 256), 2048), 256, 0, s>>>(p, slices);
-    else linear_slabs_kernel<T, 1><<<min(cdiv((long)p.M * p.N, 256), 4096), 256, 0, s>>>(p, slices);
+    const long count = (long)p.M * p.N;
+    if (p.N % 8 == 0 && count >= SUM_WIDE) linear_slabs_kernel<T, 8><<<min(cdiv(count / 8, 256), 2048), 256, 0, s>>>(p, slices);
+    else linear_slabs_kernel<T, 1><<<min(cdiv(count, 256), 4096), 256, 0, s>>>(p, slices);
     ACKTR_LAUNCH_CHECK();
     return 0;
 }
