@@ -596,6 +596,14 @@ int acktr_gated_scan_bwd(const void* dout, long dout_t, long dout_n, const void*
 int acktr_gated_scan_step(const void* gate, long gate_n, const void* value, long value_n, float* state, const float* masks, void* out,
                           long out_n, long N, long H, int dtype, void* stream);
 
+/* One step of the whole core, for acting: (gate | value) = x[N, I] w_in[2H, I]^T + b_in, the step above from `state` to `state_out` (fp32
+ * [N, H]; the same array, or apart), y[N, H] = h + silu(h w_out[H, H]^T + b_out) with h the new state, rounded.  Weights are dense,
+ * biases nullable.  The results are those of the single entries.  workspace: 256-byte aligned. */
+long acktr_gated_core_step_workspace_bytes(const void* x, long ldx, const void* w_in, const void* w_out, long N, long I, long H, int dtype);
+int acktr_gated_core_step(const void* x, long ldx, const void* w_in, const void* b_in, const void* w_out, const void* b_out,
+                          const float* state, float* state_out, const float* masks, void* y, long ldy, long N, long I, long H, int dtype,
+                          void* workspace, long workspace_bytes, void* stream);
+
 /* AdamW over many tensors (decoupled weight decay; csrc/adamw.hip has the formulas).  `tensors` (device array) lists them;
  * `chunks` (device array of {tensor, chunk number}, nchunks pairs) cuts each into pieces of acktr_adamw_chunk() elements.  Moments lie
  * in mom1 / mom2, tensor k's from element tensors[k].state on (a multiple of acktr_adamw_block(), with room for its length rounded

@@ -197,6 +197,8 @@ _PROTOS = {
     'acktr_gated_scan_workspace_bytes': (c_l, [c_l, c_l, c_l, c_i]),
     'acktr_gated_scan_fwd': (c_i, [c_p, c_l, c_l] * 2 + [c_p, c_p] + [c_p, c_l, c_l] + [c_p, c_p] + [c_l] * 3 + [c_i, c_p, c_l, c_p]),
     'acktr_gated_scan_bwd': (c_i, [c_p, c_l, c_l] * 3 + [c_p] * 4 + [c_p, c_l, c_l] * 2 + [c_p] + [c_l] * 3 + [c_i, c_p, c_l, c_p]),
+    'acktr_gated_core_step_workspace_bytes': (c_l, [c_p, c_l, c_p, c_p, c_l, c_l, c_l, c_i]),
+    'acktr_gated_core_step': (c_i, [c_p, c_l] + [c_p] * 7 + [c_p, c_l] + [c_l] * 3 + [c_i, c_p, c_l, c_p]),
     'acktr_gated_scan_step': (c_i, [c_p, c_l, c_p, c_l, c_p, c_p, c_p, c_l, c_l, c_l, c_i, c_p]),
     'acktr_adamw_chunk': (c_i, []),
     'acktr_adamw_block': (c_i, []),

@@ -173,12 +173,10 @@ def gated_forward(policy, a, x_seq, hxs, masks, infer=False):
     H = core.hidden_size
     hxs, masks, T, N = rnn_rows(x_seq, hxs, masks, H)
     (w_in, b_in), (w_out, b_out) = _wb(core.in_proj), _wb(core.out_proj)
-    proj = ops.linear_act_fwd(x_seq, w_in, b_in)                       # all steps at once: [T*N, 2H]
     if infer and T == 1:
-        state = hxs.clone()
-        h = ops.gated_scan_step(proj[:, :H], proj[:, H:], state, masks)
-        a.gru_out, a.hxs_out = ops.linear_act_fwd(h, w_out, b_out, act='silu', residual=h), state
+        a.gru_out, a.hxs_out = ops.gated_core_step(x_seq, w_in, b_in, w_out, b_out, hxs, masks)
         return a.gru_out
+    proj = ops.linear_act_fwd(x_seq, w_in, b_in)                       # all steps at once: [T*N, 2H]
     p3 = proj.view(T, N, 2 * H)
     m2 = masks.view(T, N)
     h3, last, saved = ops.gated_scan_fwd(p3[..., :H], p3[..., H:], hxs, m2, save=True)

@@ -117,7 +117,4 @@ class GatedCore(nn.Module):
     @torch.no_grad()
     def step(self, x, state, masks=None):
         """One step for acting: x [N, input_size]; `state` is updated in place; returns y [N, hidden_size]."""
-        H = self.hidden_size
-        proj = ops.linear_act_fwd(x, self.in_proj.weight, self.in_proj.bias)
-        h = ops.gated_scan_step(proj[:, :H], proj[:, H:], state, masks)
-        return ops.linear_act_fwd(h, self.out_proj.weight, self.out_proj.bias, act='silu', residual=h)
+        return ops.gated_core_step(x, self.in_proj.weight, self.in_proj.bias, self.out_proj.weight, self.out_proj.bias, state, masks, state)[0]

@@ -804,3 +804,31 @@ def gated_scan_step(gate, value, state, masks=None, out=None):
         _apart(state, 'state', (gate, value, masks), 'gated_scan_step')
     _launch(_hip.lib().acktr_gated_scan_step, at, 'gated_scan_step', 10.0 * N * H, pg, gn, pv, vn, ps, pm, po, on, N, H, code)
     return out
+
+
+def gated_core_step(x, w_in, b_in, w_out, b_out, state, masks=None, state_out=None):
+    """(y, state_out) of one step of the gated core (gated.GatedCore): x [N, I], w_in [2H, I], w_out [H, H] of one type, biases [2H] and
+    [H] or None, state [N, H] fp32, masks [N] or [N, 1] fp32 or None.  state_out: receives the new state and may be `state` itself
+    (default: a new tensor).  The same results as linear_act_fwd, gated_scan_step and linear_act_fwd, in one call."""
+    code = _dtype_code(x, 'x')
+    if x.dim() != 2 or w_in.dim() != 2 or w_in.shape[1] != x.shape[1] or x.shape[1] < 1 or w_in.shape[0] < 2 or w_in.shape[0] % 2:
+        raise RuntimeError('gated_core_step: x [N, I] and w_in [2H, I] expected, got %s and %s' % (tuple(x.shape), tuple(w_in.shape)))
+    (N, I), H, dt, at = x.shape, w_in.shape[0] // 2, x.dtype, x.get_device()
+    px, ldx = _rows(x, 'x', x.shape, dt, at)
+    pi, po = _dense(w_in, 'w_in', (2 * H, I), dt, at), _dense(w_out, 'w_out', (H, H), dt, at)
+    bi = _vec(b_in, 'b_in', 2 * H, dt, at) if b_in is not None else None
+    bo = _vec(b_out, 'b_out', H, dt, at) if b_out is not None else None
+    ps = _dense(state, 'state', (N, H), f32, at)
+    pm = _masks(masks, (N,), at)
+    if state_out is None:
+        state_out = state.new_empty((N, H))
+    else:
+        pq = _dense(state_out, 'state_out', (N, H), f32, at)
+        _apart(state_out, 'state_out', (x, w_in, b_in, w_out, b_out, masks, None if pq == ps else state), 'gated_core_step')
+    y = x.new_empty((N, H))
+    L = _hip.lib()
+    nb = L.acktr_gated_core_step_workspace_bytes(px, ldx, pi, po, N, I, H, code)
+    ws = _scratch(nb, x, 'acktr_gated_core_step')
+    _launch(L.acktr_gated_core_step, at, 'gated_core_step', 4.0 * N * H * I + 2.0 * N * H * H, px, ldx, pi, bi, po, bo, ps, state_out.data_ptr(),
+            pm, y.data_ptr(), H, N, I, H, code, ws.data_ptr(), nb)
+    return y, state_out

@@ -429,15 +429,15 @@ __global__ __launch_bounds__(NW * 64) void scan_bwd_kernel(const ScanArgs p) {
 // --------------------------------------------------------------------------------------------------------- one token
 // A channel a value, 8 bytes of gate and value a lane where rows allow it.  32 x 512 is one launch of latency.
 template <class T, int V>
-__global__ __launch_bounds__(256) void scan_step_kernel(const void* gate, long gn, const void* value, long vn, float* state, const float* masks,
-                                                        void* out, long on, int N, int H) {
+__global__ __launch_bounds__(256) void scan_step_kernel(const void* gate, long gn, const void* value, long vn, const float* from, float* to,
+                                                        const float* masks, void* out, long on, int N, int H) {
     typedef vec_t<T, V> vv;
     typedef vec_t<float, V> fv;
     const long c = ((long)blockIdx.x * 256 + threadIdx.x) * V;
     if (c >= (long)N * H) return;
     const int n = (int)(c / H), j = (int)(c - (long)n * H);
     const vv g = *reinterpret_cast<const vv*>((const T*)gate + n * gn + j), v = *reinterpret_cast<const vv*>((const T*)value + n * vn + j);
-    fv h = *reinterpret_cast<fv*>(state + c);
+    fv h = *reinterpret_cast<const fv*>(from + c);
     const float m = masks ? masks[n] : 1.f;
     vv o;
 #pragma unroll
@@ -447,7 +447,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(const void* gate, long g
         h[i] = f * cut_mul(m, h[i]) + nf * to_f32(v[i]);
         o[i] = from_f32<T>(h[i]);
     }
-    *reinterpret_cast<fv*>(state + c) = h;
+    *reinterpret_cast<fv*>(to + c) = h;
     *reinterpret_cast<vv*>((T*)out + n * on + j) = o;
 }
 // dst = src or 0: the states of a sequence of no steps
@@ -607,21 +607,64 @@ extern "C" int acktr_gated_scan_bwd(const void* dout, long dt, long dn, const vo
     return with_dtype(dtype, [&](auto t) -> int { return scan_run<decltype(t), true>(a, p, far, s); });
 }
 
+// one step from state `from` to state `to` (the same one, or apart)
+static int scan_step(const void* gate, long gn, const void* value, long vn, const float* from, float* to, const float* masks, void* out, long on,
+                     long N, long H, int dtype, hipStream_t s) {
+    return with_dtype(dtype, [&](auto t) -> int {
+        typedef decltype(t) T;
+        constexpr int W = 8 / sizeof(T);
+        auto rows8 = [](const void* q, long sn) { return ((uintptr_t)q & 7) == 0 && sn * (long)sizeof(T) % 8 == 0; };
+        const bool wide = H % W == 0 && rows8(gate, gn) && rows8(value, vn) && rows8(out, on) && (((uintptr_t)from | (uintptr_t)to) & 15) == 0;
+        if (wide) scan_step_kernel<T, W><<<cdiv(N * H, 256 * W), 256, 0, s>>>(gate, gn, value, vn, from, to, masks, out, on, (int)N, (int)H);
+        else scan_step_kernel<T, 1><<<cdiv(N * H, 256), 256, 0, s>>>(gate, gn, value, vn, from, to, masks, out, on, (int)N, (int)H);
+        ACKTR_LAUNCH_CHECK();
+        return 0;
+    });
+}
+
 extern "C" int acktr_gated_scan_step(const void* gate, long gn, const void* value, long vn, float* state, const float* masks, void* out, long on,
                                      long N, long H, int dtype, void* stream) {
     if (int rc = scan_check(1, N, H, dtype)) return rc;
     if (N * H == 0) return 0;
     ACKTR_ARG(gate && value && state && out, "gated_scan_step: gate, value, state and out are required");
     ACKTR_ARG(gn >= 0 && vn >= 0 && on >= 0, "gated_scan_step: negative stride");
-    hipStream_t s = (hipStream_t)stream;
-    return with_dtype(dtype, [&](auto t) -> int {
-        typedef decltype(t) T;
-        constexpr int W = 8 / sizeof(T);
-        auto rows8 = [](const void* q, long sn) { return ((uintptr_t)q & 7) == 0 && sn * (long)sizeof(T) % 8 == 0; };
-        const bool wide = H % W == 0 && rows8(gate, gn) && rows8(value, vn) && rows8(out, on) && ((uintptr_t)state & 15) == 0;
-        if (wide) scan_step_kernel<T, W><<<cdiv(N * H, 256 * W), 256, 0, s>>>(gate, gn, value, vn, state, masks, out, on, (int)N, (int)H);
-        else scan_step_kernel<T, 1><<<cdiv(N * H, 256), 256, 0, s>>>(gate, gn, value, vn, state, masks, out, on, (int)N, (int)H);
-        ACKTR_LAUNCH_CHECK();
-        return 0;
-    });
+    return scan_step(gate, gn, value, vn, state, state, masks, out, on, N, H, dtype, (hipStream_t)stream);
+}
+
+// One step of the whole core.  Its three launches are those of the single entries; a caller that acts, and waits for every step, saves
+// the host's work for two calls.
+struct CoreSpace { long h, scratch, bytes; };
+static int core_space(const void* x, long ldx, const void* w_in, const void* w_out, long N, long I, long H, int dtype, CoreSpace& sp) {
+    if (int rc = scan_check(1, N, H, dtype)) return rc;
+    const long e = elem_bytes(dtype);
+    const long a = acktr_linear_act_fwd_workspace_bytes(x, ldx, w_in, I, N, 2 * H, I, dtype);
+    const long b = acktr_linear_act_fwd_workspace_bytes(nullptr, H, w_out, H, N, H, H, dtype);        // (the states start at 256 bytes)
+    if (a < 0 || b < 0) return -1;
+    auto up256 = [](long v) { return (v + 255) / 256 * 256; };
+    sp.h = up256(2 * N * H * e);
+    sp.scratch = sp.h + up256(N * H * e);
+    sp.bytes = sp.scratch + max(a, b);
+    return 0;
+}
+extern "C" long acktr_gated_core_step_workspace_bytes(const void* x, long ldx, const void* w_in, const void* w_out, long N, long I, long H, int dtype) {
+    CoreSpace sp;
+    return core_space(x, ldx, w_in, w_out, N, I, H, dtype, sp) ? -1 : sp.bytes;
+}
+extern "C" int acktr_gated_core_step(const void* x, long ldx, const void* w_in, const void* b_in, const void* w_out, const void* b_out,
+                                     const float* state, float* state_out, const float* masks, void* y, long ldy, long N, long I, long H,
+                                     int dtype, void* workspace, long workspace_bytes, void* stream) {
+    CoreSpace sp;
+    if (int rc = core_space(x, ldx, w_in, w_out, N, I, H, dtype, sp)) return rc;
+    if (N == 0) return 0;
+    ACKTR_ARG(x && w_in && w_out && state && state_out && y, "gated_core_step: x, the weights, both states and y are required");
+    ACKTR_ARG(workspace && ((uintptr_t)workspace & 255) == 0 && workspace_bytes >= sp.bytes,
+              "gated_core_step: workspace of %ld bytes, %ld with 256-byte alignment are needed", workspace_bytes, sp.bytes);
+    ACKTR_ARG(ldx >= I && ldx < (1 << 21) && ldy >= H && ldy < (1 << 21),
+              "gated_core_step: row strides must be at least the rows' lengths and below 2^21 (got %ld, %ld)", ldx, ldy);
+    char *proj = (char*)workspace, *h = proj + sp.h, *scratch = proj + sp.scratch;
+    const long left = workspace_bytes - sp.scratch, e = elem_bytes(dtype);
+    if (int rc = acktr_linear_act_fwd(x, ldx, w_in, I, b_in, nullptr, 0, proj, 2 * H, nullptr, 0, N, 2 * H, I, dtype, ACKTR_ACT_NONE, scratch, left, stream))
+        return rc;
+    if (int rc = scan_step(proj, 2 * H, proj + H * e, 2 * H, state, state_out, masks, h, H, N, H, dtype, (hipStream_t)stream)) return rc;
+    return acktr_linear_act_fwd(h, H, w_out, H, b_out, h, H, y, ldy, nullptr, 0, N, H, H, dtype, ACKTR_ACT_SILU, scratch, left, stream);
 }

@@ -84,6 +84,62 @@ def test_steps_are_the_sequence():
     assert float((state - last).abs().max()) < 64 * 2.0 ** -24 * 8
 
 
+@pytest.mark.parametrize('dt', [F32, BF, HF])
+@pytest.mark.parametrize('N,I,H', [(32, 512, 512), (1, 8, 16), (5, 11, 23), (3, 1, 1), (200, 40, 64), (0, 8, 8)])
+def test_one_call_is_its_three_parts(dt, N, I, H):
+    from a2c_ppo_acktr import ops
+    wide = rnd(1, N, I + 3, dtype=dt)
+    w_in, b_in = rnd(2, 2 * H, I, scale=I ** -0.5, dtype=dt), rnd(3, 2 * H, dtype=dt)
+    w_out, b_out = rnd(4, H, H, scale=H ** -0.5, dtype=dt), rnd(5, H, dtype=dt)
+    for x in (wide[:, :I], wide[:, 3:], wide[:, :I].contiguous()):
+        for m in (None, (rnd(6, N, 1) < 0.5).float()):
+            state = rnd(7, N, H)
+            want_state = state.clone()
+            proj = ops.linear_act_fwd(x, w_in, b_in)
+            h = ops.gated_scan_step(proj[:, :H], proj[:, H:], want_state, m)
+            want = ops.linear_act_fwd(h, w_out, b_out, act='silu', residual=h)
+            before = state.clone()
+            y, new = ops.gated_core_step(x, w_in, b_in, w_out, b_out, state, m)
+            assert torch.equal(y, want) and torch.equal(new, want_state) and torch.equal(state, before)
+            y, same = ops.gated_core_step(x, w_in, b_in, w_out, b_out, state, m, state)
+            assert same is state and torch.equal(y, want) and torch.equal(state, want_state)
+
+
+def test_one_call_captured():
+    from a2c_ppo_acktr import gated, ops
+    core = gated.GatedCore(24, 40).to(DEV, BF)
+    x, m, state = torch.zeros(6, 24, dtype=BF, device=DEV), torch.ones(6, device=DEV), torch.zeros(6, 40, device=DEV)
+    core.step(x, state.clone(), m)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with ops.graph_capture(g):
+        y = core.step(x, state, m)
+    state.zero_()
+    eager = torch.zeros_like(state)
+    for k in range(4):
+        x.copy_(rnd(k, 6, 24, dtype=BF))
+        m.copy_((rnd(k + 9, 6) < 1.0).float())
+        want = core.step(x, eager, m)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and torch.equal(state, eager), k
+
+
+def test_one_call_refusals():
+    from a2c_ppo_acktr import ops
+    N, I, H = 4, 8, 16
+    ok = dict(x=rnd(1, N, I), w_in=rnd(2, 2 * H, I), b_in=rnd(3, 2 * H), w_out=rnd(4, H, H), b_out=rnd(5, H), state=rnd(6, N, H),
+              masks=torch.ones(N, device=DEV))
+    ops.gated_core_step(**ok)
+    wide = torch.zeros(2 * N, H, device=DEV)
+    for kw in (dict(x=rnd(1, N, I + 1)), dict(x=rnd(1, N, I, dtype=BF)), dict(w_in=rnd(2, 2 * H + 1, I)), dict(w_in=rnd(2, I, 2 * H).t()),
+               dict(b_in=rnd(3, H)), dict(w_out=rnd(4, H, H + 1)), dict(b_out=rnd(5, H).half()), dict(state=rnd(6, N, H, dtype=BF)),
+               dict(state=rnd(6, N + 1, H)), dict(masks=torch.ones(N, 2, device=DEV)), dict(masks=torch.ones(N, dtype=torch.bool, device=DEV)),
+               dict(state=wide[:N], state_out=wide[1:N + 1]), dict(state_out=ok['w_out'][:N]), dict(x=ok['x'].cpu()), dict(state=ok['state'].cpu())):
+        with pytest.raises(RuntimeError):
+            ops.gated_core_step(**dict(ok, **kw))
+
+
 def test_forward_and_backward_captured():
     """both passes recorded into a graph by autograd; replays follow new inputs and stay right beside eager work"""
     from a2c_ppo_acktr import gated, ops

@@ -56,6 +56,18 @@ def test_scan_entry_arguments():
     assert L.acktr_gated_scan_workspace_bytes(4, 2, 0, 1) == -1
 
 
+def test_core_step_entry_arguments():
+    L, one = lib(), ctypes.c_void_p(256)
+    call = lambda x=one, ldx=8, w=one, s=one, so=one, y=one, ldy=16, N=4, I=8, H=16, dt=1, ws=one, nb=1 << 20: L.acktr_gated_core_step(
+        x, ldx, w, None, one, None, s, so, None, y, ldy, N, I, H, dt, ws, nb, None)
+    for kw in (dict(x=None), dict(w=None), dict(s=None), dict(so=None), dict(y=None), dict(ldx=7), dict(ldy=15), dict(N=-1), dict(I=0), dict(H=0),
+               dict(H=1 << 20), dict(dt=3), dict(ws=None), dict(ws=ctypes.c_void_p(272)), dict(nb=100)):
+        assert call(**kw) == -1 and err(), kw
+    assert call(N=0) == 0
+    assert L.acktr_gated_core_step_workspace_bytes(one, 8, one, one, 4, 8, 0, 1) == -1
+    assert L.acktr_gated_core_step_workspace_bytes(one, 8, one, one, 4, 8, 16, 1) >= 4 * 16 * 2 * 3
+
+
 def test_adamw_entry_arguments():
     L, one = lib(), ctypes.c_void_p(256)
     call = lambda st=one, n=4, m=one, sc=one, bits=32, t=one: L.acktr_adamw_step(st, t, one, n, m, one, sc, bits, 0, None)
