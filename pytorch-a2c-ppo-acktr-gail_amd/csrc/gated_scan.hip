@@ -502,9 +502,13 @@ static void scan_launch_nw(const ScanArgs& a, const ScanPlan& p, hipStream_t s) 
         if constexpr (BWD) scan_bwd_kernel<T, V, NW, MODE, AGG><<<grid, NW * 64, 0, s>>>(a);
         else scan_fwd_kernel<T, V, NW, MODE, AGG><<<grid, NW * 64, 0, s>>>(a);
     };
-    if (p.nw == 1) go(std::integral_constant<int, 1>{});
-    else if (p.nw == 4) go(std::integral_constant<int, 4>{});
-    else go(std::integral_constant<int, 8>{});
+    if constexpr (AGG) {                                     // a time split has more than 256 steps and few tiles: always 8 waves
+        go(std::integral_constant<int, 8>{});
+    } else {
+        if (p.nw == 1) go(std::integral_constant<int, 1>{});
+        else if (p.nw == 4) go(std::integral_constant<int, 4>{});
+        else go(std::integral_constant<int, 8>{});
+    }
 }
 template <class T, bool BWD, bool AGG>
 static void scan_launch(const ScanArgs& a, const ScanPlan& p, bool far, hipStream_t s) {

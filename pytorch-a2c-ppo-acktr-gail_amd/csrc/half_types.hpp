@@ -7,7 +7,6 @@
 namespace acktr {
 
 typedef float f32v4 __attribute__((ext_vector_type(4)));
-typedef float f32v8 __attribute__((ext_vector_type(8)));
 
 template <class T, int N>
 struct VecOf { typedef T type __attribute__((ext_vector_type(N))); };
