@@ -36,10 +36,12 @@ __device__ __forceinline__ float cut_mul(float a, float x) { return acktr_mul_le
 
 // f = 1 / (1 + e^-x) and 1 - f = e^-x f, both relative to their own size.  x is held above -87, where f is fp32's smallest normal number
 // and e^-x still finite (maximum() keeps a NaN).  ACC (fp32 storage): the product x log2(e) is carried with its rounding error,
-// without which e^-x is off by |x| 6e-8 -- nothing beside the rounding of a 16-bit x.
+// without which e^-x is off by |x| 6e-8 -- nothing beside the rounding of a 16-bit x.  That error is infinity - infinity where the
+// product overflows, so there x is held below 200 too, where e^-x is 0 already.
 template <bool ACC>
 __device__ __forceinline__ void gate_of(float x, float& f, float& nf) {
     x = __builtin_elementwise_maximum(x, -87.f);
+    if (ACC) x = __builtin_elementwise_minimum(x, 200.f);
     const float p = x * -LOG2E;
     float e = __builtin_amdgcn_exp2f(p);
     if (ACC) {

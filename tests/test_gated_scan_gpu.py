@@ -99,6 +99,29 @@ def test_extreme_gates():
         check(t, (r, tol + 1.7e-38 * max(2 * top, 1.0) * max(back, 1.0)), name)
 
 
+@pytest.mark.parametrize('dt', [BF, HF, F32])
+@pytest.mark.parametrize('T,N,H', [(90, 2, 16), (3000, 1, 8)])
+def test_gates_without_bound(T, N, H, dt):
+    """infinite gates, and finite ones whose product with log2(e) has no fp32 value: held open (the state stays) or shut"""
+    from a2c_ppo_acktr import ops
+    g, v, m, h0, dout, dl = inputs(T, N, H, dt)
+    g, inf, most = g.clone(), float('inf'), 65504.0 if dt == HF else 3e38
+    g[::5, :, 0], g[::7, :, 1], g[::3, :, 2], g[::4, :, 3] = inf, -inf, most, -most
+    g[T // 2, :, 4], g[T // 2 + 1, :, 4], g[:, :, 5] = inf, -inf, inf
+    out, fin, saved = ops.gated_scan_fwd(g, v, h0, m, save=True)
+    dg, dv, dh0 = ops.gated_scan_bwd(dout, g, v, h0, m, saved=saved, dlast=dl)
+    ref = scan64(g, v, h0, m, dout, dl)
+    # as in test_extreme_gates: a shut gate is taken as -87, f = 1.7e-38
+    top, back = max(float(h0.abs().max()), float(v.abs().max())), float((dout.abs().float().sum(0) + dl.abs()).max())
+    for name, t in (('out', out), ('last', fin), ('dgate', dg), ('dvalue', dv), ('dh0', dh0)):
+        r, tol = ref[name]
+        check(t, (r, tol + 1.7e-38 * max(2 * top, 1.0) * max(back, 1.0)), name)
+    state = h0.clone()
+    for t in range(12):
+        y = ops.gated_scan_step(g[t], v[t], state, m[t])
+        check(y, (ref['out'][0][t], ref['out'][1][t] + 1.7e-38 * 2 * top), t)
+
+
 def test_a_mask_of_zero_cuts_what_is_not_finite():
     from a2c_ppo_acktr import ops
     for T, N, H in ((200, 2, 16), (40, 1, 5), (3000, 1, 8)):
