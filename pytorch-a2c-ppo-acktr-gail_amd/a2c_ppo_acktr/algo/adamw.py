@@ -171,6 +171,7 @@ class AdamW(object):
         ops._launch(_hip.lib().acktr_adamw_step, self._dev.index, 'adamw_step', 20.0 * self._total, *self._fixed, self.mom1.data_ptr(),
                     self.mom2.data_ptr(), self.scales.data_ptr() if self.scales is not None else None, self.state_bits,
                     1 if self._hyper[5] > 0 else 0)
+        ops._written(self.params + self._copied)
         self.step_count += 1
 
     def moments(self):

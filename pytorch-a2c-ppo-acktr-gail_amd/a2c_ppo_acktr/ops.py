@@ -591,6 +591,11 @@ def _scratch(nbytes, like, what):
     return like.new_empty(nbytes, dtype=torch.uint8)
 
 
+# A kernel writes through a pointer, which autograd does not see: every tensor of the caller's that a call wrote is marked as changed, so
+# that a backward pass that still needs its old values raises instead of using the new ones.
+_written = torch.autograd.graph.increment_version
+
+
 def linear_act_fwd(x, w, bias=None, act=None, residual=None, out=None, pre=None):
     """out = act(x w^T + bias) + residual; x [M, K], w [N, K], bias [N], residual / out / pre [M, N], all of one type (bf16, fp16 or
     fp32), sums in fp32, rounded once.  act: None, 'relu', 'tanh', 'silu' or 'gelu'.  pre [M, N]: receives
@@ -620,6 +625,10 @@ def linear_act_fwd(x, w, bias=None, act=None, residual=None, out=None, pre=None)
     ws = _scratch(nb, x, 'acktr_linear_act_fwd') if nb else None
     _launch(L.acktr_linear_act_fwd, at, 'linear_act_fwd', 2.0 * M * N * K, px, ldx, pw, ldw, pb, pr, ldr, py, ldy, pz, ldz, M, N, K, code,
             act, ws.data_ptr() if nb else None, nb)
+    if pre is not None:
+        _written(pre)
+    if given:
+        _written(out)
     return out
 
 
@@ -661,6 +670,8 @@ def linear_act_bwd(dy, x, w, pre=None, act=None, dx=None, dw=None, db=None, need
     ws = _scratch(nb, dy, 'acktr_linear_act_bwd') if nb else None
     _launch(L.acktr_linear_act_bwd, at, 'linear_act_bwd', 2.0 * M * N * K * (bool(need_dx) + bool(need_dw)), pg, ldg, px, ldx, pw, ldw, pz, ldz,
             pa, lda, qx, ldq, qw, qb, M, N, K, code, act, ws.data_ptr() if nb else None, nb)
+    if given:
+        _written(given)
     return dx if need_dx else None, dw if need_dw else None, db if need_db else None
 
 
@@ -742,6 +753,8 @@ def gated_scan_fwd(gate, value, h0=None, masks=None, out=None, save=False):
     ws = _scratch(nb, gate, 'acktr_gated_scan_fwd') if nb else None
     _launch(L.acktr_gated_scan_fwd, at, 'gated_scan_fwd', 10.0 * T * N * H, *pg, *pv, ph, pm, *po, last.data_ptr(),
             saved.data_ptr() if save else None, T, N, H, code, ws.data_ptr() if nb else None, nb)
+    if given:
+        _written(out)
     return out, last, saved
 
 
@@ -780,6 +793,8 @@ def gated_scan_bwd(dout, gate, value, h0=None, masks=None, saved=None, dlast=Non
     ws = _scratch(nb, gate, 'acktr_gated_scan_bwd') if nb else None
     _launch(L.acktr_gated_scan_bwd, at, 'gated_scan_bwd', 20.0 * T * N * H, *pd, *pg, *pv, ph, pm, ps, pl, *qg, *qv,
             dh0.data_ptr() if need_dh0 else None, T, N, H, code, ws.data_ptr() if nb else None, nb)
+    if given:
+        _written(given)
     return dgate, dvalue, dh0
 
 
@@ -803,6 +818,7 @@ def gated_scan_step(gate, value, state, masks=None, out=None):
     if lo <= pg < hi or lo <= pv < hi or pg <= lo < pg + gn * N * 4 or pv <= lo < pv + vn * N * 4 or (pm and lo - 4 * N < pm < hi):
         _apart(state, 'state', (gate, value, masks), 'gated_scan_step')
     _launch(_hip.lib().acktr_gated_scan_step, at, 'gated_scan_step', 10.0 * N * H, pg, gn, pv, vn, ps, pm, po, on, N, H, code)
+    _written((state, out) if given else state)
     return out
 
 
@@ -820,7 +836,8 @@ def gated_core_step(x, w_in, b_in, w_out, b_out, state, masks=None, state_out=No
     bo = _vec(b_out, 'b_out', H, dt, at) if b_out is not None else None
     ps = _dense(state, 'state', (N, H), f32, at)
     pm = _masks(masks, (N,), at)
-    if state_out is None:
+    given = state_out is not None
+    if not given:
         state_out = state.new_empty((N, H))
     else:
         pq = _dense(state_out, 'state_out', (N, H), f32, at)
@@ -831,4 +848,6 @@ def gated_core_step(x, w_in, b_in, w_out, b_out, state, masks=None, state_out=No
     ws = _scratch(nb, x, 'acktr_gated_core_step')
     _launch(L.acktr_gated_core_step, at, 'gated_core_step', 4.0 * N * H * I + 2.0 * N * H * H, px, ldx, pi, bi, po, bo, ps, state_out.data_ptr(),
             pm, y.data_ptr(), H, N, I, H, code, ws.data_ptr(), nb)
+    if given:
+        _written(state_out)
     return y, state_out

@@ -203,6 +203,50 @@ def test_autograd_corners():
         linear_act(x, w, None, None, r)
 
 
+def test_writes_in_place_are_seen_by_autograd():
+    """a pending backward pass whose saved tensors were overwritten raises, as it does for torch's own in-place operations"""
+    from a2c_ppo_acktr import algo, ops
+    from a2c_ppo_acktr.gated import GatedCore, gated_scan, linear_act
+    core, x, state = GatedCore(8, 16).to(DEV), rnd(1, 5, 3, 8), rnd(2, 3, 16)
+    proj = rnd(3, 3, 32)
+    # the state that a sequence started from, by each of the calls that take a step
+    for step in (lambda s: core.step(x[0], s), lambda s: ops.gated_scan_step(proj[:, :16], proj[:, 16:], s),
+                 lambda s: ops.gated_core_step(x[0], core.in_proj.weight, core.in_proj.bias, core.out_proj.weight, core.out_proj.bias, rnd(4, 3, 16), None, s)):
+        y, _ = core(x, state)
+        with torch.no_grad():
+            step(state)
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            y.sum().backward()
+    # weights, and 16-bit copies of them
+    for w, opt in ((core.out_proj.weight, lambda w: algo.AdamW([w], lr=1e-3, grads=[torch.ones_like(w)])),
+                   (rnd(5, 4, 8, dtype=BF).requires_grad_(), lambda w: algo.AdamW([w.detach().float()], lr=1e-3, grads=[torch.ones_like(w)], copies=[w]))):
+        a = rnd(6, 7, w.shape[1], dtype=w.dtype).requires_grad_()
+        y = linear_act(a, w)
+        opt(w).step()
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            y.sum().backward()
+
+
+def test_given_outputs_are_marked_as_changed():
+    from a2c_ppo_acktr import ops
+    x, w, dy = rnd(1, 6, 8), rnd(2, 4, 8), rnd(3, 6, 4)
+    new = lambda *s: torch.zeros(*s, device=DEV)
+    out, pre, dx, dw, db = new(6, 4), new(6, 4), new(6, 8), new(4, 8), new(4)
+    ops.linear_act_fwd(x, w, act='tanh', out=out, pre=pre)
+    ops.linear_act_bwd(dy, x, w, pre=pre, act='tanh', dx=dx, dw=dw, db=db)
+    g, v, so, dg, dv = rnd(4, 5, 2, 8), rnd(5, 5, 2, 8), new(5, 2, 8), new(5, 2, 8), new(5, 2, 8)
+    _, _, saved = ops.gated_scan_fwd(g, v, out=so, save=True)
+    ops.gated_scan_bwd(v, g, v, saved=saved, dgate=dg, dvalue=dv)
+    state, one = new(2, 8), new(2, 8)
+    ops.gated_scan_step(g[0], v[0], state, out=one)
+    assert [t._version for t in (out, pre, dx, dw, db, so, dg, dv, state, one)] == [1] * 10
+    assert [t._version for t in (x, w, dy, g, v)] == [0] * 5
+    with torch.inference_mode():                             # (their versions are not counted)
+        s = torch.zeros(2, 8, device=DEV)
+        ops.gated_scan_step(g[0], v[0], s)
+    assert torch.equal(s, state)
+
+
 @pytest.mark.parametrize('bits', [32, 8])
 def test_mixed_precision_training(bits):
     """bf16 weights and gradients, fp32 masters, AdamW writing both: three steps of a small core against the same steps in 64 bits on
