@@ -610,7 +610,7 @@ int acktr_gated_core_step(const void* x, long ldx, const void* w_in, const void*
  * up to that): fp32 (bits = 32) or one byte each (bits = 8) with scales[2 * (element / block)] for mom1 and the odd entries for mom2.
  * `state` (device, acktr_adamw_state_bytes(), zeroed by the caller): first six doubles lr, beta1, beta2, eps, weight decay, clip norm;
  * then two int64: steps done, seed.  The call increments the steps.  clip != 0: gradients are scaled by
- * min(1, clip norm / (2-norm over all + 1e-6)) on the fly; they are only read.  Two calls on one `state` must not overlap. */
+ * min(1, clip norm / (2-norm over all + 1e-6)) on the fly (a clip norm of 0: not scaled); they are only read.  Two calls on one `state` must not overlap. */
 typedef struct acktr_adamw_tensor {
     void* p; const void* g; void* copy;          /* parameters (updated), gradients, 16-bit copy of the parameters (nullable) */
     long n; long state;

@@ -168,9 +168,11 @@ class AdamW(object):
     def step(self):
         """One step on all tensors: two launches."""
         self.prepare()
+        # (a captured step looks the clip norm up when it is replayed, so that one given or taken away later counts)
+        clip = self._hyper[5] > 0 or torch.cuda.is_current_stream_capturing()
         ops._launch(_hip.lib().acktr_adamw_step, self._dev.index, 'adamw_step', 20.0 * self._total, *self._fixed, self.mom1.data_ptr(),
                     self.mom2.data_ptr(), self.scales.data_ptr() if self.scales is not None else None, self.state_bits,
-                    1 if self._hyper[5] > 0 else 0)
+                    1 if clip else 0)
         ops._written(self.params + self._copied)
         self.step_count += 1
 

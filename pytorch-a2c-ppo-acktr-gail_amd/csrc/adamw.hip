@@ -39,8 +39,10 @@ __device__ __forceinline__ unsigned mix32(unsigned x) {
     return x ^ (x >> 16);
 }
 
-// min(1, c / (|g| + 1e-6)); a norm that is not a number stays one
+// min(1, c / (|g| + 1e-6)); a norm that is not a number stays one.  max_norm 0: no clip, whatever the norm (a captured step goes through
+// here with and without one)
 __device__ __forceinline__ float aw_coef(double sumsq, double max_norm) {
+    if (max_norm == 0.0) return 1.f;
     const double c = max_norm / (sqrt(sumsq) + 1e-6);
     return (float)(c > 1.0 ? 1.0 : c);
 }
@@ -109,7 +111,8 @@ __device__ __forceinline__ void st4(void* p, int dt, long i, long n, bool vec, c
 // Sum of squares of all gradients, in fp64.  SMALL: partial sums only (and the step is counted): the update's workgroups add them up.
 // Otherwise the last workgroup to finish adds them, in the same fixed order, and writes the step's scalars: thousands of workgroups
 // would read too much, while for a few hundred the chain of atomics costs more than the rest of the launch (13 us against 5 for the
-// 867 thousand parameters of the NatureCNN policy).  Bound by reading: 201 million fp32 gradients in 232 us (3.5 TB/s).
+// 867 thousand parameters of the NatureCNN policy).  Bound by reading: 201 million fp32 gradients in 232 us (3.5 TB/s).  Without a
+// clip norm at the time of the launch nothing is read.
 template <bool SMALL>
 __global__ __launch_bounds__(AW_THREADS) void adamw_norm_kernel(AwState* st, const acktr_adamw_tensor* tensors, const int2* chunks, int nchunks) {
     __shared__ double sm[16];
@@ -119,7 +122,7 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_norm_kernel(AwState* st, con
     if (SMALL && blockIdx.x == 0 && threadIdx.x == 0) st->step = st->step + 1;
     // two chunks at a time, and the table entries of the next two travel with their values
     const int step = gridDim.x;
-    int q = blockIdx.x;
+    int q = st->max_norm == 0.0 ? nchunks : blockIdx.x;
     const int none = nchunks - 1;
     int2 c0 = chunks[min(q, none)], c1 = chunks[min(q + step, none)];
     acktr_adamw_tensor t0 = tensors[c0.x], t1 = tensors[c1.x];

@@ -308,6 +308,36 @@ def test_captured_and_replayed(bits, clip):
     assert all(torch.equal(a, b) for a, b in zip(*runs))
 
 
+@pytest.mark.parametrize('bits', [32, 8])
+@pytest.mark.parametrize('shapes', [SHAPES, [(1500, 1501)]])
+def test_a_clip_norm_that_comes_or_goes_between_replays(bits, shapes):
+    """the captured step and eager steps agree whatever the clip norm was at the capture; few and many chunks"""
+    from a2c_ppo_acktr import algo, ops
+    for first in (None, 0.5):
+        runs = []
+        for captured in (False, True):
+            ps, gs, cs = make(shapes, cdt=BF)
+            opt = algo.AdamW(ps, grads=gs, copies=cs, state_bits=bits, max_grad_norm=first, seed=9, **HP)
+            opt.step()
+            if captured:
+                torch.cuda.synchronize()
+                g = torch.cuda.CUDAGraph()
+                with ops.graph_capture(g):
+                    opt.step()
+            for clip in (first, 0.25 if first is None else None, 0.125, None, 0.5):
+                opt.param_groups[0]['max_grad_norm'] = clip
+                if captured:
+                    opt.prepare()
+                    g.replay()
+                else:
+                    opt.step()
+                torch.cuda.synchronize()
+                runs.append([p.clone() for p in ps] + [c.clone() for c in cs if c is not None])
+            assert opt.steps_done() == 6
+        for k in range(5):
+            assert all(torch.equal(a, b) for a, b in zip(runs[k], runs[5 + k])), (first, k)
+
+
 def test_a_captured_step_follows_the_table():
     """gradients that were replaced by an eager step are what a step captured before reads afterwards; nothing points to freed memory"""
     from a2c_ppo_acktr import algo, ops
