@@ -63,7 +63,7 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(const T* __restrict__ dy, 
     typedef typename SlopeOf<T>::type ST;
     const int cg = threadIdx.x & 31, rg = threadIdx.x >> 5;
     const int n = (blockIdx.x * 32 + cg) * V, left = N - n;
-    const int r0 = blockIdx.y * rows_per, r1 = min(M, r0 + rows_per);
+    const int r0 = blockIdx.y * rows_per, r1 = r0 + min(M - r0, rows_per);          // (r0 + rows_per may pass 2^31)
     float s[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) s[i] = 0.f;

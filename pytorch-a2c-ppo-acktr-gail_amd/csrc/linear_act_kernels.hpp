@@ -97,7 +97,7 @@ __device__ __forceinline__ void linear_tile(const LinArgs& p, int id, int slice,
     const int rows_in = min(8, p.tiles_m - band * 8);
     const int tm = band * 8 + inband % rows_in, tn = inband / rows_in;
     const int m0 = tm * BM, n0 = tn * BN;
-    const int k0 = slice * p.kslice, k1 = min(p.K, k0 + p.kslice);
+    const int k0 = slice * p.kslice, k1 = k0 + min(p.K - k0, p.kslice);       // (k0 + kslice may pass 2^31 behind the last row)
 
     G g;
     g.run(p.a, p.lda, m0, p.M, p.b, p.ldb, n0, p.N, k0, k1, sm);

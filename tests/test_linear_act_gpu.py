@@ -231,6 +231,32 @@ def test_more_than_2_31_elements():
     assert not dx[:-tail].any()
 
 
+@pytest.mark.parametrize('act', ['none', 'relu'])
+def test_most_rows(act):
+    """gradients whose sums over rows end just below 2^31, in blocks and slices whose nominal ends pass 2^31"""
+    from a2c_ppo_acktr import ops
+    M, N, K, tail = (1 << 31) - 257, 8, 8, 3000
+    x, dy = torch.zeros(M, K, dtype=BF, device=DEV), torch.zeros(M, N, dtype=BF, device=DEV)
+    x[-tail:], dy[-tail:] = rnd(1, tail, K, dtype=BF), rnd(2, tail, N, dtype=BF)
+    x[:tail], dy[:tail] = rnd(3, tail, K, dtype=BF), rnd(4, tail, N, dtype=BF)
+    w = rnd(5, N, K, dtype=BF)
+    part = lambda t: torch.cat((t[:tail], t[-tail:]))
+    pre = slope = None
+    if act != 'none':
+        pre = torch.empty(M, N, dtype=BF, device=DEV)
+        y = ops.linear_act_fwd(x, w, act=act, pre=pre)
+        ry, ty, slope, ts = linear64(part(x), w, None, act)
+        check(part(y), (ry, ty), 'y')
+        del y
+    else:
+        slope, ts = torch.ones(2 * tail, N, dtype=torch.float64, device=DEV), torch.zeros(2 * tail, N, dtype=torch.float64, device=DEV)
+    _, dw, db = ops.linear_act_bwd(dy, x, w, pre=pre, act=act, need_dx=False)
+    # rows of zeros add nothing, however many: the tolerance is that of the rows that have values
+    _, gw, gb = linear_grads64(part(dy), part(x), w, slope, ts)
+    check(dw, gw, 'dw')
+    check(db, gb, 'db')
+
+
 def test_two_streams():
     from a2c_ppo_acktr import ops
     a, b = torch.cuda.Stream(), torch.cuda.Stream()
