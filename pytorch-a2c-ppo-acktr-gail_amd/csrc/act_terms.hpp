@@ -1,5 +1,5 @@
-// Activations and their derivatives, shared by the epilogues of linear_act.hip.  All in fp32; exp and reciprocal are the
-// hardware's base-2 exponential and reciprocal (1 ulp each), which leaves sigmoid, silu and tanh within ~4 ulp.
+// Activations and their derivatives, shared by the epilogues of linear_act.hip, and the exponential they share with gated_scan.hip.  All
+// in fp32; the hardware's base-2 exponential and reciprocal are off by an ulp each.
 #pragma once
 #include "common.hpp"
 #include "../../include/acktr_hip.h"
@@ -8,48 +8,79 @@ namespace acktr {
 
 constexpr float LOG2E = 1.44269504088896340736f;
 
-__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
 __device__ __forceinline__ float fast_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
-// 1 / (1 + e^-x): e^-x overflows to infinity below x = -88, whose reciprocal is the right limit 0
-__device__ __forceinline__ float sigmoid_f(float x) { return fast_rcp(1.f + fast_exp(-x)); }
+// e^x.  The rounding of x log2(e) alone puts it off by |x| 6e-8, nothing beside the rounding of 16-bit storage.  ACC (fp32 storage, |x| at
+// most 200): that rounding is carried along (`more`: what x itself lacks), which leaves 2 ulp.  e^x below 2^-126 is 0.
+template <bool ACC>
+__device__ __forceinline__ float exp_of(float x, float more = 0.f) {
+    const float p = x * LOG2E;
+    float e = __builtin_amdgcn_exp2f(p);
+    if (ACC) {
+        const float lo = fmaf(x, LOG2E, -p) + (x * 1.92596299e-8f + more * LOG2E);
+        e = fmaf(e, lo * 0.693147182f, e);
+    }
+    return e;
+}
+// the magnitude that an exponent is formed of (minimum() keeps a NaN): beyond 100 sigmoid and tanh are at their limits
+template <bool ACC>
+__device__ __forceinline__ float magnitude(float x) { return ACC ? __builtin_elementwise_minimum(fabsf(x), 100.f) : fabsf(x); }
 
-// tanh: (1 - e^-2|x|) / (1 + e^-2|x|) with x's sign; near zero the difference cancels, there the series x - x^3/3 + 2x^5/15 - 17x^7/315
-__device__ __forceinline__ float tanh_f(float x) {
-    const float a = fabsf(x), e = fast_exp(-2.f * a);
-    const float big = (1.f - e) * fast_rcp(1.f + e), q = x * x;
+// s = 1 / (1 + e^-x) and ns = 1 - s, both within 5 ulp of their own size (down to 2^-126; 16-bit storage: 6e-8 |x| more)
+template <bool ACC>
+__device__ __forceinline__ void sigmoid_of(float x, float& s, float& ns) {
+    const float e = exp_of<ACC>(-magnitude<ACC>(x)), big = fast_rcp(1.f + e), tail = e * big;
+    s = x < 0.f ? tail : big;
+    ns = x < 0.f ? big : tail;
+}
+
+// tanh: (1 - e^-2|x|) / (1 + e^-2|x|) with x's sign; near zero the difference cancels, there the series x - x^3/3 + 2x^5/15 - 17x^7/315.
+// e: e^-2|x|, r: 1 / (1 + e).
+__device__ __forceinline__ float tanh_f(float x, float e, float r) {
+    const float a = fabsf(x), big = (1.f - e) * r, q = x * x;
     const float small = a * (1.f + q * (-0.333333343f + q * (0.133333340f + q * -0.0539682545f)));
     return copysignf(a < 0.25f ? small : big, x);
 }
-// Complementary form of the normal distribution, 1 - Phi(|x|) = erfc(|x| / sqrt 2) / 2, by Abramowitz & Stegun 7.1.26: five terms in
-// t = 1 / (1 + p |x| / sqrt 2), absolute error 7.5e-8 after the halving.  Forming the SMALL tail keeps gelu of large negative arguments
-// relative to its own size.
+// Complementary form of the normal distribution, 1 - Phi(a) = e^(-a*a/2) t P(t) with t = 1 / (1 + 0.35 a), for 0 <= a: a polynomial of
+// degree 8, fitted to the scaled complementary error function for the least relative error on [0, 13.5] (3e-8; beyond, the exponential
+// is 0).  Formed of the SMALL tail, gelu of negative arguments is within 8 ulp of its own size wherever that is above 2^-118 (16-bit
+// storage: 6e-8 z^2 more).
 __device__ __forceinline__ float normal_tail(float a, float e /* e^(-a*a/2) */) {
-    const float t = fast_rcp(1.f + 0.23164189f * a);
-    return 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    const float t = fast_rcp(fmaf(0.35f, a, 1.f));
+    float q = -0.0291258693f;
+    q = fmaf(q, t, 0.143872246f);
+    q = fmaf(q, t, -0.255504608f);
+    q = fmaf(q, t, 0.158929333f);
+    q = fmaf(q, t, -0.0229371656f);
+    q = fmaf(q, t, 0.10543295f);
+    q = fmaf(q, t, 0.119852431f);
+    q = fmaf(q, t, 0.13985908f);
+    q = fmaf(q, t, 0.139621571f);
+    return e * (t * q);
 }
 
 // y = act(z) and, with WANT, the slope act'(z); the two share their exponential
-template <int ACT, bool WANT>
+template <int ACT, bool WANT, bool ACC>
 __device__ __forceinline__ float act_of(float z, float& slope) {
     if (ACT == ACKTR_ACT_RELU) {
         if (WANT) slope = z > 0.f ? 1.f : (z != z ? z : 0.f);
         return z > 0.f ? z : (z != z ? z : 0.f);
     }
     if (ACT == ACKTR_ACT_TANH) {
-        if (WANT) {
-            const float e = fast_exp(-2.f * fabsf(z)), r = fast_rcp(1.f + e);      // 1 / cosh^2, without 1 - tanh^2's cancellation
-            slope = 4.f * e * r * r;
-        }
-        return tanh_f(z);
+        const float e = exp_of<ACC>(-2.f * magnitude<ACC>(z)), r = fast_rcp(1.f + e);
+        if (WANT) slope = 4.f * e * r * r;                                         // 1 / cosh^2, without 1 - tanh^2's cancellation
+        return tanh_f(z, e, r);
     }
     if (ACT == ACKTR_ACT_SILU) {
-        const float s = sigmoid_f(z);
-        if (WANT) slope = s * (1.f + z * (1.f - s));
+        float s, ns;
+        sigmoid_of<ACC>(z, s, ns);
+        if (WANT) slope = s * (1.f + z * ns);
         return z * s;
     }
     if (ACT == ACKTR_ACT_GELU) {
-        const float a = fabsf(z), e = fast_exp(-0.5f * z * z), tail = normal_tail(a, e), cdf = z < 0.f ? tail : 1.f - tail;
-        if (WANT) slope = cdf + z * e * 0.3989422804f;
+        // held at 18, where the exponential is 0 already; ACC: z^2 / 2 with the rounding of z^2
+        const float a = __builtin_elementwise_minimum(fabsf(z), 18.f), q = a * a;
+        const float e = exp_of<ACC>(-0.5f * q, ACC ? -0.5f * fmaf(a, a, -q) : 0.f), tail = normal_tail(a, e), cdf = z < 0.f ? tail : 1.f - tail;
+        if (WANT) slope = cdf + copysignf(a, z) * e * 0.3989422804f;
         return z * cdf;
     }
     if (WANT) slope = 1.f;

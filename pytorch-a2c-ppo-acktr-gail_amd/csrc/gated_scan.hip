@@ -42,12 +42,7 @@ template <bool ACC>
 __device__ __forceinline__ void gate_of(float x, float& f, float& nf) {
     x = __builtin_elementwise_maximum(x, -87.f);
     if (ACC) x = __builtin_elementwise_minimum(x, 200.f);
-    const float p = x * -LOG2E;
-    float e = __builtin_amdgcn_exp2f(p);
-    if (ACC) {
-        const float lo = fmaf(x, -LOG2E, -p) + x * -1.92596299e-8f;
-        e = fmaf(e, lo * 0.693147182f, e);
-    }
+    const float e = exp_of<ACC>(-x);
     f = fast_rcp(1.f + e);
     nf = e * f;
 }

@@ -19,7 +19,7 @@ __device__ __forceinline__ void finish8(const LinArgs& p, int m, int n, float (&
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         float slope;
-        float o = act_of<ACT, SLOPE>(v[i] + b[i], slope);
+        float o = act_of<ACT, SLOPE, sizeof(T) == 4>(v[i] + b[i], slope);
         if (res) o += to_f32(r[i]);
         y[i] = from_f32<T>(o);
         if (SLOPE) {
@@ -36,7 +36,7 @@ template <class T, int ACT, bool SLOPE>
 __device__ __forceinline__ void finish1(const LinArgs& p, int m, int n, float v, float b, T r, bool res) {
     typedef typename SlopeOf<T>::type ST;
     float slope;
-    float o = act_of<ACT, SLOPE>(v + b, slope);
+    float o = act_of<ACT, SLOPE, sizeof(T) == 4>(v + b, slope);
     if (res) o += to_f32(r);
     ((T*)p.y)[(long)m * p.ldy + n] = from_f32<T>(o);
     if (SLOPE) put_slope(((ST*)p.pre)[(long)m * p.ldp + n], slope);

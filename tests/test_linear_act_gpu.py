@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from gated_refs import ACTS, check, linear64, linear_grads64
+from gated_refs import ACTS, E32, EPS, TINY, act64, check, linear64, linear_grads64
 
 pytestmark = pytest.mark.gpu
 DEV = 'cuda:0'
@@ -79,6 +79,46 @@ def test_large_pre_activations():
     """tails of every activation: values far from zero"""
     for act in ACTS:
         run(96, 64, 64, F32, act, big=30.0)
+
+
+@pytest.mark.parametrize('dt', [BF, HF, F32])
+@pytest.mark.parametrize('act', ['tanh', 'silu', 'gelu'])
+def test_tails_are_right_relative_to_their_own_size(act, dt):
+    """Values and slopes of negative pre-activations, which an identity weight makes exact, down to where the exponential is 0.
+    With E = 2^-24: the exponential is off by 4 E (exp2 2, its correction 1), 1 + e by 1, a reciprocal by 2, a product by 1; the
+    polynomial of gelu's tail, its argument's reciprocal included, by 8.  silu: 4 + 1 + 2 + 1 + 1, gelu: 4 + 8 + 1 + 1: 16 E.  tanh goes
+    through 1 - e, which is 0.39 and more where it is used, 4 E 0.61 / 0.39 + 1 + 3 + 1 = 12, or a series (its next term 3.3e-7 = 6 E, its
+    roundings 4).  16-bit storage does not carry the rounding of the exponent, E z^2 for gelu (two of z^2 / 2), E |z| for silu, 2 E |z| for tanh."""
+    from a2c_ppo_acktr import ops
+    low = {'tanh': 40.0, 'silu': 86.0, 'gelu': 12.8}[act]
+    x = torch.cat((torch.linspace(-low, 0.0, 40000, device=DEV), torch.linspace(0.0, 6.0, 4000, device=DEV))).to(dt).view(-1, 8)
+    pre = torch.empty_like(x)
+    y = ops.linear_act_fwd(x, torch.eye(8, dtype=dt, device=DEV), act=act, pre=pre)
+    z = x.double()
+    ref, slope = act64(z, act)
+    rel = 16 * E32 + (0 if dt == F32 else E32 * {'tanh': 2 * z.abs(), 'silu': z.abs(), 'gelu': z * z}[act])
+    check(y, (ref, (rel * (1 + EPS[dt]) + (EPS[dt] if dt != F32 else 0)) * ref.abs() + TINY[dt] + 2.0 ** -118), 'y')
+    if dt == F32:                                            # (16 bits: fixed-point steps)
+        # tanh 4 e r^2: 4 + 2 (1 + 2) + 3.  silu s (1 + z ns) and gelu Q - a phi have a root at -1.28 and at -0.75; from -2 down their two terms
+        # are at most 2.4 and 1.6 times the result: 8 + 2.4 (4 + 1) + 2 and 1.6 (13 + 1) + 1.  Elsewhere to the same part of 1.13.
+        d, big = (pre.double() - slope).abs(), 24 * E32
+        tol = torch.where((z <= -2) | (act == 'tanh'), slope.abs(), torch.full_like(z, 1.13)) * big + 2.0 ** -118
+        assert bool((d <= tol).all()), float((d / tol).max())
+
+
+@pytest.mark.parametrize('dt', [BF, HF, F32])
+def test_activations_at_infinity(dt):
+    """limits of values and gradients where the definition has them: act(+inf) = inf, slope 1 (tanh: 1, 0); relu and tanh at -inf"""
+    from a2c_ppo_acktr import ops
+    inf = float('inf')
+    x, w = torch.tensor([[inf], [-inf], [0.5]], dtype=dt, device=DEV), torch.ones(1, 1, dtype=dt, device=DEV)
+    for act, top, low in (('relu', inf, 0.0), ('tanh', 1.0, -1.0), ('silu', inf, None), ('gelu', inf, None)):
+        pre = torch.empty(3, 1, dtype=dt, device=DEV)
+        y = ops.linear_act_fwd(x, w, act=act, pre=pre)
+        assert float(y[0]) == top and (low is None or float(y[1]) == low), act
+        if act in ('relu', 'tanh', 'gelu'):
+            dx, _, _ = ops.linear_act_bwd(torch.ones(3, 1, dtype=dt, device=DEV), x, w, pre=pre, act=act, need_dw=False, need_db=False)
+            assert float(dx[0]) == (0.0 if act == 'tanh' else 1.0) and float(dx[1]) == 0.0, act
 
 
 def test_slices_at_odd_offsets():
