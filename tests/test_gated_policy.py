@@ -50,6 +50,17 @@ def test_what_was_falsy_or_truthy_still_is():
     assert hasattr(Policy((11,), Box(), base_kwargs={'recurrent': 1}).base, 'gru')
 
 
+@pytest.mark.parametrize('value', ['gru', 'yes', 'True', '1'])
+def test_strings_are_taken_by_their_truth(value):
+    from a2c_ppo_acktr.model import Policy
+    torch.manual_seed(3)
+    a = Policy((11,), Box(), base_kwargs={'recurrent': value})
+    torch.manual_seed(3)
+    b = Policy((11,), Box(), base_kwargs={'recurrent': True})
+    assert hasattr(a.base, 'gru') and torch.equal(a.flat_params, b.flat_params)
+    assert not Policy((11,), Box(), base_kwargs={'recurrent': ''}).is_recurrent
+
+
 def test_the_gru_is_what_it_was():
     """same initialiser calls in the same order: a seed gives the same GRU policy with and without the new core in the package"""
     from a2c_ppo_acktr.model import Policy
