@@ -38,10 +38,10 @@ __device__ const uint4 g_tile_zero = {0, 0, 0, 0};
 
 // memory -> LDS, 16 bytes a lane: from `base` (uniform) + off (per lane); to lds (uniform) + 16 * lane
 __device__ __forceinline__ void dma16(const void* base, unsigned off, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
 __device__ __forceinline__ void dma16_ptr(const void* p, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
 }
 // all but the newest LEFT loads and every LDS access of this wave are done, then the workgroup's
 template <int LEFT>
