@@ -33,6 +33,23 @@ __device__ __forceinline__ void forget(X& x) {
 // product that is 0 where a factor is, even if the other one is not finite: what a mask of 0 drops leaves no trace
 extern "C" __device__ float acktr_mul_legacy(float, float) __asm("llvm.amdgcn.fmul.legacy");      // v_mul_legacy_f32
 __device__ __forceinline__ float cut_mul(float a, float x) { return acktr_mul_legacy(a, x); }
+// Such a product must not become 0 by itself, however many steps it spans: a state that is not finite stays so until a mask drops it.  A
+// composed factor without a zero in it is held at 2^-126 (what it adds to a finite state is what a shut gate's f adds).
+__device__ __forceinline__ float held(float A) { return fabsf(A) < 1.17549435e-38f ? 1.17549435e-38f : A; }
+// Products of factors, and the least of them, which tells a mask from an underflow.
+template <int V>
+struct Factor {
+    float prod[V], least[V];
+    __device__ __forceinline__ Factor() {
+#pragma unroll
+        for (int i = 0; i < V; ++i) prod[i] = least[i] = 1.f;
+    }
+    __device__ __forceinline__ void take(int i, float a) {
+        prod[i] *= a;
+        least[i] = fminf(least[i], fabsf(a));
+    }
+    __device__ __forceinline__ float value(int i) const { return least[i] == 0.f ? 0.f : held(prod[i]); }
+};
 
 // f = 1 / (1 + e^-x) and 1 - f = e^-x f, both relative to their own size.  x is held above -87, where f is fp32's smallest normal number
 // and e^-x still finite (maximum() keeps a NaN).  ACC (fp32 storage): the product x log2(e) is carried with its rounding error,
@@ -192,9 +209,9 @@ struct Scan {
     }
 
     // (A, B): this wave's composed steps (REV: in descending order).  Returns the state at their start in `in` and moves `carry`
-    // behind the last wave; PROD: `prod` collects the product of all A.  sm: NW * CT * 2 floats; the caller alternates two of them.
+    // behind the last wave; PROD: `all` collects the product of all A.  sm: NW * CT * 2 floats; the caller alternates two of them.
     template <bool REV, bool PROD>
-    __device__ __forceinline__ void exchange(const float (&A)[V], const float (&B)[V], float (&carry)[V], float (&in)[V], float (&prod)[V],
+    __device__ __forceinline__ void exchange(const float (&A)[V], const float (&B)[V], float (&carry)[V], float (&in)[V], Factor<V>& all,
                                              pairs* sm) const {
         pairs mine;
 #pragma unroll
@@ -212,7 +229,7 @@ struct Scan {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 carry[i] = cut_mul(q[2 * i], carry[i]) + q[2 * i + 1];
-                if (PROD) prod[i] = cut_mul(q[2 * i], prod[i]);
+                if (PROD) all.take(i, q[2 * i]);
             }
         }
     }
@@ -223,25 +240,29 @@ struct Scan {
         const int cnt = REV ? p.blocks - 1 - blk : blk, per = (cnt + NW - 1) / NW;
         const int r = REV ? NW - 1 - wave : wave, b0 = min(cnt, r * per), b1 = min(cnt, b0 + per);
         float A[V], B[V], in[V];
+        Factor<V> all;
 #pragma unroll
-        for (int i = 0; i < V; ++i) A[i] = 1.f, B[i] = 0.f;
+        for (int i = 0; i < V; ++i) B[i] = 0.f;
         for (int b = b0; b < b1; ++b) {
             const float* q = p.agg + 2L * (REV ? p.blocks - 1 - b : b) * C + c;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 B[i] = cut_mul(q[i], B[i]) + q[C + i];
-                A[i] = cut_mul(q[i], A[i]);
+                all.take(i, q[i]);
             }
         }
-        exchange<REV, false>(A, B, carry, in, in, sm);
+#pragma unroll
+        for (int i = 0; i < V; ++i) A[i] = all.value(i);
+        exchange<REV, false>(A, B, carry, in, all, sm);
     }
 };
 
 // --------------------------------------------------------------------------------------------------------- forward
 // AGG: only the block's composition is formed (first pass of a time split).  Bound by memory: bf16, 2048 x 32 x 1024 in 89 us (4.5 TB/s
-// over two reads and a write); 65536 x 1 x 512, split, 29 us for the compositions and 38 for the states.
+// over two reads and a write); 65536 x 1 x 512, split, 29 us for the compositions and 38 for the states.  With two channels a lane the
+// registers are kept to 128, which lets two workgroups of 8 waves share a CU (that case, forward + backward, 171 us against 181 with 133).
 template <class T, int V, int NW, int MODE, bool AGG>
-__global__ __launch_bounds__(NW * 64) void scan_fwd_kernel(const ScanArgs p) {
+__global__ __launch_bounds__(NW * 64, V == 2 && (NW == 8 || MODE == SCAN_WHOLE) ? 4 : 1) void scan_fwd_kernel(const ScanArgs p) {
     typedef Scan<T, V, NW, MODE> S;
     typedef typename S::vv vv;
     __shared__ typename S::pairs sm[2][NW * 64];
@@ -251,10 +272,11 @@ __global__ __launch_bounds__(NW * 64) void scan_fwd_kernel(const ScanArgs p) {
     const int blk = blockIdx.y, tb = blk * p.block_steps, te = min(p.T, tb + p.block_steps);
     const typename S::Rows rg = s.rows(p.gate, p.gt, p.gn), rv = s.rows(p.value, p.vt, p.vn), ro = s.rows(p.out, p.ot, p.on);
     const bool all = (long)(s.tile + 1) * S::CT <= C;    // every lane of the tile has channels
-    float carry[V], prod[V];
+    float carry[V];
+    Factor<V> prod;
     int par = 0;
 #pragma unroll
-    for (int i = 0; i < V; ++i) carry[i] = !AGG && p.h0 ? p.h0[s.c + i] : 0.f, prod[i] = 1.f;
+    for (int i = 0; i < V; ++i) carry[i] = !AGG && p.h0 ? p.h0[s.c + i] : 0.f;
     if (!AGG && p.blocks > 1) {
         s.template skip_blocks<false>(p, blk, carry, sm[par]);
         par ^= 1;
@@ -264,7 +286,7 @@ __global__ __launch_bounds__(NW * 64) void scan_fwd_kernel(const ScanArgs p) {
     fetch(tb + s.wave * SCAN_L);
     for (int t0 = tb; t0 < te; t0 += S::SC) {
         const int tw = t0 + s.wave * SCAN_L;
-        float m[SCAN_L], a[SCAN_L][V], b[SCAN_L][V], A[V], B[V], in[V];
+        float m[SCAN_L], a[SCAN_L][V], b[SCAN_L][V], A[V], B[V], in[V], kept = 1.f;
         s.masks(p, tw, te, m);
 #pragma unroll
         for (int i = 0; i < V; ++i) A[i] = 1.f, B[i] = 0.f;
@@ -279,7 +301,10 @@ __global__ __launch_bounds__(NW * 64) void scan_fwd_kernel(const ScanArgs p) {
                 B[i] = cut_mul(a[l][i], B[i]) + b[l][i];
                 A[i] = cut_mul(a[l][i], A[i]);
             }
+            kept = cut_mul(kept, m[l]);                      // 0 where a mask of these steps is
         }
+#pragma unroll
+        for (int i = 0; i < V; ++i) A[i] = kept == 0.f ? 0.f : held(A[i]);
         if (t0 + S::SC < te) fetch(tw + S::SC);
         s.template exchange<false, AGG>(A, B, carry, in, prod, sm[par]);
         par ^= 1;
@@ -303,7 +328,7 @@ __global__ __launch_bounds__(NW * 64) void scan_fwd_kernel(const ScanArgs p) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             if (AGG) {
-                p.agg[(2L * blk) * C + s.c + i] = prod[i];
+                p.agg[(2L * blk) * C + s.c + i] = prod.value(i);
                 p.agg[(2L * blk + 1) * C + s.c + i] = carry[i];
             } else if (te == p.T && p.last) {
                 p.last[s.c + i] = carry[i];
@@ -316,7 +341,7 @@ __global__ __launch_bounds__(NW * 64) void scan_fwd_kernel(const ScanArgs p) {
 // The states are formed again from the saved ones, in fp32, rather than read from the rounded output.  Bound by memory: bf16,
 // 2048 x 32 x 1024 in 152 us (4.4 TB/s over three reads and two writes); 65536 x 1 x 512, split, 27 + 77 us.
 template <class T, int V, int NW, int MODE, bool AGG>
-__global__ __launch_bounds__(NW * 64) void scan_bwd_kernel(const ScanArgs p) {
+__global__ __launch_bounds__(NW * 64, V == 2 ? 2 : 1) void scan_bwd_kernel(const ScanArgs p) {
     typedef Scan<T, V, NW, MODE> S;
     typedef typename S::vv vv;
     __shared__ typename S::pairs sm[2][2][NW * 64];
@@ -327,10 +352,11 @@ __global__ __launch_bounds__(NW * 64) void scan_bwd_kernel(const ScanArgs p) {
     const typename S::Rows rg = s.rows(p.gate, p.gt, p.gn), rv = s.rows(p.value, p.vt, p.vn), rd = s.rows(p.dout, p.dt, p.dn);
     const typename S::Rows qg = s.rows(p.dgate, p.dgt, p.dgn), qv = s.rows(p.dvalue, p.dvt, p.dvn);
     const bool all = (long)(s.tile + 1) * S::CT <= C;
-    float carry[V], prod[V];                                 // carry: E behind the steps that are done
+    float carry[V];                                          // E behind the steps that are done
+    Factor<V> prod;
     int par = 0;
 #pragma unroll
-    for (int i = 0; i < V; ++i) carry[i] = !AGG && p.dlast ? p.dlast[s.c + i] : 0.f, prod[i] = 1.f;
+    for (int i = 0; i < V; ++i) carry[i] = !AGG && p.dlast ? p.dlast[s.c + i] : 0.f;
     if (!AGG && p.blocks > 1) {
         s.template skip_blocks<true>(p, blk, carry, sm[0][par]);
         par ^= 1;
@@ -341,7 +367,7 @@ __global__ __launch_bounds__(NW * 64) void scan_bwd_kernel(const ScanArgs p) {
     fetch(tb + (chunks - 1) * S::SC + s.wave * SCAN_L);
     for (int q = chunks - 1; q >= 0; --q) {
         const int t0 = tb + q * S::SC, tw = t0 + s.wave * SCAN_L;
-        float f[SCAN_L][V], nf[SCAN_L][V], A[V], B[V], P[V], Q[V], in[V], ein[V];
+        float f[SCAN_L][V], nf[SCAN_L][V], A[V], B[V], P[V], Q[V], in[V], ein[V], kept = 1.f;
         vv vc[SCAN_L], dc[SCAN_L];
         float mc[SCAN_L];
         s.masks(p, tw, te, mc);
@@ -362,13 +388,17 @@ __global__ __launch_bounds__(NW * 64) void scan_bwd_kernel(const ScanArgs p) {
             }
         }
 #pragma unroll
-        for (int l = SCAN_L - 1; l >= 0; --l)
+        for (int l = SCAN_L - 1; l >= 0; --l) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const float a = mc[l] * f[l][i];
                 Q[i] = cut_mul(a, to_f32(dc[l][i]) + Q[i]);
                 P[i] = cut_mul(a, P[i]);
             }
+            kept = cut_mul(kept, mc[l]);
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) A[i] = kept == 0.f ? 0.f : held(A[i]), P[i] = kept == 0.f ? 0.f : held(P[i]);
         if (q > 0) fetch(tw - S::SC);
         if (!AGG) {
             // fp32 copies of values and derivatives and the products m f would take 96 registers more
@@ -414,7 +444,7 @@ __global__ __launch_bounds__(NW * 64) void scan_bwd_kernel(const ScanArgs p) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             if (AGG) {
-                p.agg[(2L * blk) * C + s.c + i] = prod[i];
+                p.agg[(2L * blk) * C + s.c + i] = prod.value(i);
                 p.agg[(2L * blk + 1) * C + s.c + i] = carry[i];
             } else if (tb == 0 && p.dh0) {
                 p.dh0[s.c + i] = carry[i];

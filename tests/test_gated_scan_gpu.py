@@ -148,6 +148,40 @@ def test_a_mask_of_zero_cuts_what_is_not_finite():
         assert torch.equal(got[0][cut:], ok[0][cut:]) and torch.equal(got[1], ok[1])
 
 
+@pytest.mark.parametrize('dt', [BF, F32])
+@pytest.mark.parametrize('T,N,H,shift', [(3000, 1, 8, 0.0), (400, 3, 40, -12.0), (20, 2, 8, -30.0), (700, 64, 256, -1.0)])
+def test_what_is_not_finite_stays_until_a_mask(T, N, H, shift, dt):
+    """factors over many steps are far below fp32's smallest number; what they multiply is lost only where a mask is 0"""
+    from a2c_ppo_acktr import ops
+    g, v, m, h0, dout, dl = inputs(T, N, H, dt, shift=shift)
+    m = torch.ones_like(m)
+    cut = T * 3 // 4
+    m[cut, 0] = 0
+    nan, at = float('nan'), T // 3
+    out, last, saved = ops.gated_scan_fwd(g, v, h0, m, save=True)
+    dg, dv, dh0 = ops.gated_scan_bwd(dout, g, v, h0, m, saved=saved, dlast=dl)
+    # a state, a value: every step up to the cut, and no other channel
+    h1, v1 = h0.clone(), v.clone()
+    h1[0, 0], h1[-1, 3], v1[at, 0, 1] = nan, float('inf'), nan
+    o, l, s1 = ops.gated_scan_fwd(g, v1, h1, m, save=True)
+    bad = torch.zeros(T, N, H, dtype=torch.bool, device=DEV)
+    bad[:cut, 0, 0], bad[at:cut, 0, 1] = True, True
+    bad[:cut if N == 1 else T, -1, 3] = True
+    assert torch.equal(~o.isfinite(), bad) and torch.equal(o[~bad], out[~bad])
+    assert torch.equal(~l.isfinite(), bad[-1]) and torch.equal(l[~bad[-1]], last[~bad[-1]])
+    a, b, _ = ops.gated_scan_bwd(dout, g, v1, h1, m, saved=s1, dlast=dl)
+    # (a gate's gradient takes the state before its step)
+    assert bool(a[1:cut, 0, 0].isnan().all()) and bool(a[at:cut, 0, 1].isnan().all()) and torch.equal(a[cut:, 0], dg[cut:, 0]) and torch.equal(b, dv)
+    # a derivative: every step down to the cut
+    d1, l1 = dout.clone(), dl.clone()
+    d1[at, 0, 2], l1[0, 4] = nan, nan
+    a, b, c = ops.gated_scan_bwd(d1, g, v, h0, m, saved=saved, dlast=l1)
+    bad = torch.zeros(T, N, H, dtype=torch.bool, device=DEV)
+    bad[:at + 1, 0, 2], bad[cut:, 0, 4] = True, True
+    assert torch.equal(a.isnan(), bad) and torch.equal(b.isnan(), bad) and torch.equal(c.isnan(), bad[0])
+    assert torch.equal(a[~bad], dg[~bad]) and torch.equal(b[~bad], dv[~bad]) and torch.equal(c[~bad[0]], dh0[~bad[0]])
+
+
 def test_every_step_masked():
     from a2c_ppo_acktr import ops
     g, v, m, h0, dout, dl = inputs(100, 2, 24, F32)
