@@ -815,7 +815,8 @@ def gated_scan_step(gate, value, state, masks=None, out=None):
     if given:
         _apart(out, 'out', (gate, value, state, masks), 'gated_scan_step')
     lo, hi = ps, ps + 4 * N * H
-    if lo <= pg < hi or lo <= pv < hi or pg <= lo < pg + gn * N * 4 or pv <= lo < pv + vn * N * 4 or (pm and lo - 4 * N < pm < hi):
+    # (a row that all sequences share has a stride of 0, and still H values)
+    if lo <= pg < hi or lo <= pv < hi or pg <= lo < pg + max(gn, H) * N * 4 or pv <= lo < pv + max(vn, H) * N * 4 or (pm and lo - 4 * N < pm < hi):
         _apart(state, 'state', (gate, value, masks), 'gated_scan_step')
     _launch(_hip.lib().acktr_gated_scan_step, at, 'gated_scan_step', 10.0 * N * H, pg, gn, pv, vn, ps, pm, po, on, N, H, code)
     _written((state, out) if given else state)

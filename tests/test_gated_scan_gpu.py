@@ -337,3 +337,17 @@ def test_refusals_on_the_device():
     for f in bad:
         with pytest.raises(RuntimeError):
             f()
+
+
+def test_a_shared_row_in_the_state_is_refused():
+    """a gate or value row that all sequences share may not reach into the state that the step updates"""
+    from a2c_ppo_acktr import ops
+    N, H = 4, 16
+    buf = rnd(1, N * H + 3 * H)
+    row, other, state = buf[:H].expand(N, H), buf[-H:].expand(N, H), buf[H // 2:H // 2 + N * H].view(N, H)
+    for g, v in ((row, other), (other, row)):
+        with pytest.raises(RuntimeError, match='overlaps'):
+            ops.gated_scan_step(g, v, state)
+    state = buf[H:H + N * H].view(N, H)                      # apart from both rows
+    want = scan64(row[None], other[None], state.clone(), None)['out']
+    check(ops.gated_scan_step(row, other, state), (want[0][0], want[1][0]), 'out')
