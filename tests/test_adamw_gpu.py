@@ -96,6 +96,68 @@ def test_16_bit_parameters(pdt):
         assert bool(((p.to(F64) - r).abs() <= EPS[pdt] * r.abs() + 1e-6).all())      # one rounding; fp32 inside
 
 
+# more chunks (of 2048) than the update's workgroups sum for themselves, around the norm's 1024 workgroups with two chunks each
+LONG = [[(1025 * 2048 - 700,), (300,)], [(1200, 1700), (3,), (2048, 1031), (77,)], [(5000, 2048), (1,), (65537,)]]
+
+
+@pytest.mark.parametrize('odd', [False, True])
+@pytest.mark.parametrize('shapes', LONG)
+@pytest.mark.parametrize('gdt', [F32, BF])
+def test_clipped_lists_of_many_chunks(gdt, shapes, odd):
+    """the norm of a long list: its own launch finishes it, step after step, captured too"""
+    from a2c_ppo_acktr import algo, ops
+    steps, clip, runs = 4, 0.5, []
+    for captured in (False, True, False):
+        ps, gs, cs = make(shapes, gdt=gdt, cdt=BF, odd=odd)
+        p0 = [p.clone() for p in ps]
+        opt = algo.AdamW(ps, grads=gs, copies=cs, max_grad_norm=clip, **HP)
+        graph, hist = None, []
+        for k in range(steps):
+            for i, g in enumerate(gs):
+                g.copy_(rnd(500 + 50 * k + i, *g.shape, scale=0.1 + 0.2 * k))
+            hist.append([g.clone() for g in gs])
+            if captured and k == 1:
+                torch.cuda.synchronize()
+                graph = torch.cuda.CUDAGraph()
+                with ops.graph_capture(graph):
+                    opt.step()
+            opt.step() if graph is None else graph.replay()
+            torch.cuda.synchronize()
+        assert opt.steps_done() == steps
+        runs.append([p.clone() for p in ps] + list(opt.moments()))
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(*runs))
+    rp, rm, rv = ref_steps(p0, hist, clip)
+    m, v = moments_of(opt, shapes)
+    for i in range(len(shapes)):                             # (as in test_fp32_moments)
+        amax = torch.stack([h[i].to(F64).abs() for h in hist]).amax(0)
+        tp = steps * (3 * E32 * (rp[i].abs() + 0.1) + 64 * E32 * HP['lr'] / (1 - HP['betas'][0]))
+        assert bool(((m[i].to(F64) - rm[i]).abs() <= 8 * steps * E32 * amax).all()), i
+        assert bool(((v[i].to(F64) - rv[i]).abs() <= 8 * steps * E32 * amax ** 2).all()), i
+        assert bool(((ps[i].to(F64) - rp[i]).abs() <= tp).all()), (i, float((ps[i].to(F64) - rp[i]).abs().max()))
+        if cs[i] is not None:
+            assert torch.equal(cs[i], ps[i].to(BF))
+
+
+@pytest.mark.parametrize('shapes', LONG)
+def test_clipped_8_bit_lists_of_many_chunks(shapes):
+    """the first step does not depend on how moments are kept; later ones repeat bit for bit, and a clip far above the norm is none"""
+    from a2c_ppo_acktr import algo
+    runs = []
+    for clip in (0.5, 0.5, 1e9, None):
+        ps, gs, _ = make(shapes)
+        p0 = [p.clone() for p in ps]
+        opt = algo.AdamW(ps, grads=gs, max_grad_norm=clip, state_bits=8, seed=7, **HP)
+        opt.step()
+        if clip != 1e9:
+            rp, _, _ = ref_steps(p0, [gs], clip)
+            for p, r in zip(ps, rp):
+                assert bool(((p.to(F64) - r).abs() <= 3 * E32 * (r.abs() + 0.1) + 64 * E32 * HP['lr'] / (1 - HP['betas'][0])).all())
+        opt.step(), opt.step()
+        runs.append([p.clone() for p in ps] + list(opt.moments()))
+    assert all(torch.equal(a, b) for a, b in zip(runs[0], runs[1])) and all(torch.equal(a, b) for a, b in zip(runs[2], runs[3]))
+    assert not torch.equal(runs[0][0], runs[2][0])
+
+
 # ------------------------------------------------------------------------------------------------ 8-bit moments, restated
 def mix(x):
     x = (x ^ (x >> 16)) * 0x7feb352d & 0xffffffff

@@ -75,6 +75,33 @@ def test_time_is_split_over_workgroups(T, N, H, dt):
     run(T, N, H, dt, masked=False, seed=3, shift=6.0)
 
 
+@pytest.mark.parametrize('T,N,H,dt', [
+    (300, 32, 1024, BF),                 # two channels a lane, 8 waves, whole tiles: three superchunks
+    (150, 36, 974, BF), (150, 36, 974, HF),          # the same with tiles of several sequences
+    (200, 64, 1024, BF), (333, 64, 1024, HF),        # 4 waves, whole tiles: several superchunks of 64 steps
+    (150, 70, 974, BF), (150, 70, 974, HF),          # 4 waves, tiles of several sequences
+    (150, 40, 973, BF), (150, 40, 973, F32), (300, 33, 1024, F32),       # one channel a lane, 4 waves
+    (8200, 1, 512, BF), (8200, 1, 512, HF),          # two channels a lane, time split over workgroups, whole tiles
+    (4500, 5, 190, BF),                              # the same with tiles of several sequences
+    (2100, 3, 77, F32), (2100, 3, 77, HF),           # one channel a lane, split, tiles of several sequences
+])
+def test_every_plan(T, N, H, dt):
+    run(T, N, H, dt, shift=2.0)
+
+
+@pytest.mark.parametrize('T,N,H', [(300, 32, 1024), (8200, 1, 512)])
+def test_the_two_passes_may_be_laid_out_apart(T, N, H):
+    """a backward pass whose derivative has odd rows takes one channel a lane, on states that a forward pass with two has saved"""
+    from a2c_ppo_acktr import ops
+    g, v, m, h0, dout, dl = inputs(T, N, H, BF, shift=2.0)
+    odd = torch.empty(T, N, H + 1, dtype=BF, device=DEV)[..., :H].copy_(dout)
+    out, fin, saved = ops.gated_scan_fwd(g, v, h0, m, save=True)
+    got = ops.gated_scan_bwd(odd, g, v, h0, m, saved=saved, dlast=dl)
+    ref = scan64(g, v, h0, m, dout, dl)
+    for name, t in (('out', out), ('last', fin), ('dgate', got[0]), ('dvalue', got[1]), ('dh0', got[2])):
+        check(t, ref[name], name)
+
+
 def test_many_channels():
     run(40, 96, 768, BF)
 

@@ -75,6 +75,68 @@ def test_largest_tiles_with_ragged_edges(dt, M, N, K):
     run(M, N, K, dt, 'silu')
 
 
+# One shape, with ragged edges, for every kernel that the estimate in linear_act.hpp can pick: product, tile, split reduction or not.
+TILES16 = [
+    ('forward', 84, 70, 913),            # 64 x 64, split
+    ('forward', 8249, 72, 74),           # 128 x 64
+    ('forward', 1426, 73, 1473),         # 128 x 64, split
+    ('forward', 16647, 324, 72),         # 128 x 128
+    ('forward', 4090, 2046, 520),        # 128 x 128
+    ('forward', 5453, 72, 3920),         # 128 x 128, split
+    ('forward', 19769, 520, 76),         # 256 x 256
+    ('forward', 16605, 193, 3652),       # 256 x 256, split
+    ('dx', 73, 73, 71),                  # 64 x 64
+    ('dx', 73, 897, 70),                 # 64 x 64, split
+    ('dx', 8249, 72, 74),                # 128 x 64
+    ('dx', 76, 3278, 595),               # 128 x 64, split
+    ('dx', 14063, 72, 401),              # 128 x 128
+    ('dx', 5620, 3912, 72),              # 128 x 128, split
+    ('dx', 19598, 72, 555),              # 256 x 256
+    ('dx', 17391, 3920, 196),            # 256 x 256, split
+    ('dw', 73, 73, 71),                  # 64 x 64
+    ('dw', 903, 71, 75),                 # 64 x 64, split
+    ('dw', 71, 195, 4139),               # 128 x 64
+    ('dw', 7152, 71, 280),               # 128 x 64, split
+    ('dw', 71, 1440, 4240),              # 128 x 128
+    ('dw', 11909, 1828, 71),             # 128 x 128, split
+    ('dw', 300, 4088, 4090),             # 256 x 256
+    ('dw', 10758, 137, 4242),            # 256 x 256, split
+    ('both', 73, 73, 71),                # one launch, dx in 64 x 64
+    ('both', 903, 71, 75),               # one launch, dx in 64 x 64, dw split
+    ('both', 201, 132, 4286),            # one launch, dx in 128 x 64
+    ('both', 7134, 77, 215),             # one launch, dx in 128 x 64, dw split
+    ('both', 16380, 2044, 2050),         # apart: dx in 128 x 128, dw in 256 x 256, split
+]
+TILES32 = [
+    ('forward', 76, 70, 314), ('forward', 19780, 129, 71), ('forward', 75, 3065, 1413),         # 64 x 64 split; 128 x 64; the same split
+    ('dx', 70, 71, 76), ('dx', 73, 290, 74), ('dx', 17770, 73, 130), ('dx', 2870, 1439, 72),    # 64 x 64, split; 128 x 64, split
+    ('dw', 70, 71, 76), ('dw', 301, 71, 71), ('dw', 70, 4803, 647), ('dw', 1439, 72, 3006),
+    ('both', 70, 71, 76), ('both', 301, 71, 71), ('both', 234, 160, 4900), ('both', 841, 74, 1293),
+]
+
+
+@pytest.mark.parametrize('dt,what,M,N,K', [(dt,) + t for dt in (BF, HF) for t in TILES16] + [(F32,) + t for t in TILES32])
+def test_every_kernel(dt, what, M, N, K):
+    from a2c_ppo_acktr import ops
+    x, w = rnd(1, M, K, dtype=dt), rnd(2, N, K, scale=1.5 / K ** 0.5, dtype=dt)
+    b, r, dy = rnd(3, N, scale=0.5, dtype=dt), rnd(4, M, N, dtype=dt), rnd(5, M, N, scale=0.1, dtype=dt)
+    pre = torch.empty(M, N, dtype=dt, device=DEV)
+    y = ops.linear_act_fwd(x, w, b, act='silu', residual=r, pre=pre)
+    ry, ty, slope, ts = linear64(x, w, b, 'silu', r)
+    check(y, (ry, ty), 'y')
+    if what == 'forward':
+        assert all(torch.equal(ops.linear_act_fwd(x, w, b, act='silu', residual=r), y) for _ in range(3))
+        return
+    need = dict(need_dx=what != 'dw', need_dw=what != 'dx', need_db=what != 'dx')
+    got = ops.linear_act_bwd(dy, x, w, pre=pre, act='silu', **need)
+    for name, t, ref in zip(('dx', 'dw', 'db'), got, linear_grads64(dy, x, w, slope, ts)):
+        if t is not None:
+            check(t, ref, name)
+    for _ in range(3):
+        again = ops.linear_act_bwd(dy, x, w, pre=pre, act='silu', **need)
+        assert all(p is None if q is None else torch.equal(p, q) for p, q in zip(again, got))
+
+
 def test_large_pre_activations():
     """tails of every activation: values far from zero"""
     for act in ACTS:
