@@ -82,8 +82,10 @@ def test_time_is_split_over_workgroups(T, N, H, dt):
     (150, 70, 974, BF), (150, 70, 974, HF),          # 4 waves, tiles of several sequences
     (150, 40, 973, BF), (150, 40, 973, F32), (300, 33, 1024, F32),       # one channel a lane, 4 waves
     (8200, 1, 512, BF), (8200, 1, 512, HF),          # two channels a lane, time split over workgroups, whole tiles
-    (4500, 5, 190, BF),                              # the same with tiles of several sequences
+    (4500, 5, 190, BF), (4500, 5, 190, HF),          # the same with tiles of several sequences
     (2100, 3, 77, F32), (2100, 3, 77, HF),           # one channel a lane, split, tiles of several sequences
+    (16, 64, 1024, BF), (16, 64, 1024, HF), (10, 70, 974, BF), (10, 70, 974, HF),        # two channels a lane, a wave
+    (50, 2, 64, BF), (50, 2, 64, HF), (12, 2, 64, BF), (12, 2, 64, HF),                  # one channel a lane, whole tiles, 4 waves and one
 ])
 def test_every_plan(T, N, H, dt):
     run(T, N, H, dt, shift=2.0)
@@ -299,6 +301,24 @@ def test_strides_that_need_64_bits(far, dt):
     g, v, m, h0, dout, dl = inputs(T, N, H, dt)
     out, dg, dv = spread(torch.zeros_like(dout)), spread(torch.zeros_like(dout)), spread(torch.zeros_like(dout))
     gs, vs, ds = spread(g), spread(v), spread(dout)
+    _, fin, saved = ops.gated_scan_fwd(gs, vs, h0, m, out=out, save=True)
+    _, _, dh0 = ops.gated_scan_bwd(ds, gs, vs, h0, m, saved=saved, dlast=dl, dgate=dg, dvalue=dv)
+    ref = scan64(g, v, h0, m, dout, dl)
+    for name, t in (('out', out), ('last', fin), ('dgate', dg), ('dvalue', dv), ('dh0', dh0)):
+        check(t, ref[name], name)
+
+
+@pytest.mark.parametrize('dt', [BF, HF, F32])
+@pytest.mark.parametrize('T', [9, 50, 130, 400])
+def test_sequences_gigabytes_apart(T, dt):
+    """64-bit offsets with a wave, with 4, with 8, and with the time split"""
+    from a2c_ppo_acktr import ops
+    N, H = 3, 40
+    e = torch.empty(0, dtype=dt).element_size()
+    spread = lambda t: torch.empty(N, (1 << 30) // e + 8, dtype=dt, device=DEV)[:, :T * H].view(N, T, H).transpose(0, 1).copy_(t)
+    g, v, m, h0, dout, dl = inputs(T, N, H, dt)
+    gs, vs, ds = spread(g), spread(v), spread(dout)
+    out, dg, dv = (spread(torch.zeros_like(dout)) for _ in range(3))
     _, fin, saved = ops.gated_scan_fwd(gs, vs, h0, m, out=out, save=True)
     _, _, dh0 = ops.gated_scan_bwd(ds, gs, vs, h0, m, saved=saved, dlast=dl, dgate=dg, dvalue=dv)
     ref = scan64(g, v, h0, m, dout, dl)

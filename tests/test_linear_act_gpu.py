@@ -111,8 +111,22 @@ TILES32 = [
     ('forward', 76, 70, 314), ('forward', 19780, 129, 71), ('forward', 75, 3065, 1413),         # 64 x 64 split; 128 x 64; the same split
     ('dx', 70, 71, 76), ('dx', 73, 290, 74), ('dx', 17770, 73, 130), ('dx', 2870, 1439, 72),    # 64 x 64, split; 128 x 64, split
     ('dw', 70, 71, 76), ('dw', 301, 71, 71), ('dw', 70, 4803, 647), ('dw', 1439, 72, 3006),
-    ('both', 70, 71, 76), ('both', 301, 71, 71), ('both', 234, 160, 4900), ('both', 841, 74, 1293),
+    ('both', 70, 71, 76), ('both', 301, 71, 71), ('both', 841, 74, 1293), ('both', 333, 4085, 4309),
 ]
+
+
+@pytest.mark.parametrize('dt', [BF, HF, F32])
+@pytest.mark.parametrize('act', ['none', 'gelu'])
+@pytest.mark.parametrize('M,N', [(1, 1), (777, 35), (5000, 264)])
+def test_bias_gradient_alone(M, N, act, dt):
+    from a2c_ppo_acktr import ops
+    x, w, dy = rnd(1, M, 24, dtype=dt), rnd(2, N, 24, scale=0.3, dtype=dt), rnd(3, M, N, dtype=dt)
+    pre = torch.empty(M, N, dtype=dt, device=DEV) if act != 'none' else None
+    ops.linear_act_fwd(x, w, act=act, pre=pre)
+    dx, dw, db = ops.linear_act_bwd(dy, x, w, pre=pre, act=act, need_dx=False, need_dw=False)
+    _, _, slope, ts = linear64(x, w, None, act)
+    assert dx is None and dw is None
+    check(db, linear_grads64(dy, x, w, slope, ts)[2], 'db')
 
 
 @pytest.mark.parametrize('dt,what,M,N,K', [(dt,) + t for dt in (BF, HF) for t in TILES16] + [(F32,) + t for t in TILES32])
