@@ -227,6 +227,68 @@ def test_writes_in_place_are_seen_by_autograd():
             y.sum().backward()
 
 
+@pytest.mark.parametrize('T,N', [(0, 3), (5, 0), (0, 0)])
+def test_no_steps_or_no_sequences(T, N):
+    from a2c_ppo_acktr.gated import GatedCore
+    core = GatedCore(8, 16).to(DEV, BF)
+    x, s0 = torch.zeros(T, N, 8, dtype=BF, device=DEV).requires_grad_(), rnd(1, N, 16).requires_grad_()
+    y, last = core(x, s0, torch.ones(T, N, 1, device=DEV))
+    assert y.shape == (T, N, 16) and last.shape == (N, 16) and (T or torch.equal(last, s0))
+    (y.sum(dtype=F32) + last.sum()).backward()
+    assert x.grad.shape == x.shape and (T or torch.equal(s0.grad, torch.ones_like(s0)))
+    assert all(p.grad is not None and not p.grad.any() for p in core.parameters())
+    assert core.step(torch.zeros(N, 8, dtype=BF, device=DEV), last.detach()).shape == (N, 16)
+
+
+@pytest.mark.parametrize('dt', [BF, F32])
+def test_gradients_into_rows_of_wider_tensors(dt):
+    from a2c_ppo_acktr import ops
+    M, N, K = 70, 40, 51
+    x, w, dy = rnd(1, M, K, dtype=dt), rnd(2, N, K, dtype=dt), rnd(3, M, N, dtype=dt)
+    want = ops.linear_act_bwd(dy, x, w)
+    big, vec = torch.full((M + 2, 2 * K + 3), 5.0, dtype=dt, device=DEV), torch.full((N + 2,), 5.0, dtype=dt, device=DEV)
+    ops.linear_act_bwd(dy, x, w, dx=big[1:M + 1, K:2 * K], db=vec[1:N + 1])
+    assert torch.equal(big[1:M + 1, K:2 * K], want[0]) and torch.equal(vec[1:N + 1], want[2])
+    big[1:M + 1, K:2 * K] = 5
+    vec[1:N + 1] = 5
+    assert bool((big == 5).all()) and bool((vec == 5).all())
+
+
+def test_streams_of_their_own():
+    """training steps of two cores on two streams at once, and what they give in turn on one"""
+    from a2c_ppo_acktr import algo
+    from a2c_ppo_acktr.gated import GatedCore
+    T, N, I, H = 300, 4, 40, 64
+
+    def make(seed):
+        torch.manual_seed(seed)
+        core = GatedCore(I, H).to(DEV, BF)
+        masters = [p.detach().float() for p in core.parameters()]
+        opt = algo.AdamW(masters, lr=1e-3, copies=list(core.parameters()), max_grad_norm=0.5, state_bits=8, seed=seed)
+        return core, masters, opt, rnd(seed, T, N, I, dtype=BF), (rnd(seed + 9, T, N) < 1.5).float()
+
+    def train(core, masters, opt, x, m):
+        y, last = core(x, None, m)
+        for p, g in zip(core.parameters(), torch.autograd.grad((y.float() ** 2).mean() + last.mean(), list(core.parameters()))):
+            p.grad = g
+        opt.step()
+    want = []
+    for seed in (1, 2):
+        job = make(seed)
+        for _ in range(4):
+            train(*job)
+        want.append([p.clone() for p in job[1]])
+    jobs, streams = [make(1), make(2)], [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for job, st in zip(jobs, streams):
+            with torch.cuda.stream(st):
+                train(*job)
+    torch.cuda.synchronize()
+    for job, w in zip(jobs, want):
+        assert all(torch.equal(p, q) for p, q in zip(job[1], w))
+
+
 def test_given_outputs_are_marked_as_changed():
     from a2c_ppo_acktr import ops
     x, w, dy = rnd(1, 6, 8), rnd(2, 4, 8), rnd(3, 6, 4)
@@ -402,6 +464,27 @@ def test_ppo_adamw_without_recurrence(kind):
         out.append(pol.flat_params.clone())
     # 12 steps of at most lr each; the two kernels round differently, and a step's direction follows the sign of tiny gradients
     assert float((out[0] - out[1]).abs().max()) < 12 * 3e-4 * 0.5 and rel(out[0], out[1].double()) < 1e-4
+
+
+@pytest.mark.parametrize('rec', ['gated', False])
+def test_ppo_adamw_clip_changes(rec):
+    """the agent's clip norm may be None, and may change between updates; replays and plain launches agree"""
+    from a2c_ppo_acktr import algo
+    from a2c_ppo_acktr.model import Policy
+    res = []
+    for graph in (True, False):
+        torch.manual_seed(5)
+        pol = Policy((11,), Box(3), base_kwargs={'recurrent': rec}).to(DEV)
+        agent = algo.PPO(pol, 0.2, 2, 2, 0.5, 0.01, lr=3e-4, eps=1e-5, max_grad_norm=None, weight_decay=0.01)
+        agent.use_graph = graph
+        rs = make_storage('mlp', 8, 4, pol.recurrent_hidden_state_size)
+        for it, clip in enumerate((None, None, None, 0.1, 0.1, 0.1, None, None, None)):
+            agent.max_grad_norm = clip
+            agent.optimizer.param_groups[0]['lr'] = 3e-4 / (it + 1)
+            torch.manual_seed(100 + it)
+            agent.update(rs)
+        res.append(pol.flat_params.clone())
+    assert torch.equal(*res)
 
 
 def test_a2c_updates():
