@@ -9,8 +9,8 @@
 // it is exact) and a value is sign + 4 exponent + 3 mantissa bits (m) or 5 exponent + 3 mantissa bits (v; a running mean of squares
 // spans twice the octaves).  Rounding is stochastic: with b2 = 0.999 a step changes v by at most 0.1 % of its distance to g^2, far
 // below half a code's spacing of 6 %, so rounding to nearest would freeze v; rounding up with the probability of the cut-off bits
-// keeps its expectation.  The random bits are a function of (seed, step, element), so runs repeat.  A positive v never becomes 0:
-// m may survive where v would not, and m / eps is no step.
+// keeps its expectation.  The random bits are a function of (seed, step, element), so runs repeat.  A positive v never becomes 0 (but in a
+// block that lies below 2^-126): m may survive where v would not, and m / eps is no step.
 #include "half_types.hpp"
 
 #pragma clang fp contract(off)
@@ -33,6 +33,7 @@ struct AwState {
     double partial[AW_PARTIALS];
 };
 
+// 32-bit mixing function: multiply and xor-shift with the low-bias constants that C. Wellons published (2018)
 __device__ __forceinline__ unsigned mix32(unsigned x) {
     x = (x ^ (x >> 16)) * 0x7feb352du;
     x = (x ^ (x >> 15)) * 0x846ca68bu;

@@ -259,7 +259,7 @@ struct Scan {
 
 // --------------------------------------------------------------------------------------------------------- forward
 // AGG: only the block's composition is formed (first pass of a time split).  Bound by memory: bf16, 2048 x 32 x 1024 in 89 us (4.5 TB/s
-// over two reads and a write); 65536 x 1 x 512, split, 29 us for the compositions and 38 for the states.  With two channels a lane the
+// over two reads and a write); 65536 x 1 x 512, split, 30 us for the compositions and 39 for the states.  With two channels a lane the
 // registers are kept to 128, which lets two workgroups of 8 waves share a CU (that case, forward + backward, 171 us against 181 with 133).
 template <class T, int V, int NW, int MODE, bool AGG>
 __global__ __launch_bounds__(NW * 64, V == 2 && (NW == 8 || MODE == SCAN_WHOLE) ? 4 : 1) void scan_fwd_kernel(const ScanArgs p) {
@@ -339,7 +339,8 @@ __global__ __launch_bounds__(NW * 64, V == 2 && (NW == 8 || MODE == SCAN_WHOLE) 
 
 // --------------------------------------------------------------------------------------------------------- backward
 // The states are formed again from the saved ones, in fp32, rather than read from the rounded output.  Bound by memory: bf16,
-// 2048 x 32 x 1024 in 152 us (4.4 TB/s over three reads and two writes); 65536 x 1 x 512, split, 27 + 77 us.
+// 2048 x 32 x 1024 in 152 us (4.4 TB/s over three reads and two writes); 65536 x 1 x 512, split, 31 + 77 us.  With two
+// channels a lane the registers are kept to 256, two waves a SIMD, for a few spilled ones (forward + backward, 600 x 36 x 974 fp16 116 -> 112 us).
 template <class T, int V, int NW, int MODE, bool AGG>
 __global__ __launch_bounds__(NW * 64, V == 2 ? 2 : 1) void scan_bwd_kernel(const ScanArgs p) {
     typedef Scan<T, V, NW, MODE> S;
