@@ -130,11 +130,9 @@ class AdamW(object):
         self._tensors.copy_(torch.frombuffer(bytearray(bytes(rows)), dtype=torch.uint8))
         self._seen = seen
 
-    def prepare(self):
-        """Brings the device side up to date with the parameter list and the hyperparameters: outside a graph capture, and before a
-        replay when a hyperparameter changed."""
-        g = self.param_groups[0]
-        dev = g['params'][0].device
+    def _place(self):
+        """Moments, tables and device state, made where the parameters are when they are first needed."""
+        dev = self.params[0].device
         if self._dev != dev:
             if dev.type != 'cuda':
                 raise RuntimeError('AdamW: parameters must live on the MI355X device (got %s): this package has no CPU path' % dev)
@@ -142,6 +140,12 @@ class AdamW(object):
                 raise RuntimeError('AdamW: the parameters moved to %s; build a new optimiser' % dev)
             with torch.no_grad():
                 self._allocate(dev)
+
+    def prepare(self):
+        """Brings the device side up to date with the parameter list and the hyperparameters: outside a graph capture, and before a
+        replay when a hyperparameter changed."""
+        g = self.param_groups[0]
+        self._place()
         b1, b2 = g['betas']
         hyper = (float(g['lr']), float(b1), float(b2), float(g['eps']), float(g['weight_decay']), float(g['max_grad_norm'] or 0.0))
         if hyper != self._hyper:
@@ -179,8 +183,7 @@ class AdamW(object):
     def moments(self):
         """(m, v) as fp32, one value per element of the state buffers (tensor k from offsets()[k] on): the buffers themselves, or, of
         8-bit moments, the values they stand for."""
-        if self._dev is None:
-            self.prepare()
+        self._place()
         if self.state_bits == 32:
             return self.mom1, self.mom2
         m, v = torch.empty(self._total, dtype=f32, device=self._dev), torch.empty(self._total, dtype=f32, device=self._dev)
@@ -190,13 +193,11 @@ class AdamW(object):
 
     def offsets(self):
         """Where each tensor's moments start in the state buffers."""
-        if self._dev is None:
-            self.prepare()
+        self._place()
         return list(self._offs)
 
     def state_dict(self):
-        if self._dev is None:
-            self.prepare()
+        self._place()
         own = lambda t: None if t is None else t.clone()
         return dict(step=self.steps_done(), seed=self.seed, state_bits=self.state_bits, mom1=own(self.mom1), mom2=own(self.mom2),
                     scales=own(self.scales), hyper={k: v for k, v in self.param_groups[0].items() if k != 'params'})
@@ -204,8 +205,7 @@ class AdamW(object):
     def load_state_dict(self, sd):
         if sd['state_bits'] != self.state_bits:
             raise ValueError('AdamW: the state holds %d-bit moments, this optimiser %d' % (sd['state_bits'], self.state_bits))
-        if self._dev is None:
-            self._allocate(self.params[0].device)
+        self._place()
         if sd['mom1'].numel() != self._total:
             raise ValueError('AdamW: the state belongs to other parameters')
         self.param_groups[0].update(sd['hyper'])

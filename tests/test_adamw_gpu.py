@@ -347,6 +347,26 @@ def test_state_round_trip(bits, tmp_path):
 
 
 @pytest.mark.parametrize('bits', [32, 8])
+def test_state_before_the_first_step(bits):
+    """an optimiser is saved, looked into and restored before there is any gradient"""
+    from a2c_ppo_acktr import algo
+    ps = [rnd(1, 300).requires_grad_(), rnd(2, 5, 7).requires_grad_()]
+    opt = algo.AdamW(ps, state_bits=bits, seed=3, **HP)
+    assert opt.offsets() == [0, 512] and not any(t.any() for t in opt.moments())
+    sd = opt.state_dict()
+    assert sd['step'] == 0
+    qs = [p.detach().clone().requires_grad_() for p in ps]
+    other = algo.AdamW(qs, state_bits=bits, lr=1.0)
+    other.load_state_dict(sd)
+    with pytest.raises(RuntimeError, match='no gradient'):
+        opt.step()
+    for k, (p, q) in enumerate(zip(ps, qs)):
+        p.grad, q.grad = rnd(10 + k, *p.shape), rnd(10 + k, *p.shape)
+    opt.step(), other.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps, qs))
+
+
+@pytest.mark.parametrize('bits', [32, 8])
 @pytest.mark.parametrize('clip', [None, 0.5])
 def test_captured_and_replayed(bits, clip):
     from a2c_ppo_acktr import algo, ops

@@ -25,6 +25,15 @@ def test_no_cpu_path():
             f()
 
 
+def test_adamw_state_has_no_cpu_path():
+    from a2c_ppo_acktr import algo
+    opt = algo.AdamW([torch.zeros(8)], lr=1.0)
+    sd = dict(step=1, seed=0, state_bits=32, mom1=torch.zeros(256), mom2=torch.zeros(256), scales=None, hyper={})
+    for f in (opt.state_dict, opt.moments, opt.offsets, opt.prepare, lambda: opt.load_state_dict(sd)):
+        with pytest.raises(RuntimeError, match='no CPU path'):
+            f()
+
+
 def test_linear_entry_arguments():
     L, one = lib(), ctypes.c_void_p(256)
     fwd = lambda M=4, N=8, K=8, ldx=8, ldw=8, ldy=8, dt=1, act=0, x=one, ws=one, nb=1 << 20: L.acktr_linear_act_fwd(
