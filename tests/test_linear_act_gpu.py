@@ -2,7 +2,8 @@
 import pytest
 import torch
 
-from gated_refs import ACTS, E32, EPS, TINY, act64, check, linear64, linear_grads64
+from gated_refs import ACTS, check, linear64, linear_grads64
+from gated_refs import E32, EPS, TINY, act64
 
 pytestmark = pytest.mark.gpu
 DEV = 'cuda:0'
